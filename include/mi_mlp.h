@@ -205,6 +205,86 @@ int mi_convert_f32_to_bf16(void* dst_bf16, const float* src, size_t n, void* str
 int mi_convert_bf16_to_f32(float* dst, const void* src_bf16, size_t n, void* stream);
 
 /* ------------------------------------------------------------------------------------------ */
+/* classifier loss on device pointers                                                         */
+
+/*
+ * Softmax cross entropy of a linear classifier over V classes, without ever holding the M x V logits:
+ *   z = X[M x K] * W[V x K]^T (+ bias[V])
+ *   lse[i]  = log sum_j exp z_ij
+ *   loss[i] = lse[i] - z_i,target[i]
+ * A target outside [0, V) marks a row that does not count (padding): its loss is 0 and its gradient
+ * zero; its lse is still written.  Infinite logits mean what they mean in the formula: -inf (a bias of
+ * -inf, say) is a class of probability zero, +inf or NaN makes the row's lse +inf or NaN.
+ * Stands beside mi_l2_loss_static; no counterpart in the reference, whose harness has the L2 loss only.
+ *   dtype MI_BF16: X and W bf16, MFMA products with fp32 accumulation; MI_F32: X and W fp32.
+ *   bias, loss, lse, dloss, dbias: fp32.  target: 32-bit integers.  bias may be NULL.
+ *   M, V, K: 1 .. 2097152.  Any strides and alignment of the element type; 16-byte aligned rows and
+ *   K a multiple of 64 are read in place, others are copied into the workspace first.
+ * workspace: device memory, 256-byte aligned, at least what mi_xent_workspace says for the same dtype,
+ * M, V and K.  Its contents do not matter before a call and mean nothing after it; calls that may run
+ * at the same time need one each.  Nothing is allocated and nothing synchronises, so the calls can be
+ * captured into a graph once each has run outside a capture on that device.  Results do not depend on
+ * timing: the same inputs give the same bits.
+ */
+int mi_xent_workspace(int dtype, int M, int V, int K, size_t* forward_bytes, size_t* backward_bytes);
+int mi_xent_forward(int dtype, int M, int V, int K, const void* X, int ldx, const void* W, int ldw,
+                    const float* bias, const int* target, float* loss, float* lse, void* workspace,
+                    size_t workspace_bytes, void* stream);
+/*
+ * The gradient, from lse as the forward call wrote it:
+ *   g_ij = dloss[i] * (exp(z_ij - lse[i]) - [j = target[i]])      (0 where the row does not count)
+ *   dX[M x K] = g * W       dW[V x K] = g^T * X       dbias[V] = column sums of g
+ * dloss = NULL stands for ones; for the mean over the rows that count, fill it with their 1 / count.
+ * All three results are written, not added to; dbias may be NULL.  The outputs may not overlap the inputs.
+ * Wt (MI_BF16 only, may be NULL): W^T [K x V] with leading dimension ldwt, the copy that
+ * mi_reduce_sgd_bf16t_raw and mi_ortho_update_raw write; without it, or where its rows are not 16-byte
+ * aligned, the call makes the copy itself, piece by piece.
+ * dX has the dtype of X.  dW is bf16 (dw_dtype = MI_BF16) or fp32 (MI_F32; always for MI_F32 models).
+ * bf16: g is rounded to bf16 (half a step, 2^-9 of each term) before the two products that read it,
+ * like every dY of the framework's bf16 models; dbias is summed before that rounding.
+ */
+int mi_xent_backward(int dtype, int M, int V, int K, const void* X, int ldx, const void* W, int ldw,
+                     const void* Wt, int ldwt, const float* bias, const int* target, const float* lse,
+                     const float* dloss, void* dX, int lddx, int dw_dtype, void* dW, int lddw,
+                     float* dbias, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------------------ */
+/* orthogonalised update on device pointers                                                   */
+
+/*
+ * O = G with its singular values driven towards one, the direction of steepest descent under the
+ * spectral norm:  X_0 = G / |G|_F, then `steps` (1 .. 16; 5 is customary) times
+ *   A = X X^T,  X <- a X + (b A + c A^2) X,   a, b, c = 3.4445, -4.7750, 2.0315
+ * (on the transposed matrix where rows > cols), which leaves singular values of G that are not tiny
+ * against |G|_F between about 0.7 and 1.2.  `batch` matrices of one shape, strideG / strideO elements
+ * apart; G is fp32 (in_dtype = MI_F32) or bf16, O is bf16.  The products run in fp16 with fp32
+ * accumulation and the iterate is kept in fp32: O is off by about 1e-3 of |O|_F before its rounding.
+ * G = 0 gives O = 0; a G with an infinity or NaN gives NaN throughout.  O may be G itself (bf16, same
+ * strides).  rows, cols: 1 .. 65536, batch: 1 .. 4096.
+ * workspace as for mi_xent_forward, sized by mi_ortho_workspace for the same batch, rows and cols.
+ */
+int mi_ortho_workspace(int batch, int rows, int cols, size_t* bytes);
+int mi_orthogonalize(int in_dtype, int batch, int rows, int cols, const void* G, int ldg, long long strideG,
+                     void* O, int ldo, long long strideO, int steps, void* workspace,
+                     size_t workspace_bytes, void* stream);
+/*
+ * The update of `batch` weight matrices of one shape with it, gradient reduce included:
+ *   g = G[0] + ... + G[R-1] (replica_stride floats apart)      momentum <- mu momentum + g
+ *   u = nesterov ? g + mu momentum : momentum                  O = orthogonalised u, as above
+ *   W <- (1 - lr decay) W - lr scale O
+ * and, unless NULL, W_bf16 = W and Wt_bf16 = W^T rounded to bf16: what mi_reduce_sgd_bf16t_raw is for
+ * plain SGD.  Every matrix is dense [rows x cols] (Wt_bf16 [cols x rows]); consecutive ones are
+ * layer_stride elements apart in W, W_bf16, Wt_bf16, momentum and each replica of G alike, the layout
+ * of the parameter arena of a model with equal layers.  momentum: zeros before the first call.
+ * scale is the caller's convention for the step length, e.g. 0.2 sqrt(max(rows, cols)) for an update
+ * of root mean square 0.2 lr, or sqrt(max(1, rows / cols)).
+ */
+int mi_ortho_update_raw(int batch, int rows, int cols, float* W, void* W_bf16, void* Wt_bf16,
+                        float* momentum, const float* G, size_t layer_stride, size_t replica_stride,
+                        int R, float lr, float scale, float decay, float mu, int nesterov, int steps,
+                        void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------------------------ */
 /* handle API: the whole model resident in HBM                                                */
 
 typedef struct mi_mlp mi_mlp;

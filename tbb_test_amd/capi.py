@@ -88,6 +88,17 @@ SIGNATURES = {
     "mi_loss_backward": [c_void_p],
     "mi_mlp_get_loss": [c_void_p, POINTER(c_double), POINTER(c_double)],
     "mi_mlp_trace_step": [c_void_p, c_float, c_char_p],
+    "mi_xent_workspace": [c_int, c_int, c_int, c_int, POINTER(c_size_t), POINTER(c_size_t)],
+    "mi_xent_forward": [c_int, c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p,
+                        c_void_p, c_void_p, c_size_t, c_void_p],
+    "mi_xent_backward": [c_int, c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p,
+                         c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p,
+                         c_size_t, c_void_p],
+    "mi_ortho_workspace": [c_int, c_int, c_int, POINTER(c_size_t)],
+    "mi_orthogonalize": [c_int, c_int, c_int, c_int, c_void_p, c_int, c_longlong, c_void_p, c_int, c_longlong, c_int,
+                         c_void_p, c_size_t, c_void_p],
+    "mi_ortho_update_raw": [c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_size_t,
+                            c_int, c_float, c_float, c_float, c_float, c_int, c_int, c_void_p, c_size_t, c_void_p],
     "mi_l2_loss_static": [c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p],
 }
 

@@ -912,6 +912,119 @@ int mi_convert_bf16_to_f32(float* dst, const void* src, size_t n, void* stream) 
   return MI_OK;
 }
 
+// ---- classifier loss ----------------------------------------------------------------------------
+
+static int check_workspace(const void* workspace, size_t have, size_t need) {
+  MI_REQUIRE(workspace != nullptr, "null workspace");
+  MI_REQUIRE((reinterpret_cast<uintptr_t>(workspace) & 255) == 0, "the workspace must be 256-byte aligned");
+  MI_REQUIRE(have >= need, "workspace of %zu bytes, %zu needed", have, need);
+  return MI_OK;
+}
+
+static int check_xent(int dtype, int M, int V, int K) {
+  constexpr int kMost = 1 << 21;
+  MI_REQUIRE(dtype == MI_F32 || dtype == MI_BF16, "dtype must be MI_F32 or MI_BF16 (got %d)", dtype);
+  MI_REQUIRE(M >= 1 && V >= 1 && K >= 1 && M <= kMost && V <= kMost && K <= kMost,
+             "M, V and K must be 1 .. %d (got %d, %d, %d)", kMost, M, V, K);
+  return MI_OK;
+}
+
+int mi_xent_workspace(int dtype, int M, int V, int K, size_t* forward_bytes, size_t* backward_bytes) {
+  if (int rc = check_xent(dtype, M, V, K)) return rc;
+  if (forward_bytes) *forward_bytes = mi::xent_forward_bytes(dtype == MI_BF16, M, V, K);
+  if (backward_bytes) *backward_bytes = mi::xent_backward_bytes(dtype == MI_BF16, M, V, K);
+  return MI_OK;
+}
+
+int mi_xent_forward(int dtype, int M, int V, int K, const void* X, int ldx, const void* W, int ldw, const float* bias,
+                    const int* target, float* loss, float* lse, void* workspace, size_t workspace_bytes, void* stream) {
+  if (int rc = check_xent(dtype, M, V, K)) return rc;
+  MI_REQUIRE(X && W && target && loss && lse, "null pointer");
+  MI_REQUIRE(ldx >= K && ldw >= K, "ldx %d, ldw %d must be >= K %d", ldx, ldw, K);
+  const bool bf16 = dtype == MI_BF16;
+  if (int rc = check_workspace(workspace, workspace_bytes, mi::xent_forward_bytes(bf16, M, V, K))) return rc;
+  hipStream_t s = as_stream(stream);
+  const hipError_t e = bf16 ? mi::xent_forward_bf16(M, V, K, (const uint16_t*)X, ldx, (const uint16_t*)W, ldw, bias, target,
+                                                    loss, lse, workspace, s)
+                            : mi::xent_forward_f32(M, V, K, (const float*)X, ldx, (const float*)W, ldw, bias, target, loss,
+                                                   lse, workspace, s);
+  if (e != hipSuccess) return hip_fail(e, "mi_xent_forward launch");
+  return MI_OK;
+}
+
+int mi_xent_backward(int dtype, int M, int V, int K, const void* X, int ldx, const void* W, int ldw, const void* Wt,
+                     int ldwt, const float* bias, const int* target, const float* lse, const float* dloss, void* dX,
+                     int lddx, int dw_dtype, void* dW, int lddw, float* dbias, void* workspace, size_t workspace_bytes,
+                     void* stream) {
+  if (int rc = check_xent(dtype, M, V, K)) return rc;
+  MI_REQUIRE(X && W && target && lse && dX && dW, "null pointer");
+  MI_REQUIRE(ldx >= K && ldw >= K && lddx >= K && lddw >= K, "ldx %d, ldw %d, lddx %d, lddw %d must be >= K %d", ldx, ldw,
+             lddx, lddw, K);
+  const bool bf16 = dtype == MI_BF16;
+  MI_REQUIRE(dw_dtype == MI_F32 || (bf16 && dw_dtype == MI_BF16), "dw_dtype must be MI_F32%s (got %d)",
+             bf16 ? " or MI_BF16" : " for an fp32 model", dw_dtype);
+  MI_REQUIRE(!Wt || bf16, "Wt is for bf16 models");
+  MI_REQUIRE(!Wt || ldwt >= V, "ldwt %d < V %d", ldwt, V);
+  if (int rc = check_workspace(workspace, workspace_bytes, mi::xent_backward_bytes(bf16, M, V, K))) return rc;
+  hipStream_t s = as_stream(stream);
+  const hipError_t e =
+      bf16 ? mi::xent_backward_bf16(M, V, K, (const uint16_t*)X, ldx, (const uint16_t*)W, ldw, (const uint16_t*)Wt, ldwt, bias,
+                                    target, lse, dloss, (uint16_t*)dX, lddx, dw_dtype == MI_BF16, dW, lddw, dbias, workspace, s)
+           : mi::xent_backward_f32(M, V, K, (const float*)X, ldx, (const float*)W, ldw, bias, target, lse, dloss, (float*)dX,
+                                   lddx, (float*)dW, lddw, dbias, workspace, s);
+  if (e != hipSuccess) return hip_fail(e, "mi_xent_backward launch");
+  return MI_OK;
+}
+
+// ---- orthogonalised update ----------------------------------------------------------------------
+
+static int check_ortho(int batch, int rows, int cols) {
+  MI_REQUIRE(batch >= 1 && batch <= 4096, "batch must be 1 .. 4096 (got %d)", batch);
+  MI_REQUIRE(rows >= 1 && cols >= 1 && rows <= 65536 && cols <= 65536, "rows and cols must be 1 .. 65536 (got %d, %d)", rows, cols);
+  return MI_OK;
+}
+
+int mi_ortho_workspace(int batch, int rows, int cols, size_t* bytes) {
+  if (int rc = check_ortho(batch, rows, cols)) return rc;
+  MI_REQUIRE(bytes != nullptr, "null result pointer");
+  *bytes = mi::ortho_bytes(batch, rows, cols);
+  return MI_OK;
+}
+
+int mi_orthogonalize(int in_dtype, int batch, int rows, int cols, const void* G, int ldg, long long strideG, void* O,
+                     int ldo, long long strideO, int steps, void* workspace, size_t workspace_bytes, void* stream) {
+  MI_REQUIRE(in_dtype == MI_F32 || in_dtype == MI_BF16, "in_dtype must be MI_F32 or MI_BF16 (got %d)", in_dtype);
+  if (int rc = check_ortho(batch, rows, cols)) return rc;
+  MI_REQUIRE(steps >= 1 && steps <= 16, "steps must be 1 .. 16 (got %d)", steps);
+  MI_REQUIRE(G && O, "null pointer");
+  MI_REQUIRE(ldg >= cols && ldo >= cols, "ldg %d, ldo %d must be >= cols %d", ldg, ldo, cols);
+  MI_REQUIRE(batch == 1 || strideO >= (long long)(rows - 1) * ldo + cols, "strideO overlaps matrices");
+  MI_REQUIRE(batch == 1 || strideG >= 0, "negative strideG");
+  if (int rc = check_workspace(workspace, workspace_bytes, mi::ortho_bytes(batch, rows, cols))) return rc;
+  const hipError_t e = mi::orthogonalize(in_dtype == MI_BF16, batch, rows, cols, G, ldg, strideG, (uint16_t*)O, ldo, strideO,
+                                         steps, workspace, as_stream(stream));
+  if (e != hipSuccess) return hip_fail(e, "mi_orthogonalize launch");
+  return MI_OK;
+}
+
+int mi_ortho_update_raw(int batch, int rows, int cols, float* W, void* W_bf16, void* Wt_bf16, float* momentum,
+                        const float* G, size_t layer_stride, size_t replica_stride, int R, float lr, float scale,
+                        float decay, float mu, int nesterov, int steps, void* workspace, size_t workspace_bytes,
+                        void* stream) {
+  if (int rc = check_ortho(batch, rows, cols)) return rc;
+  MI_REQUIRE(steps >= 1 && steps <= 16, "steps must be 1 .. 16 (got %d)", steps);
+  MI_REQUIRE(R >= 1, "R must be at least 1 (got %d)", R);
+  MI_REQUIRE(W && momentum && G, "null pointer");
+  const size_t n = (size_t)rows * cols;
+  MI_REQUIRE(batch == 1 || layer_stride >= n, "layer_stride %zu < rows * cols %zu", layer_stride, n);
+  MI_REQUIRE(R == 1 || replica_stride >= n, "replica_stride %zu < rows * cols %zu", replica_stride, n);
+  if (int rc = check_workspace(workspace, workspace_bytes, mi::ortho_bytes(batch, rows, cols))) return rc;
+  const hipError_t e = mi::ortho_update(batch, rows, cols, W, (uint16_t*)W_bf16, (uint16_t*)Wt_bf16, momentum, G, layer_stride,
+                                        replica_stride, R, lr, scale, decay, mu, nesterov, steps, workspace, as_stream(stream));
+  if (e != hipSuccess) return hip_fail(e, "mi_ortho_update_raw launch");
+  return MI_OK;
+}
+
 // ---- handle -------------------------------------------------------------------------------------
 
 int mi_mlp_create(mi_mlp** out, int L, const int* nfeatures, int batch_per_replica, int R, int dtype,

@@ -149,6 +149,30 @@ hipError_t rowsum_bf16(int batch, int rows, int cols, const uint16_t* src, int l
 // dst[0..bytes) = src[0..bytes) on the device (16-byte aligned: own kernel; else the runtime's copy)
 hipError_t device_copy(void* dst, const void* src, size_t bytes, hipStream_t s);
 
+// xent.hip: softmax cross entropy of a linear classifier, see the operator's description there.  `ws`
+// holds xent_*_bytes; rows whose target is outside [0, V) do not count.
+size_t xent_forward_bytes(bool bf16, int M, int V, int K);
+size_t xent_backward_bytes(bool bf16, int M, int V, int K);
+hipError_t xent_forward_bf16(int M, int V, int K, const uint16_t* X, int ldx, const uint16_t* W, int ldw, const float* bias,
+                             const int* target, float* loss, float* lse, void* ws, hipStream_t s);
+hipError_t xent_backward_bf16(int M, int V, int K, const uint16_t* X, int ldx, const uint16_t* W, int ldw,
+                              const uint16_t* Wt, int ldwt, const float* bias, const int* target, const float* lse,
+                              const float* dloss, uint16_t* dX, int lddx, bool dw_bf16, void* dW, int lddw, float* db,
+                              void* ws, hipStream_t s);
+hipError_t xent_forward_f32(int M, int V, int K, const float* X, int ldx, const float* W, int ldw, const float* bias,
+                            const int* target, float* loss, float* lse, void* ws, hipStream_t s);
+hipError_t xent_backward_f32(int M, int V, int K, const float* X, int ldx, const float* W, int ldw, const float* bias,
+                             const int* target, const float* lse, const float* dloss, float* dX, int lddx, float* dW,
+                             int lddw, float* db, void* ws, hipStream_t s);
+
+// ortho.hip: Newton-Schulz orthogonalisation of a matrix and the weight update built on it.
+size_t ortho_bytes(int batch, int rows, int cols);
+hipError_t orthogonalize(bool bf16, int batch, int rows, int cols, const void* G, int ldg, long long strideG, uint16_t* O,
+                         int ldo, long long strideO, int steps, void* ws, hipStream_t s);
+hipError_t ortho_update(int batch, int rows, int cols, float* W, uint16_t* W16, uint16_t* Wt16, float* momentum,
+                        const float* G, size_t layer_stride, size_t replica_stride, int R, float lr, float scale,
+                        float decay, float mu, int nesterov, int steps, void* ws, hipStream_t s);
+
 hipError_t convert_f32_to_bf16(uint16_t* dst, const float* src, size_t n, hipStream_t s);
 hipError_t convert_bf16_to_f32(float* dst, const uint16_t* src, size_t n, hipStream_t s);
 

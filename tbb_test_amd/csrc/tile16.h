@@ -1,0 +1,226 @@
+// Building block of the loss and update operators: one tile of C = A[M,K] * B[N,K]^T on 16-bit
+// operands (bf16 or fp16), both K-contiguous, fp32 accumulation on v_mfma_f32_16x16x32, handed to an
+// epilogue that the operator supplies.  Used by xent.hip and ortho.hip.
+//
+// K is a multiple of 64 and rows start at multiples of 16 bytes (callers pack operands that do not);
+// M and N are arbitrary: tile rows behind the last one read the last one again, and the epilogue drops
+// what does not belong to the result.
+//
+// Orientation, as in gemm_bf16_x32.hip: the register-side index of the 16 x 16 result block is n, the
+// lane-side index is m, and the rows of the B tile are dealt to the four n blocks of a wavefront's 64
+// columns so that a lane holds two runs of eight consecutive columns of one row:
+//   lane (q = lane / 16, l = lane % 16), block row jq, half h, element e
+//     ->  row 16 jq + l,  column 32 h + 8 q + e.
+#pragma once
+#include "gemm_bf16_common.h"
+
+namespace mi {
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+
+constexpr int TILE16_MAX_LD = 1 << 22;  // 2 * 256 rows * this many elements: 32-bit byte offsets
+
+struct Tile16 {
+  const u16* A;
+  const u16* B;
+  long long batchA, batchB;  // elements between the operands of consecutive batch entries
+  int lda, ldb, M, N, K;
+  int tiles_m, tiles_n;
+  int splits;     // the K steps are dealt to this many workgroups per tile; blockIdx.z = entry * splits + split
+  int symmetric;  // only tiles with tile_m >= tile_n are launched (square results, BM == BN)
+};
+
+// Two values rounded to nearest even, packed (low half first).
+template <bool F16>
+__device__ __forceinline__ unsigned pack16(float lo, float hi) {
+  const f32x2 v = {lo, hi};
+  if constexpr (F16) return __builtin_bit_cast(unsigned, __builtin_convertvector(v, f16x2));
+  else return __builtin_bit_cast(unsigned, __builtin_convertvector(v, bf16x2));
+}
+__device__ __forceinline__ float f16_lo(unsigned v) { return (float)__builtin_bit_cast(f16x2, v)[0]; }
+__device__ __forceinline__ float f16_hi(unsigned v) { return (float)__builtin_bit_cast(f16x2, v)[1]; }
+
+// Workgroup -> tile.  Workgroups go to the 8 XCDs round-robin; each XCD gets one contiguous range of an
+// order in which neighbours share operand panels: bands of eight tile rows, walked column by column (32
+// workgroups of an XCD in flight share eight A panels and four B panels), or the rows of the lower
+// triangle one after another.
+__device__ __forceinline__ void tile16_of_workgroup(const Tile16& p, int id, int total, int& tm, int& tn) {
+  const int xcd = id & 7, rest = total & 7;
+  id = xcd * (total >> 3) + (xcd < rest ? xcd : rest) + (id >> 3);
+  if (p.symmetric) {
+    tm = (int)((__builtin_sqrtf(8.0f * (float)id + 1.0f) - 1.0f) * 0.5f);
+    while (tm * (tm + 1) / 2 > id) --tm;  // the root is good to a unit only
+    while ((tm + 1) * (tm + 2) / 2 <= id) ++tm;
+    tn = id - tm * (tm + 1) / 2;
+    return;
+  }
+  const int band = id / (8 * p.tiles_n), within = id - band * 8 * p.tiles_n;
+  const int height = p.tiles_m - band * 8 < 8 ? p.tiles_m - band * 8 : 8;
+  tn = within / height;
+  tm = band * 8 + within - tn * height;
+}
+
+// Transposed store of a wavefront's WTM x 64 packed results: dst[col][row], `ld` elements per column,
+// dst at the first row and column.  32 columns at a time through `stage` (32 * (2 WTM + 8) bytes of LDS
+// private to the wavefront).  Neighbouring lanes hold neighbouring rows: one exchange with lane ^ 1 turns
+// a register (columns 2k, 2k+1 of a row) into rows 2p, 2p+1 of one column.
+template <int QB>
+__device__ __forceinline__ void store_transposed(u16* __restrict__ dst, size_t ld, const u32x4 (&pk)[QB][2], int lane,
+                                                 unsigned char* stage) {
+  constexpr int COL = QB * 16 * 2 + 8;
+  const int l16 = lane & 15, q = lane >> 4;
+  const unsigned sel = (lane & 1) ? 0x07060302u : 0x01000504u;  // bytes of {own (4-7), partner (0-3)}
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+#pragma unroll
+    for (int jq = 0; jq < QB; ++jq)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const unsigned own = pk[jq][h][k];
+        const unsigned partner = (unsigned)__builtin_amdgcn_update_dpp(0, (int)own, 0xB1, 0xf, 0xf, false);  // lane ^ 1
+        *reinterpret_cast<unsigned*>(stage + (8 * q + 2 * k + (lane & 1)) * COL + (16 * jq + (l16 & 14)) * 2) =
+            __builtin_amdgcn_perm(own, partner, sel);
+      }
+    constexpr int CHUNKS = QB * 2;  // 16-byte chunks per column
+#pragma unroll
+    for (int i = lane; i < 32 * CHUNKS; i += 64) {
+      const int c = i / CHUNKS, piece = i % CHUNKS;
+      const u32x2 lo = *reinterpret_cast<const u32x2*>(stage + c * COL + piece * 16);
+      const u32x2 up = *reinterpret_cast<const u32x2*>(stage + c * COL + piece * 16 + 8);
+      *reinterpret_cast<u32x4*>(dst + (size_t)(32 * h + c) * ld + piece * 8) = u32x4{lo[0], lo[1], up[0], up[1]};
+    }
+  }
+}
+
+// The tile kernel.  WM x WN wavefronts of (BM / WM) x 64; a ring of STAGES LDS buffers filled by direct
+// global -> LDS loads, one barrier per K step of 64.  At the top of step t the tile of step t has landed
+// (the counter retires loads in order) and every wavefront is done with the buffer of step t - 1, which
+// takes the tile of step t + STAGES - 1.
+template <bool F16, int BM, int BN, int WM, int WN, int STAGES, class Epi>
+struct TileKernel {
+  static constexpr int NW = WM * WN, QB = BM / WM / 16, BK = 64;
+  static constexpr int A_ELEMS = BM * BK, B_ELEMS = BN * BK, BUF = A_ELEMS + B_ELEMS;
+  static constexpr int NIA = BM / (8 * NW), NIB = BN / (8 * NW), INSTR = NIA + NIB;  // 8 rows of 128 bytes per load instruction
+  static constexpr size_t RING = (size_t)STAGES * BUF * 2;
+  static constexpr size_t STAGE_REGION = 32 * (QB * 16 * 2 + 8);
+  static constexpr size_t LDS = RING > NW * STAGE_REGION ? RING : NW * STAGE_REGION;
+  static_assert(BN / WN == 64 && BM % (8 * NW) == 0 && BN % (8 * NW) == 0 && LDS <= 160 * 1024, "tile shape");
+};
+
+__device__ __forceinline__ int swz16_a(int row) { return (row >> 1) & 7; }
+__device__ __forceinline__ int swz16_b(int row) { return ((row >> 3) & 3) * 2 + ((row >> 1) & 1); }
+
+template <bool F16, int BM, int BN, int WM, int WN, int STAGES, class Epi>
+__global__ __launch_bounds__(WM* WN * 64) void tile16_kernel(Tile16 p, typename Epi::Args e) {
+  using K_ = TileKernel<F16, BM, BN, WM, WN, STAGES, Epi>;
+  constexpr int NW = K_::NW, QB = K_::QB, BK = K_::BK;
+  using frag = std::conditional_t<F16, f16x8, bf16x8>;
+  typedef __attribute__((address_space(3))) const frag lds_frag_t;
+  extern __shared__ __attribute__((aligned(16))) u16 smem_t[];
+  const unsigned lds_base = __builtin_amdgcn_readfirstlane((unsigned)(size_t)((__attribute__((address_space(3))) const void*)smem_t));
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int l16 = lane & 15, q = lane >> 4;
+  const int wm0 = (wave / WN) * (BM / WM), wn0 = (wave % WN) * 64;
+
+  int tm, tn;
+  tile16_of_workgroup(p, blockIdx.x, gridDim.x, tm, tn);
+  const int m0 = tm * BM, n0 = tn * BN;
+  const int entry = blockIdx.z / p.splits, split = blockIdx.z - entry * p.splits;
+  const int steps = p.K / BK;
+  const int k0 = (int)((long long)steps * split / p.splits), nk = (int)((long long)steps * (split + 1) / p.splits) - k0;
+
+  unsigned offa[K_::NIA], offb[K_::NIB];
+  const int lrow = lane >> 3, pc = lane & 7;
+#pragma unroll
+  for (int j = 0; j < K_::NIA; ++j) {
+    const int row = (j * NW + wave) * 8 + lrow, real = m0 + row < p.M ? row : p.M - 1 - m0;
+    offa[j] = 2u * ((unsigned)real * (unsigned)p.lda + (unsigned)(pc ^ swz16_a(row)) * 8u);
+  }
+#pragma unroll
+  for (int j = 0; j < K_::NIB; ++j) {
+    const int row = (j * NW + wave) * 8 + lrow, real = n0 + row < p.N ? row : p.N - 1 - n0;
+    offb[j] = 2u * ((unsigned)real * (unsigned)p.ldb + (unsigned)(pc ^ swz16_b(row)) * 8u);
+  }
+  const u16* a = p.A + (size_t)entry * p.batchA + (size_t)m0 * p.lda + (size_t)k0 * BK;
+  const u16* b = p.B + (size_t)entry * p.batchB + (size_t)n0 * p.ldb + (size_t)k0 * BK;
+  auto issue = [&](int buf) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < K_::NIA; ++j)
+      load_to_lds_uniform(a, offa[j], lds_base + 2u * (unsigned)(buf * K_::BUF + (j * NW + wave) * 8 * BK));
+#pragma unroll
+    for (int j = 0; j < K_::NIB; ++j)
+      load_to_lds_uniform(b, offb[j], lds_base + 2u * (unsigned)(buf * K_::BUF + K_::A_ELEMS + (j * NW + wave) * 8 * BK));
+    a += BK;
+    b += BK;
+  };
+
+  unsigned qa[2], pa[2];
+#pragma unroll
+  for (int kc = 0; kc < 2; ++kc) {
+    const int ra = wm0 + l16, rb = wn0 + 8 * (l16 >> 2) + (l16 & 3);
+    qa[kc] = lds_base + 2u * (unsigned)(ra * BK + ((kc * 4 + q) ^ swz16_a(ra)) * 8);
+    pa[kc] = lds_base + 2u * (unsigned)(K_::A_ELEMS + rb * BK + ((kc * 4 + q) ^ swz16_b(rb)) * 8);
+  }
+  f32x4 acc[QB][4];
+#pragma unroll
+  for (int jq = 0; jq < QB; ++jq)
+#pragma unroll
+    for (int ip = 0; ip < 4; ++ip) acc[jq][ip] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+#pragma unroll
+  for (int s = 0; s < STAGES - 1; ++s)
+    if (s < nk) issue(s);
+  int cur = 0;
+  for (int t = 0; t < nk; ++t) {
+    if (t + STAGES - 1 <= nk) __builtin_amdgcn_s_waitcnt(vmcnt_imm((STAGES - 2) * K_::INSTR));
+    else __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+    ring_barrier();
+    if (t + STAGES - 1 < nk) issue(cur == 0 ? STAGES - 1 : cur - 1);
+    const unsigned off = 2u * (unsigned)(cur * K_::BUF);
+#pragma unroll
+    for (int kc = 0; kc < 2; ++kc) {
+      frag fp[4];
+#pragma unroll
+      for (int ip = 0; ip < 4; ++ip)
+        fp[ip] = *reinterpret_cast<lds_frag_t*>((__attribute__((address_space(3))) const char*)(size_t)(
+            pa[kc] + off + 2u * (unsigned)((32 * (ip >> 1) + 4 * (ip & 1)) * BK)));
+#pragma unroll
+      for (int jq = 0; jq < QB; ++jq) {
+        const frag fq = *reinterpret_cast<lds_frag_t*>((__attribute__((address_space(3))) const char*)(size_t)(
+            qa[kc] + off + 2u * (unsigned)(jq * 16 * BK)));
+#pragma unroll
+        for (int ip = 0; ip < 4; ++ip) {
+          if constexpr (F16) acc[jq][ip] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fp[ip], fq, acc[jq][ip], 0, 0, 0);
+          else acc[jq][ip] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp[ip], fq, acc[jq][ip], 0, 0, 0);
+        }
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);  // this step's reads have returned (its MFMAs are issued) before the next barrier
+    cur = cur + 1 == STAGES ? 0 : cur + 1;
+  }
+  __syncthreads();  // every wavefront is done with the operand tiles: the epilogue may use the LDS
+  unsigned char* stage = reinterpret_cast<unsigned char*>(smem_t) + (size_t)wave * K_::STAGE_REGION;
+  auto get = [&](int jq, int h, int i) __attribute__((always_inline)) { return acc[jq][2 * h + (i >> 2)][i & 3]; };
+  Epi::template run<QB>(e, p, get, m0 + wm0, n0 + wn0, lane, stage, entry, split);
+}
+
+template <bool F16, int BM, int BN, int WM, int WN, int STAGES, class Epi>
+hipError_t launch_tile16(Tile16 p, const typename Epi::Args& e, int batch, hipStream_t s) {
+  using K_ = TileKernel<F16, BM, BN, WM, WN, STAGES, Epi>;
+  p.tiles_m = (p.M + BM - 1) / BM;
+  p.tiles_n = (p.N + BN - 1) / BN;
+  const long long total = p.symmetric ? (long long)p.tiles_m * (p.tiles_m + 1) / 2 : (long long)p.tiles_m * p.tiles_n;
+  if (total <= 0 || batch <= 0) return hipSuccess;
+  if (total > 0x7fffffffLL / 2 || (long long)batch * p.splits > 65535) return hipErrorInvalidValue;
+  auto kern = tile16_kernel<F16, BM, BN, WM, WN, STAGES, Epi>;
+  static LdsOptIn opt_in;
+  if (hipError_t err = opt_in.ensure(reinterpret_cast<const void*>(kern), K_::LDS); err != hipSuccess) return err;
+  launch_kernel(kern, dim3((unsigned)total, 1, batch * p.splits), dim3(WM * WN * 64), K_::LDS, s, p, e);
+  return hipGetLastError();
+}
+
+}  // namespace mi

@@ -1,0 +1,692 @@
+// Softmax cross entropy of a linear classifier without keeping its logits.
+//
+//   z = X W^T + b [M x V]      lse_i = log sum_j exp z_ij      loss_i = lse_i - z_i,t(i)
+//   g_ij = d_i (exp(z_ij - lse_i) - [j = t(i)])      dX = g W      dW = g^T X      db_j = sum_i g_ij
+//
+// Forward, bf16: one pass of MFMA tiles over z.  A tile leaves two numbers per row and 64 columns, the
+// maximum m and s = sum exp(z - m) over the columns other than the target, and the target's own logit;
+// a fold joins them.  The target is kept apart because lse - z_t cancels where a row is sure of its
+// answer; with o = log sum over the others, loss = softplus(o - z_t) does not.
+// Backward, bf16: the vocabulary is walked in pieces.  Per piece the tiles of z are computed again and
+// leave as g (rounded to bf16, the operand type of the products that follow: half a step of 2^-8 per
+// term) in both orders that the next two products read, g for dX += g W and g^T for dW = g^T X.
+// fp32 models: the same pieces through the framework's fp32 GEMMs, with the softmax between them.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+
+#include "kernels.h"
+#include "tile16.h"
+
+namespace mi {
+
+namespace {
+
+constexpr float LOG2E = 1.44269504088896340736f;
+
+__device__ __forceinline__ float finite_or_zero(float m) { return __builtin_isinf(m) ? 0.0f : m; }
+
+// (m, s) stands for m' + log s with m' = 0 where m is infinite.  m = -inf: nothing but -inf (s = 0) or
+// NaN (s = NaN) so far; m = +inf: s = inf.  NaN travels in s, which every NaN logit reaches.
+__device__ __forceinline__ void join(float& m, float& s, float m2, float s2) {
+  const float top = fmaxf(m, m2), t = finite_or_zero(top);
+  const float w1 = m == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f((finite_or_zero(m) - t) * LOG2E);
+  const float w2 = m2 == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f((finite_or_zero(m2) - t) * LOG2E);
+  s = s * w1 + s2 * w2;
+  m = top;
+}
+
+// Loss and lse of a row from the statistics of its other columns and the target's logit.
+__device__ __forceinline__ void finish_row(float m, float s, bool counts, float zt, float* loss, float* lse) {
+  const float others = finite_or_zero(m) + logf(s);
+  if (!counts) {
+    *loss = 0.0f;
+    *lse = others;
+    return;
+  }
+  const float d = others - zt;
+  const float tail = log1pf(expf(-fabsf(d)));
+  *loss = fmaxf(d, 0.0f) + tail;  // d = NaN: the tail is NaN
+  *lse = others == zt && __builtin_isinf(zt) ? zt : fmaxf(others, zt) + tail;
+}
+
+// ---- bf16 tiles -------------------------------------------------------------------------------------
+
+struct EpiStats {
+  struct Args {
+    const float* bias;    // of the first column, or null
+    const int* target;
+    int first, vocab;     // first column of this launch in the vocabulary, size of the vocabulary
+    float* zt;            // [M]
+    float2* part;         // [column block of 64][M], from this launch's first block on
+  };
+  template <int QB, class Get>
+  static __device__ __forceinline__ void run(const Args& e, const Tile16& p, Get get, int row0, int colw, int lane,
+                                             unsigned char*, int, int) {
+    const int l16 = lane & 15, q = lane >> 4, lane_col = colw + 8 * q;
+    if (colw >= p.N) return;
+    float bias[2][8];
+    const bool edge = colw + 64 > p.N;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int col = lane_col + 32 * h + i;
+        bias[h][i] = e.bias && col < p.N ? e.bias[col] : 0.0f;
+      }
+#pragma unroll
+    for (int jq = 0; jq < QB; ++jq) {
+      const int row = row0 + 16 * jq + l16;
+      int t = row < p.M ? e.target[row] : -1;
+      t = t >= 0 && t < e.vocab ? t - e.first - lane_col : -1;  // relative to the lane's first column
+      float v[2][8];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[h][i] = get(jq, h, i) + bias[h][i];
+      if (t >= 0 && t < 40 && (t & 31) < 8) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (t == 32 * h + i) {
+              e.zt[row] = v[h][i];
+              v[h][i] = -__builtin_inff();
+            }
+      }
+      if (edge) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (lane_col + 32 * h + i >= p.N) v[h][i] = -__builtin_inff();
+      }
+      float m = v[0][0];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = fmaxf(m, v[h][i]);
+      m = fmaxf(m, __shfl_xor(m, 16, 64));
+      m = fmaxf(m, __shfl_xor(m, 32, 64));
+      const float mm = finite_or_zero(m);
+      float s = 0.0f;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s += __builtin_amdgcn_exp2f((v[h][i] - mm) * LOG2E);
+      s += __shfl_xor(s, 16, 64);
+      s += __shfl_xor(s, 32, 64);
+      if (q == 0 && row < p.M) e.part[(size_t)(colw >> 6) * p.M + row] = float2{m, s};
+    }
+  }
+};
+
+struct EpiGrad {
+  struct Args {
+    const float* bias;
+    const int* target;
+    const float* lse;
+    const float* dloss;  // null: 1 for every row
+    int first, vocab;
+    u16* G;              // [rows padded][ldg]
+    u16* GT;             // [columns padded][ldgt]
+    int ldg, ldgt;
+    float* db_part;      // [row0 / (16 QB)][ldg] or null
+  };
+  template <int QB, class Get>
+  static __device__ __forceinline__ void run(const Args& e, const Tile16& p, Get get, int row0, int colw, int lane,
+                                             unsigned char* stage, int, int) {
+    const int l16 = lane & 15, q = lane >> 4, lane_col = colw + 8 * q;
+    float bias[2][8], sums[2][8];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int col = lane_col + 32 * h + i;
+        bias[h][i] = e.bias && col < p.N ? e.bias[col] : 0.0f;
+        sums[h][i] = 0.0f;
+      }
+    const bool edge = colw + 64 > p.N;
+    u32x4 pk[QB][2];
+#pragma unroll
+    for (int jq = 0; jq < QB; ++jq) {
+      const int row = row0 + 16 * jq + l16;
+      int t = row < p.M ? e.target[row] : -1;
+      const bool live = t >= 0 && t < e.vocab;
+      t = t - e.first - lane_col;
+      const float lse = live ? e.lse[row] : 0.0f;
+      const float d = live ? (e.dloss ? e.dloss[row] : 1.0f) : 0.0f;
+      float g[2][8];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float x = __builtin_amdgcn_exp2f((get(jq, h, i) + bias[h][i] - lse) * LOG2E);
+          g[h][i] = live ? d * x : 0.0f;
+        }
+      if (live && t >= 0 && t < 40 && (t & 31) < 8) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (t == 32 * h + i) g[h][i] = d * expm1f(get(jq, h, i) + bias[h][i] - lse);
+      }
+      if (edge) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (lane_col + 32 * h + i >= p.N) g[h][i] = 0.0f;
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sums[h][i] += g[h][i];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) pk[jq][h][k] = pack16<false>(g[h][2 * k], g[h][2 * k + 1]);
+        *reinterpret_cast<u32x4*>(e.G + (size_t)row * e.ldg + lane_col + 32 * h) = pk[jq][h];
+      }
+    }
+    if (e.db_part) {
+      float* dst = e.db_part + (size_t)(row0 / (16 * QB)) * e.ldg + lane_col;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+          for (int off = 1; off < 16; off <<= 1) sums[h][i] += __shfl_xor(sums[h][i], off, 64);
+        if (l16 == 0) {
+          *reinterpret_cast<f32x4*>(dst + 32 * h) = f32x4{sums[h][0], sums[h][1], sums[h][2], sums[h][3]};
+          *reinterpret_cast<f32x4*>(dst + 32 * h + 4) = f32x4{sums[h][4], sums[h][5], sums[h][6], sums[h][7]};
+        }
+      }
+    }
+    store_transposed<QB>(e.GT + (size_t)colw * e.ldgt + row0, e.ldgt, pk, lane, stage);
+  }
+};
+
+// C (fp32 or bf16), one slab per K split; rows and columns behind the result are dropped.
+template <bool OUT_BF16>
+struct EpiOut {
+  struct Args {
+    void* C;
+    long long slab;  // elements between the results of consecutive splits
+    int ldc;
+    int vec;         // 16-byte stores allowed
+    int add;         // fp32: C += instead of C =
+  };
+  template <int QB, class Get>
+  static __device__ __forceinline__ void run(const Args& e, const Tile16& p, Get get, int row0, int colw, int lane,
+                                             unsigned char*, int, int split) {
+    const int l16 = lane & 15, col0 = colw + 8 * (lane >> 4);
+#pragma unroll
+    for (int jq = 0; jq < QB; ++jq) {
+      const int row = row0 + 16 * jq + l16;
+      if (row >= p.M) continue;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int col = col0 + 32 * h;
+        if (col >= p.N) continue;
+        const size_t at = (size_t)split * e.slab + (size_t)row * e.ldc + col;
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = get(jq, h, i);
+        const bool whole = e.vec && col + 8 <= p.N;
+        if constexpr (OUT_BF16) {
+          u16* c = reinterpret_cast<u16*>(e.C) + at;
+          if (whole) {
+            *reinterpret_cast<u32x4*>(c) = u32x4{pack16<false>(v[0], v[1]), pack16<false>(v[2], v[3]),
+                                                 pack16<false>(v[4], v[5]), pack16<false>(v[6], v[7])};
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (col + i < p.N) c[i] = f2bf(v[i]);
+          }
+        } else {
+          float* c = reinterpret_cast<float*>(e.C) + at;
+          if (whole) {
+            f32x4* c4 = reinterpret_cast<f32x4*>(c);
+            f32x4 lo = {v[0], v[1], v[2], v[3]}, hi = {v[4], v[5], v[6], v[7]};
+            if (e.add) {
+              lo += c4[0];
+              hi += c4[1];
+            }
+            c4[0] = lo;
+            c4[1] = hi;
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (col + i < p.N) c[i] = e.add ? c[i] + v[i] : v[i];
+          }
+        }
+      }
+    }
+  }
+};
+
+constexpr int TB = 128;  // rows and columns of a tile: what padded sizes are multiples of
+
+template <class Epi>
+hipError_t tiles(const u16* A, int lda, const u16* B, int ldb, int M, int N, int K, int splits, const typename Epi::Args& e,
+                 hipStream_t s) {
+  Tile16 p{};
+  p.A = A; p.B = B; p.lda = lda; p.ldb = ldb; p.M = M; p.N = N; p.K = K;
+  p.splits = splits;
+  return launch_tile16<false, TB, TB, 2, 2, 2, Epi>(p, e, 1, s);
+}
+
+// ---- joins and copies -------------------------------------------------------------------------------
+
+// Joins a row's column-block statistics.  16 rows x 16 lanes per workgroup: a lane takes every 16th block
+// of one row, the 16 lanes of a row are joined in a fixed order.
+__global__ __launch_bounds__(256) void xent_fold_kernel(const float2* __restrict__ part, int blocks, int M, int vocab,
+                                                        const int* __restrict__ target, const float* __restrict__ zt,
+                                                        float* __restrict__ loss, float* __restrict__ lse) {
+  __shared__ float2 red[16][17];
+  const int r = threadIdx.x & 15, w = threadIdx.x >> 4, row = blockIdx.x * 16 + r;
+  float m = -__builtin_inff(), s = 0.0f;
+  if (row < M)
+    for (int c = w; c < blocks; c += 16) {
+      const float2 v = part[(size_t)c * M + row];
+      join(m, s, v.x, v.y);
+    }
+  red[w][r] = float2{m, s};
+  __syncthreads();
+  if (w != 0 || row >= M) return;
+  for (int i = 1; i < 16; ++i) join(m, s, red[i][r].x, red[i][r].y);
+  const int t = target[row];
+  const bool counts = t >= 0 && t < vocab;
+  finish_row(m, s, counts, counts ? zt[row] : 0.0f, loss + row, lse + row);
+}
+
+// dst[rows][ldd] = src[rows][cols], zeros up to ldd.
+__global__ __launch_bounds__(256) void pack_rows_kernel(u16* __restrict__ dst, const u16* __restrict__ src, int rows, int cols,
+                                                        int ld, int ldd) {
+  const size_t n = (size_t)rows * ldd, step = (size_t)gridDim.x * 256;
+  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += step) {
+    const size_t r = i / ldd;
+    const int c = (int)(i - r * ldd);
+    dst[i] = c < cols ? src[r * ld + c] : (u16)0;
+  }
+}
+
+// dst[c][r] = src[r][c] for c < cols, r < ldd; zeros from row `rows` on.  64 x 64 tiles through LDS.
+__global__ __launch_bounds__(256) void pack_transposed_kernel(u16* __restrict__ dst, const u16* __restrict__ src, int rows,
+                                                              int cols, int ld, int ldd, int vec) {
+  __shared__ __attribute__((aligned(16))) u16 tile[64][72];
+  const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;
+  const int part = threadIdx.x & 7, line = threadIdx.x >> 3;
+  if (vec && r0 + 64 <= rows && c0 + 64 <= cols) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      *reinterpret_cast<u32x4*>(&tile[line + 32 * i][part * 8]) =
+          *reinterpret_cast<const u32x4*>(src + (size_t)(r0 + line + 32 * i) * ld + c0 + part * 8);
+  } else {
+    const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
+    for (int i = ty; i < 64; i += 4)
+      tile[i][tx] = r0 + i < rows && c0 + tx < cols ? src[(size_t)(r0 + i) * ld + c0 + tx] : (u16)0;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {  // ldd is a multiple of 64 and dst 16-byte aligned
+    const int c = line + 32 * i;
+    if (c0 + c >= cols) continue;
+    u16 v[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = tile[part * 8 + k][c];
+    *reinterpret_cast<u32x4*>(dst + (size_t)(c0 + c) * ldd + r0 + part * 8) =
+        u32x4{(unsigned)v[0] | ((unsigned)v[1] << 16), (unsigned)v[2] | ((unsigned)v[3] << 16),
+              (unsigned)v[4] | ((unsigned)v[5] << 16), (unsigned)v[6] | ((unsigned)v[7] << 16)};
+  }
+}
+
+// C[row][col] = sum over slabs, in slab order, of part[slab][row][col] (fp32), to fp32 or bf16.
+template <bool OUT_BF16>
+__global__ __launch_bounds__(256) void fold_slabs_kernel(void* __restrict__ C, int ldc, const float* __restrict__ part, int ldp,
+                                                         long long slab, int slabs, int rows, int cols) {
+  const size_t n = (size_t)rows * cols, step = (size_t)gridDim.x * 256;
+  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += step) {
+    const size_t r = i / cols;
+    const int c = (int)(i - r * cols);
+    const float* src = part + r * ldp + c;
+    float v = 0.0f;
+    for (int k = 0; k < slabs; ++k) v += src[(size_t)k * slab];
+    if constexpr (OUT_BF16) reinterpret_cast<u16*>(C)[r * ldc + c] = f2bf(v);
+    else reinterpret_cast<float*>(C)[r * ldc + c] = v;
+  }
+}
+
+// out[c] = sum over blocks of part[block][c]
+__global__ __launch_bounds__(256) void fold_columns_kernel(float* __restrict__ out, const float* __restrict__ part, int ld,
+                                                           int blocks, int cols) {
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c >= cols) return;
+  float v = 0.0f;
+  for (int b = 0; b < blocks; ++b) v += part[(size_t)b * ld + c];
+  out[c] = v;
+}
+
+// ---- fp32 models ------------------------------------------------------------------------------------
+
+// Statistics of one piece of logits Z [M x cols], joined to those of the pieces before (first: none).
+// One workgroup per row; `last` turns them into loss and lse.
+__global__ __launch_bounds__(256) void xent_rows_f32_kernel(const float* __restrict__ Z, int ldz, int cols, int first, int vocab,
+                                                            int last, const int* __restrict__ target, float2* __restrict__ part,
+                                                            float* __restrict__ zt, float* __restrict__ loss, float* __restrict__ lse) {
+  __shared__ float2 red[256];
+  const int row = blockIdx.x, tid = threadIdx.x;
+  int t = target[row];
+  const bool counts = t >= 0 && t < vocab;
+  t = counts ? t - first : -1;
+  const float* z = Z + (size_t)row * ldz;
+  float m = -__builtin_inff(), s = 0.0f;
+  for (int c = tid; c < cols; c += 256) {
+    if (c == t) continue;
+    join(m, s, z[c], __builtin_isinf(z[c]) ? (z[c] > 0.0f ? __builtin_inff() : 0.0f) : z[c] - z[c] + 1.0f);
+  }
+  red[tid] = float2{m, s};
+  __syncthreads();
+  for (int off = 128; off > 0; off >>= 1) {
+    if (tid < off) {
+      float2 a = red[tid];
+      const float2 b = red[tid + off];
+      join(a.x, a.y, b.x, b.y);
+      red[tid] = a;
+    }
+    __syncthreads();
+  }
+  if (tid != 0) return;
+  float2 all = red[0];
+  if (first > 0) {
+    float2 before = part[row];
+    join(before.x, before.y, all.x, all.y);
+    all = before;
+  }
+  if (t >= 0 && t < cols) zt[row] = z[t];
+  if (last) finish_row(all.x, all.y, counts, counts ? zt[row] : 0.0f, loss + row, lse + row);
+  else part[row] = all;
+}
+
+__global__ __launch_bounds__(256) void xent_grad_f32_kernel(float* __restrict__ Z, int ldz, int M, int cols, int first, int vocab,
+                                                            const int* __restrict__ target, const float* __restrict__ lse,
+                                                            const float* __restrict__ dloss) {
+  const size_t n = (size_t)M * cols, step = (size_t)gridDim.x * 256;
+  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += step) {
+    const size_t r = i / cols;
+    const int c = (int)(i - r * cols), t = target[r];
+    float g = 0.0f;
+    if (t >= 0 && t < vocab) {
+      const float x = Z[r * ldz + c] - lse[r];
+      g = (dloss ? dloss[r] : 1.0f) * (c == t - first ? expm1f(x) : expf(x));
+    }
+    Z[r * ldz + c] = g;
+  }
+}
+
+__global__ __launch_bounds__(256) void add_rows_kernel(float* __restrict__ dst, int ldd, const float* __restrict__ src, int rows,
+                                                       int cols) {
+  const size_t n = (size_t)rows * cols, step = (size_t)gridDim.x * 256;
+  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += step) {
+    const size_t r = i / cols;
+    dst[r * ldd + (i - r * cols)] += src[i];
+  }
+}
+
+// ---- sizes ------------------------------------------------------------------------------------------
+
+inline size_t up(size_t x, size_t a) { return (x + a - 1) / a * a; }
+inline bool al16(const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0; }
+inline unsigned flat_grid(size_t n) { return (unsigned)std::min<size_t>((n + 255) / 256, 8192); }
+
+// Hands out 256-byte aligned parts of a workspace (or only adds them up, base = null).
+struct Carver {
+  char* base;
+  size_t used = 0;
+  template <class T>
+  T* take(size_t n) {
+    T* q = base ? reinterpret_cast<T*>(base + used) : nullptr;
+    used += up(n * sizeof(T), 256);
+    return q;
+  }
+};
+
+struct ForwardPlan {
+  int Kp;          // K rounded up to whole K steps
+  int pack_cols;   // columns per launch where W has to be packed
+  u16 *Xp, *Wp;
+  float* zt;
+  float2* part;
+  size_t bytes;
+};
+ForwardPlan plan_forward(char* base, int M, int V, int K) {
+  ForwardPlan f{};
+  Carver c{base};
+  f.Kp = (int)up(K, 64);
+  f.pack_cols = (int)std::min<size_t>(up(V, TB), std::max<size_t>(((size_t)1 << 24) / f.Kp / TB * TB, TB));
+  f.Xp = c.take<u16>((size_t)M * f.Kp);
+  f.Wp = c.take<u16>((size_t)std::min(V, f.pack_cols) * f.Kp);
+  f.zt = c.take<float>(M);
+  f.part = c.take<float2>((size_t)M * (up(V, 64) / 64));
+  f.bytes = c.used;
+  return f;
+}
+
+struct BackwardPlan {
+  int Kp, Mp, piece, splits_x, splits_w;
+  bool sum_x;      // dX comes out of fp32 slabs
+  u16 *Xp, *Xt, *Wp, *Wt, *G, *GT;
+  float *db_part, *x_part, *w_part;
+  size_t bytes;
+};
+int splits_for(size_t rows, size_t cols, size_t steps) {
+  const size_t n = up(rows, TB) / TB * (up(cols, TB) / TB);
+  // enough workgroups for the 256 CUs, but at least eight K steps for each
+  return (int)std::max<size_t>(1, std::min<size_t>({(256 + n - 1) / n, steps / 8, 64}));
+}
+BackwardPlan plan_backward(char* base, int M, int V, int K) {
+  BackwardPlan b{};
+  Carver c{base};
+  b.Kp = (int)up(K, 64);
+  b.Mp = (int)up(M, TB);
+  // g and g^T of a piece take at most 2 x 512 MB, the copies of W's piece 256 MB each
+  const size_t most = std::min(((size_t)1 << 28) / b.Mp, ((size_t)1 << 27) / b.Kp) / 256 * 256;
+  b.piece = (int)std::min<size_t>(up(V, TB), std::max<size_t>(most, 256));
+  b.splits_x = splits_for(M, K, b.piece / 64);
+  b.splits_w = splits_for(b.piece, K, b.Mp / 64);
+  b.sum_x = b.splits_x > 1 || b.piece < V;
+  b.Xp = c.take<u16>((size_t)M * b.Kp);
+  b.Xt = c.take<u16>((size_t)K * b.Mp);
+  b.Wp = c.take<u16>((size_t)std::min(V, b.piece) * b.Kp);
+  b.Wt = c.take<u16>((size_t)K * b.piece);
+  b.G = c.take<u16>((size_t)b.Mp * b.piece);
+  b.GT = c.take<u16>((size_t)b.Mp * b.piece);
+  b.db_part = c.take<float>((size_t)(b.Mp / 64) * b.piece);
+  if (b.sum_x) b.x_part = c.take<float>((size_t)b.splits_x * M * b.Kp);
+  if (b.splits_w > 1) b.w_part = c.take<float>((size_t)b.splits_w * b.piece * b.Kp);
+  b.bytes = c.used;
+  return b;
+}
+
+struct F32Plan {
+  int piece;
+  float *Z, *zt, *x_part;
+  float2* part;
+  size_t bytes;
+};
+F32Plan plan_f32(char* base, int M, int V, int K, bool backward) {
+  F32Plan f{};
+  Carver c{base};
+  const size_t most = std::max<size_t>(((size_t)1 << 28) / M / 64 * 64, 64);  // a piece of logits takes at most 1 GB
+  f.piece = (int)std::min<size_t>(up(V, 64), most);
+  f.Z = c.take<float>((size_t)M * f.piece);
+  if (backward) {
+    if (f.piece < V) f.x_part = c.take<float>((size_t)M * K);
+  } else {
+    f.zt = c.take<float>(M);
+    f.part = c.take<float2>(M);
+  }
+  f.bytes = c.used;
+  return f;
+}
+
+#define TRY(call)                          \
+  do {                                     \
+    hipError_t e_ = (call);                \
+    if (e_ != hipSuccess) return e_;       \
+  } while (0)
+
+// Whether the tiles can read an operand where it is: 16-byte rows, whole K steps, 32-bit offsets in a tile.
+bool direct(const u16* q, int ld, int K) { return al16(q) && ld % 8 == 0 && ld <= TILE16_MAX_LD && K % 64 == 0; }
+
+hipError_t pack_rows(u16* dst, const u16* src, int rows, int cols, int ld, int ldd, hipStream_t s) {
+  launch_kernel(pack_rows_kernel, dim3(flat_grid((size_t)rows * ldd)), dim3(256), 0, s, dst, src, rows, cols, ld, ldd);
+  return hipGetLastError();
+}
+hipError_t pack_transposed(u16* dst, const u16* src, int rows, int cols, int ld, int ldd, hipStream_t s) {
+  launch_kernel(pack_transposed_kernel, dim3((cols + 63) / 64, ldd / 64), dim3(256), 0, s, dst, src, rows, cols, ld, ldd,
+                (int)(al16(src) && ld % 8 == 0));
+  return hipGetLastError();
+}
+
+}  // namespace
+
+size_t xent_forward_bytes(bool bf16, int M, int V, int K) {
+  return bf16 ? plan_forward(nullptr, M, V, K).bytes : plan_f32(nullptr, M, V, K, false).bytes;
+}
+size_t xent_backward_bytes(bool bf16, int M, int V, int K) {
+  return bf16 ? plan_backward(nullptr, M, V, K).bytes : plan_f32(nullptr, M, V, K, true).bytes;
+}
+
+hipError_t xent_forward_bf16(int M, int V, int K, const u16* X, int ldx, const u16* W, int ldw, const float* bias,
+                             const int* target, float* loss, float* lse, void* ws, hipStream_t s) {
+  const ForwardPlan f = plan_forward(static_cast<char*>(ws), M, V, K);
+  const bool x_direct = direct(X, ldx, K), w_direct = direct(W, ldw, K);
+  if (!x_direct) {
+    TRY(pack_rows(f.Xp, X, M, K, ldx, f.Kp, s));
+    X = f.Xp;
+    ldx = f.Kp;
+  }
+  const int per = w_direct ? V : f.pack_cols;
+  for (int v0 = 0; v0 < V; v0 += per) {
+    const int cols = std::min(per, V - v0);
+    const u16* w = W + (size_t)v0 * ldw;
+    if (!w_direct) {
+      TRY(pack_rows(f.Wp, w, cols, K, ldw, f.Kp, s));
+      w = f.Wp;
+    }
+    const EpiStats::Args e{bias ? bias + v0 : nullptr, target, v0, V, f.zt, f.part + (size_t)(v0 / 64) * M};
+    TRY(tiles<EpiStats>(X, ldx, w, w_direct ? ldw : f.Kp, M, cols, f.Kp, 1, e, s));
+  }
+  launch_kernel(xent_fold_kernel, dim3((M + 15) / 16), dim3(256), 0, s, (const float2*)f.part, (int)(up(V, 64) / 64), M, V,
+                target, (const float*)f.zt, loss, lse);
+  return hipGetLastError();
+}
+
+hipError_t xent_backward_bf16(int M, int V, int K, const u16* X, int ldx, const u16* W, int ldw, const u16* Wt, int ldwt,
+                              const float* bias, const int* target, const float* lse, const float* dloss, u16* dX, int lddx,
+                              bool dw_bf16, void* dW, int lddw, float* db, void* ws, hipStream_t s) {
+  const BackwardPlan b = plan_backward(static_cast<char*>(ws), M, V, K);
+  const bool x_direct = direct(X, ldx, K), w_direct = direct(W, ldw, K);
+  TRY(pack_transposed(b.Xt, X, M, K, ldx, b.Mp, s));
+  if (!x_direct) {
+    TRY(pack_rows(b.Xp, X, M, K, ldx, b.Kp, s));
+    X = b.Xp;
+    ldx = b.Kp;
+  }
+  for (int v0 = 0; v0 < V; v0 += b.piece) {
+    const int cols = std::min(b.piece, V - v0), padded = (int)up(cols, TB), steps = (int)up(cols, 64) / 64;
+    const u16* w = W + (size_t)v0 * ldw;
+    int ld_w = ldw;
+    if (!w_direct) {
+      TRY(pack_rows(b.Wp, w, cols, K, ldw, b.Kp, s));
+      w = b.Wp;
+      ld_w = b.Kp;
+    }
+    const EpiGrad::Args g{bias ? bias + v0 : nullptr, target, lse, dloss, v0, V, b.G, b.GT, padded, b.Mp, db ? b.db_part : nullptr};
+    TRY(tiles<EpiGrad>(X, ldx, w, ld_w, M, cols, b.Kp, 1, g, s));
+    if (db) {
+      launch_kernel(fold_columns_kernel, dim3((cols + 255) / 256), dim3(256), 0, s, db + v0, (const float*)b.db_part, padded,
+                    b.Mp / 64, cols);
+      TRY(hipGetLastError());
+    }
+    // dX (+)= g W: the caller's transposed copy where whole 16-byte chunks of it can be read
+    const u16* wt = Wt ? Wt + v0 : nullptr;
+    int ld_t = ldwt;
+    if (!wt || !direct(wt, ldwt, cols)) {
+      TRY(pack_transposed(b.Wt, W + (size_t)v0 * ldw, cols, K, ldw, padded, s));
+      wt = b.Wt;
+      ld_t = padded;
+    }
+    if (b.sum_x) {
+      const int splits = std::min(b.splits_x, steps);
+      const EpiOut<false>::Args e{b.x_part, (long long)M * b.Kp, b.Kp, 1, v0 > 0};
+      TRY(tiles<EpiOut<false>>(b.G, padded, wt, ld_t, M, K, steps * 64, splits, e, s));
+    } else {
+      const EpiOut<true>::Args e{dX, 0, lddx, al16(dX) && lddx % 8 == 0, 0};
+      TRY(tiles<EpiOut<true>>(b.G, padded, wt, ld_t, M, K, steps * 64, 1, e, s));
+    }
+    // dW = g^T X
+    void* dw = static_cast<char*>(dW) + (size_t)v0 * lddw * (dw_bf16 ? 2 : 4);
+    if (b.splits_w > 1) {
+      const EpiOut<false>::Args e{b.w_part, (long long)b.piece * b.Kp, b.Kp, 1, 0};
+      TRY(tiles<EpiOut<false>>(b.GT, b.Mp, b.Xt, b.Mp, cols, K, b.Mp, b.splits_w, e, s));
+      const dim3 grid(flat_grid((size_t)cols * K));
+      if (dw_bf16)
+        launch_kernel(fold_slabs_kernel<true>, grid, dim3(256), 0, s, dw, lddw, (const float*)b.w_part, b.Kp,
+                      (long long)b.piece * b.Kp, b.splits_w, cols, K);
+      else
+        launch_kernel(fold_slabs_kernel<false>, grid, dim3(256), 0, s, dw, lddw, (const float*)b.w_part, b.Kp,
+                      (long long)b.piece * b.Kp, b.splits_w, cols, K);
+      TRY(hipGetLastError());
+    } else if (dw_bf16) {
+      const EpiOut<true>::Args e{dw, 0, lddw, al16(dw) && lddw % 8 == 0, 0};
+      TRY(tiles<EpiOut<true>>(b.GT, b.Mp, b.Xt, b.Mp, cols, K, b.Mp, 1, e, s));
+    } else {
+      const EpiOut<false>::Args e{dw, 0, lddw, al16(dw) && lddw % 4 == 0, 0};
+      TRY(tiles<EpiOut<false>>(b.GT, b.Mp, b.Xt, b.Mp, cols, K, b.Mp, 1, e, s));
+    }
+  }
+  if (b.sum_x) {
+    // the last piece may have had fewer splits than there are slabs; the first piece wrote them all
+    launch_kernel(fold_slabs_kernel<true>, dim3(flat_grid((size_t)M * K)), dim3(256), 0, s, (void*)dX, lddx,
+                  (const float*)b.x_part, b.Kp, (long long)M * b.Kp, std::min(b.splits_x, (int)up(std::min(b.piece, V), 64) / 64), M, K);
+    TRY(hipGetLastError());
+  }
+  return hipSuccess;
+}
+
+hipError_t xent_forward_f32(int M, int V, int K, const float* X, int ldx, const float* W, int ldw, const float* bias,
+                            const int* target, float* loss, float* lse, void* ws, hipStream_t s) {
+  const F32Plan f = plan_f32(static_cast<char*>(ws), M, V, K, false);
+  for (int v0 = 0; v0 < V; v0 += f.piece) {
+    const int cols = std::min(f.piece, V - v0);
+    TRY(sgemm_nt(M, cols, K, X, ldx, W + (size_t)v0 * ldw, ldw, f.Z, f.piece, bias ? bias + v0 : nullptr, 0, s, 0));
+    launch_kernel(xent_rows_f32_kernel, dim3(M), dim3(256), 0, s, (const float*)f.Z, f.piece, cols, v0, V,
+                  (int)(v0 + cols == V), target, f.part, f.zt, loss, lse);
+    TRY(hipGetLastError());
+  }
+  return hipSuccess;
+}
+
+hipError_t xent_backward_f32(int M, int V, int K, const float* X, int ldx, const float* W, int ldw, const float* bias,
+                             const int* target, const float* lse, const float* dloss, float* dX, int lddx, float* dW, int lddw,
+                             float* db, void* ws, hipStream_t s) {
+  const F32Plan f = plan_f32(static_cast<char*>(ws), M, V, K, true);
+  for (int v0 = 0; v0 < V; v0 += f.piece) {
+    const int cols = std::min(f.piece, V - v0);
+    const float* w = W + (size_t)v0 * ldw;
+    TRY(sgemm_nt(M, cols, K, X, ldx, w, ldw, f.Z, f.piece, bias ? bias + v0 : nullptr, 0, s, 0));
+    launch_kernel(xent_grad_f32_kernel, dim3(flat_grid((size_t)M * cols)), dim3(256), 0, s, f.Z, f.piece, M, cols, v0, V, target,
+                  lse, dloss);
+    TRY(hipGetLastError());
+    TRY(sgemm_nn(M, K, cols, f.Z, f.piece, w, ldw, v0 ? f.x_part : dX, v0 ? K : lddx, nullptr, 0, s, 0));
+    if (v0) {
+      launch_kernel(add_rows_kernel, dim3(flat_grid((size_t)M * K)), dim3(256), 0, s, dX, lddx, (const float*)f.x_part, M, K);
+      TRY(hipGetLastError());
+    }
+    TRY(sgemm_tn(1, cols, K, M, f.Z, f.piece, X, ldx, dW + (size_t)v0 * lddw, lddw, 0, db ? db + v0 : nullptr, 0, s, 0));
+  }
+  return hipSuccess;
+}
+
+}  // namespace mi
