@@ -27,7 +27,6 @@ namespace {
 
 constexpr float NS_A = 3.4445f, NS_B = -4.7750f, NS_C = 2.0315f;
 constexpr float GRAM_SCALE = 4096.0f;  // A and b A + c A^2 are stored times this: off-diagonal entries start near 1 / (m sqrt n)
-constexpr int TB = 128;
 
 inline size_t up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 
@@ -153,7 +152,7 @@ struct EpiGram {
         for (int k = 0; k < 4; ++k) pk[jq][h][k] = pack16<true>(e.scale * get(jq, h, 2 * k), e.scale * get(jq, h, 2 * k + 1));
         *reinterpret_cast<u32x4*>(A + (size_t)(row0 + 16 * jq + l16) * e.ld + col + 32 * h) = pk[jq][h];
       }
-    if (row0 / TB != colw / TB) store_transposed<QB>(A + (size_t)colw * e.ld + row0, e.ld, pk, lane, stage);
+    if (row0 / p.tile != colw / p.tile) store_transposed<QB>(A + (size_t)colw * e.ld + row0, e.ld, pk, lane, stage);
   }
 };
 
@@ -177,7 +176,7 @@ struct EpiPoly {
     for (int jq = 0; jq < QB; ++jq)
 #pragma unroll
       for (int h = 0; h < 2; ++h) pk[jq][h] = *reinterpret_cast<const u32x4*>(A + (size_t)(row0 + 16 * jq + l16) * e.ld + col + 32 * h);
-    const bool on_diagonal = row0 / TB == colw / TB;
+    const bool on_diagonal = row0 / p.tile == colw / p.tile;
 #pragma unroll
     for (int jq = 0; jq < QB; ++jq)
 #pragma unroll
@@ -292,6 +291,7 @@ __global__ __launch_bounds__(256) void ortho_finish_kernel(FinishArgs p) {
 
 struct Plan {
   int m, n, mp, np;
+  int tile;    // of the products; m and n are padded to multiples of it
   bool flip;
   float scale;  // of the fp16 copies of X: a power of two near sqrt(n), so that typical entries start near 1 / sqrt(m)
   float* X;
@@ -305,8 +305,11 @@ Plan plan_ortho(char* base, int batch, int rows, int cols) {
   q.flip = rows > cols;
   q.m = std::min(rows, cols);
   q.n = std::max(rows, cols);
-  q.mp = (int)up(q.m, TB);
-  q.np = (int)up(q.n, TB);
+  // large matrices: 256 x 256 tiles once even the smallest products (the triangle of m x m) fill the CUs
+  const size_t t = up(q.m, 256) / 256;
+  q.tile = batch * t * (t + 1) / 2 >= 200 ? 256 : 128;
+  q.mp = (int)up(q.m, q.tile);
+  q.np = (int)up(q.n, q.tile);
   q.scale = 1.0f;
   while (q.scale * q.scale < (float)q.n && q.scale < 256.0f) q.scale *= 2.0f;
   size_t used = 0;
@@ -330,14 +333,15 @@ Plan plan_ortho(char* base, int batch, int rows, int cols) {
 }
 
 template <class Epi>
-hipError_t tiles(const u16* A, const u16* B, int M, int N, int K, long long batchA, long long batchB, int batch, bool symmetric,
+hipError_t tiles(int tile, const u16* A, const u16* B, int M, int N, int K, long long batchA, long long batchB, int batch, bool symmetric,
                  const typename Epi::Args& e, hipStream_t s) {
   Tile16 p{};
   p.A = A; p.B = B; p.lda = K; p.ldb = K; p.M = M; p.N = N; p.K = K;
   p.batchA = batchA; p.batchB = batchB;
   p.splits = 1;
   p.symmetric = symmetric;
-  return launch_tile16<true, TB, TB, 2, 2, 2, Epi>(p, e, batch, s);
+  p.tile = tile;
+  return launch_tile16<true, Epi>(p, e, batch, s);
 }
 
 #define TRY(call)                          \
@@ -370,12 +374,12 @@ hipError_t newton_schulz(const Plan& q, GatherArgs g, bool bf16, int batch, int 
   for (int k = 0; k < steps; ++k) {
     const bool last = k + 1 == steps;
     const EpiGram::Args gram{q.A, q.mp, a, GRAM_SCALE / (q.scale * q.scale)};
-    TRY(tiles<EpiGram>(q.Xh, q.Xh, q.mp, q.mp, q.np, x, x, batch, true, gram, s));
+    TRY(tiles<EpiGram>(q.tile, q.Xh, q.Xh, q.mp, q.mp, q.np, x, x, batch, true, gram, s));
     const EpiPoly::Args poly{q.A, q.P, q.diag, q.mp, a};
-    TRY(tiles<EpiPoly>(q.A, q.A, q.mp, q.mp, q.mp, a, a, batch, true, poly, s));
+    TRY(tiles<EpiPoly>(q.tile, q.A, q.A, q.mp, q.mp, q.mp, a, a, batch, true, poly, s));
     const EpiStep::Args step{q.X, q.diag, last ? nullptr : q.Xh, last ? nullptr : q.XhT[(k + 1) & 1], q.mp, q.np,
                              1.0f / (GRAM_SCALE * q.scale), q.scale};
-    TRY(tiles<EpiStep>(q.P, q.XhT[k & 1], q.mp, q.np, q.mp, a, x, batch, false, step, s));
+    TRY(tiles<EpiStep>(q.tile, q.P, q.XhT[k & 1], q.mp, q.np, q.mp, a, x, batch, false, step, s));
   }
   return hipSuccess;
 }

@@ -13,6 +13,7 @@
 //     ->  row 16 jq + l,  column 32 h + 8 q + e.
 #pragma once
 #include "gemm_bf16_common.h"
+#include "x32w4_loop.h"
 
 namespace mi {
 
@@ -30,6 +31,7 @@ struct Tile16 {
   long long batchA, batchB;  // elements between the operands of consecutive batch entries
   int lda, ldb, M, N, K;
   int tiles_m, tiles_n;
+  int tile;       // rows and columns of a tile
   int splits;     // the K steps are dealt to this many workgroups per tile; blockIdx.z = entry * splits + split
   int symmetric;  // only tiles with tile_m >= tile_n are launched (square results, BM == BN)
 };
@@ -100,7 +102,7 @@ __device__ __forceinline__ void store_transposed(u16* __restrict__ dst, size_t l
 // global -> LDS loads, one barrier per K step of 64.  At the top of step t the tile of step t has landed
 // (the counter retires loads in order) and every wavefront is done with the buffer of step t - 1, which
 // takes the tile of step t + STAGES - 1.
-template <bool F16, int BM, int BN, int WM, int WN, int STAGES, class Epi>
+template <int BM, int BN, int WM, int WN, int STAGES>
 struct TileKernel {
   static constexpr int NW = WM * WN, QB = BM / WM / 16, BK = 64;
   static constexpr int A_ELEMS = BM * BK, B_ELEMS = BN * BK, BUF = A_ELEMS + B_ELEMS;
@@ -111,12 +113,9 @@ struct TileKernel {
   static_assert(BN / WN == 64 && BM % (8 * NW) == 0 && BN % (8 * NW) == 0 && LDS <= 160 * 1024, "tile shape");
 };
 
-__device__ __forceinline__ int swz16_a(int row) { return (row >> 1) & 7; }
-__device__ __forceinline__ int swz16_b(int row) { return ((row >> 3) & 3) * 2 + ((row >> 1) & 1); }
-
 template <bool F16, int BM, int BN, int WM, int WN, int STAGES, class Epi>
 __global__ __launch_bounds__(WM* WN * 64) void tile16_kernel(Tile16 p, typename Epi::Args e) {
-  using K_ = TileKernel<F16, BM, BN, WM, WN, STAGES, Epi>;
+  using K_ = TileKernel<BM, BN, WM, WN, STAGES>;
   constexpr int NW = K_::NW, QB = K_::QB, BK = K_::BK;
   using frag = std::conditional_t<F16, f16x8, bf16x8>;
   typedef __attribute__((address_space(3))) const frag lds_frag_t;
@@ -138,12 +137,12 @@ __global__ __launch_bounds__(WM* WN * 64) void tile16_kernel(Tile16 p, typename 
 #pragma unroll
   for (int j = 0; j < K_::NIA; ++j) {
     const int row = (j * NW + wave) * 8 + lrow, real = m0 + row < p.M ? row : p.M - 1 - m0;
-    offa[j] = 2u * ((unsigned)real * (unsigned)p.lda + (unsigned)(pc ^ swz16_a(row)) * 8u);
+    offa[j] = 2u * ((unsigned)real * (unsigned)p.lda + (unsigned)(pc ^ x32::swz_a(row)) * 8u);
   }
 #pragma unroll
   for (int j = 0; j < K_::NIB; ++j) {
     const int row = (j * NW + wave) * 8 + lrow, real = n0 + row < p.N ? row : p.N - 1 - n0;
-    offb[j] = 2u * ((unsigned)real * (unsigned)p.ldb + (unsigned)(pc ^ swz16_b(row)) * 8u);
+    offb[j] = 2u * ((unsigned)real * (unsigned)p.ldb + (unsigned)(pc ^ x32::swz_b(row)) * 8u);
   }
   const u16* a = p.A + (size_t)entry * p.batchA + (size_t)m0 * p.lda + (size_t)k0 * BK;
   const u16* b = p.B + (size_t)entry * p.batchB + (size_t)n0 * p.ldb + (size_t)k0 * BK;
@@ -162,8 +161,8 @@ __global__ __launch_bounds__(WM* WN * 64) void tile16_kernel(Tile16 p, typename 
 #pragma unroll
   for (int kc = 0; kc < 2; ++kc) {
     const int ra = wm0 + l16, rb = wn0 + 8 * (l16 >> 2) + (l16 & 3);
-    qa[kc] = lds_base + 2u * (unsigned)(ra * BK + ((kc * 4 + q) ^ swz16_a(ra)) * 8);
-    pa[kc] = lds_base + 2u * (unsigned)(K_::A_ELEMS + rb * BK + ((kc * 4 + q) ^ swz16_b(rb)) * 8);
+    qa[kc] = lds_base + 2u * (unsigned)(ra * BK + ((kc * 4 + q) ^ x32::swz_a(ra)) * 8);
+    pa[kc] = lds_base + 2u * (unsigned)(K_::A_ELEMS + rb * BK + ((kc * 4 + q) ^ x32::swz_b(rb)) * 8);
   }
   f32x4 acc[QB][4];
 #pragma unroll
@@ -208,18 +207,63 @@ __global__ __launch_bounds__(WM* WN * 64) void tile16_kernel(Tile16 p, typename 
   Epi::template run<QB>(e, p, get, m0 + wm0, n0 + wn0, lane, stage, entry, split);
 }
 
-template <bool F16, int BM, int BN, int WM, int WN, int STAGES, class Epi>
+// The same on tiles of 256 x 256 with four wavefronts of 128 x 128 and the hand-ordered K loop.
+template <bool F16, class Epi>
+__global__ __launch_bounds__(x32::W4_NW * 64) void tile256_kernel(Tile16 p, typename Epi::Args e) {
+  extern __shared__ __attribute__((aligned(16))) u16 smem_t[];
+  const unsigned lds_base = __builtin_amdgcn_readfirstlane((unsigned)(size_t)((__attribute__((address_space(3))) const void*)smem_t));
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  int tm, tn;
+  tile16_of_workgroup(p, blockIdx.x, gridDim.x, tm, tn);
+  const int m0 = tm * x32::BM, n0 = tn * x32::BN;
+  const int entry = blockIdx.z / p.splits, split = blockIdx.z - entry * p.splits;
+  const int steps = p.K / x32::BK;
+  const int k0 = (int)((long long)steps * split / p.splits), nk = (int)((long long)steps * (split + 1) / p.splits) - k0;
+  f32x4 acc[2][x32::QB][4];
+  const x32::W4Operands op{p.A + (size_t)entry * p.batchA + (size_t)m0 * p.lda + (size_t)k0 * x32::BK,
+                           p.B + (size_t)entry * p.batchB + (size_t)n0 * p.ldb + (size_t)k0 * x32::BK,
+                           p.lda, p.ldb, p.M - m0, p.N - n0};
+  x32::w4_loop<false, F16, true>(op, nk, lds_base, wave, lane, acc);
+  __syncthreads();  // every wavefront is done with the operand tiles: the epilogue may use the LDS
+  unsigned char* stage = reinterpret_cast<unsigned char*>(smem_t) + (size_t)wave * x32::STAGE_REGION;
+  // made opaque, so that none of the epilogue's addresses is computed ahead of the K loop and kept through it
+  int lane_e = lane, row_e = m0 + wave / x32::W4_WN * x32::WTM, col_e = n0 + wave % x32::W4_WN * x32::W4_WTN;
+  asm volatile("" : "+v"(lane_e), "+s"(row_e), "+s"(col_e));
+  // the accumulators are read out of the AGPRs where they are used (one register each, not 256 at once)
+  auto half = [&](auto h_c) __attribute__((always_inline)) {
+    constexpr int hc = decltype(h_c)::value;
+    auto get = [&](int jq, int h, int i) __attribute__((always_inline)) {
+      float v;
+      asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(v) : "a"(acc[hc][jq][2 * h + (i >> 2)][i & 3]));
+      return v;
+    };
+    Epi::template run<x32::QB>(e, p, get, row_e, col_e + 64 * hc, lane_e, stage, entry, split);
+  };
+  half(std::integral_constant<int, 0>{});
+  half(std::integral_constant<int, 1>{});
+}
+
+// p.tile: 128 or 256.
+template <bool F16, class Epi>
 hipError_t launch_tile16(Tile16 p, const typename Epi::Args& e, int batch, hipStream_t s) {
-  using K_ = TileKernel<F16, BM, BN, WM, WN, STAGES, Epi>;
-  p.tiles_m = (p.M + BM - 1) / BM;
-  p.tiles_n = (p.N + BN - 1) / BN;
+  p.tiles_m = (p.M + p.tile - 1) / p.tile;
+  p.tiles_n = (p.N + p.tile - 1) / p.tile;
   const long long total = p.symmetric ? (long long)p.tiles_m * (p.tiles_m + 1) / 2 : (long long)p.tiles_m * p.tiles_n;
   if (total <= 0 || batch <= 0) return hipSuccess;
-  if (total > 0x7fffffffLL / 2 || (long long)batch * p.splits > 65535) return hipErrorInvalidValue;
-  auto kern = tile16_kernel<F16, BM, BN, WM, WN, STAGES, Epi>;
-  static LdsOptIn opt_in;
-  if (hipError_t err = opt_in.ensure(reinterpret_cast<const void*>(kern), K_::LDS); err != hipSuccess) return err;
-  launch_kernel(kern, dim3((unsigned)total, 1, batch * p.splits), dim3(WM * WN * 64), K_::LDS, s, p, e);
+  if (total > 0x3fffffff || (long long)batch * p.splits > 65535) return hipErrorInvalidValue;
+  const dim3 grid((unsigned)total, 1, batch * p.splits);
+  if (p.tile == 256) {
+    auto kern = tile256_kernel<F16, Epi>;
+    static LdsOptIn opt_in;
+    if (hipError_t err = opt_in.ensure(reinterpret_cast<const void*>(kern), x32::LDS_BYTES); err != hipSuccess) return err;
+    launch_kernel(kern, grid, dim3(x32::W4_NW * 64), x32::LDS_BYTES, s, p, e);
+  } else {
+    using K_ = TileKernel<128, 128, 2, 2, 2>;
+    auto kern = tile16_kernel<F16, 128, 128, 2, 2, 2, Epi>;
+    static LdsOptIn opt_in;
+    if (hipError_t err = opt_in.ensure(reinterpret_cast<const void*>(kern), K_::LDS); err != hipSuccess) return err;
+    launch_kernel(kern, grid, dim3(256), K_::LDS, s, p, e);
+  }
   return hipGetLastError();
 }
 

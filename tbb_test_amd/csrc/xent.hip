@@ -127,11 +127,12 @@ struct EpiGrad {
     const int* target;
     const float* lse;
     const float* dloss;  // null: 1 for every row
+    const float* top;    // g is kept divided by *top, the largest |dloss| (see xent_top_kernel)
     int first, vocab;
     u16* G;              // [rows padded][ldg]
     u16* GT;             // [columns padded][ldgt]
     int ldg, ldgt;
-    float* db_part;      // [row0 / (16 QB)][ldg] or null
+    float* db_part;      // column sums per wavefront tile of 16 QB rows, [row0 / (16 QB)][ldg], or null
   };
   template <int QB, class Get>
   static __device__ __forceinline__ void run(const Args& e, const Tile16& p, Get get, int row0, int colw, int lane,
@@ -147,6 +148,7 @@ struct EpiGrad {
         sums[h][i] = 0.0f;
       }
     const bool edge = colw + 64 > p.N;
+    const float inv_top = e.dloss ? 1.0f / *e.top : 1.0f;
     u32x4 pk[QB][2];
 #pragma unroll
     for (int jq = 0; jq < QB; ++jq) {
@@ -155,7 +157,7 @@ struct EpiGrad {
       const bool live = t >= 0 && t < e.vocab;
       t = t - e.first - lane_col;
       const float lse = live ? e.lse[row] : 0.0f;
-      const float d = live ? (e.dloss ? e.dloss[row] : 1.0f) : 0.0f;
+      const float d = live ? (e.dloss ? e.dloss[row] * inv_top : 1.0f) : 0.0f;
       float g[2][8];
 #pragma unroll
       for (int h = 0; h < 2; ++h)
@@ -214,11 +216,13 @@ struct EpiOut {
     int ldc;
     int vec;         // 16-byte stores allowed
     int add;         // fp32: C += instead of C =
+    const float* factor;  // of the result, or null
   };
   template <int QB, class Get>
   static __device__ __forceinline__ void run(const Args& e, const Tile16& p, Get get, int row0, int colw, int lane,
                                              unsigned char*, int, int split) {
     const int l16 = lane & 15, col0 = colw + 8 * (lane >> 4);
+    const float factor = e.factor ? *e.factor : 1.0f;
 #pragma unroll
     for (int jq = 0; jq < QB; ++jq) {
       const int row = row0 + 16 * jq + l16;
@@ -230,7 +234,7 @@ struct EpiOut {
         const size_t at = (size_t)split * e.slab + (size_t)row * e.ldc + col;
         float v[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = get(jq, h, i);
+        for (int i = 0; i < 8; ++i) v[i] = factor * get(jq, h, i);
         const bool whole = e.vec && col + 8 <= p.N;
         if constexpr (OUT_BF16) {
           u16* c = reinterpret_cast<u16*>(e.C) + at;
@@ -264,15 +268,17 @@ struct EpiOut {
   }
 };
 
-constexpr int TB = 128;  // rows and columns of a tile: what padded sizes are multiples of
+// 256 x 256 tiles once there are enough of them for most of the 256 CUs, else 128 x 128.
+int tile_for(size_t rows, size_t cols) { return ((rows + 255) / 256) * ((cols + 255) / 256) >= 200 ? 256 : 128; }
 
 template <class Epi>
-hipError_t tiles(const u16* A, int lda, const u16* B, int ldb, int M, int N, int K, int splits, const typename Epi::Args& e,
+hipError_t tiles(int tile, const u16* A, int lda, const u16* B, int ldb, int M, int N, int K, int splits, const typename Epi::Args& e,
                  hipStream_t s) {
   Tile16 p{};
   p.A = A; p.B = B; p.lda = lda; p.ldb = ldb; p.M = M; p.N = N; p.K = K;
   p.splits = splits;
-  return launch_tile16<false, TB, TB, 2, 2, 2, Epi>(p, e, 1, s);
+  p.tile = tile;
+  return launch_tile16<false, Epi>(p, e, 1, s);
 }
 
 // ---- joins and copies -------------------------------------------------------------------------------
@@ -297,6 +303,28 @@ __global__ __launch_bounds__(256) void xent_fold_kernel(const float2* __restrict
   const int t = target[row];
   const bool counts = t >= 0 && t < vocab;
   finish_row(m, s, counts, counts ? zt[row] : 0.0f, loss + row, lse + row);
+}
+
+// *top = the largest |dloss| of the rows that count (1 if that is zero).  g is rounded to bf16 divided by it:
+// with the mean's weights, all the same, a rounding of 1 / count would shift every term the same way and
+// not average out in the sums over rows and classes.  One workgroup.
+__global__ __launch_bounds__(1024) void xent_top_kernel(const float* __restrict__ dloss, const int* __restrict__ target, int M,
+                                                        int vocab, float* __restrict__ top) {
+  __shared__ float red[1024];
+  float m = 0.0f;
+  for (int i = threadIdx.x; i < M; i += 1024) {
+    const int t = target[i];
+    const float d = fabsf(dloss[i]);
+    if (t >= 0 && t < vocab && d < __builtin_inff()) m = fmaxf(m, d);
+  }
+  red[threadIdx.x] = m;
+  __syncthreads();
+  for (int off = 512; off > 0; off >>= 1) {
+    if ((int)threadIdx.x < off) red[threadIdx.x] = fmaxf(red[threadIdx.x], red[threadIdx.x + off]);
+    __syncthreads();
+  }
+  // (below the smallest normal number the quotients could overflow)
+  if (threadIdx.x == 0) *top = red[0] >= 1.17549435e-38f ? red[0] : 1.0f;
 }
 
 // dst[rows][ldd] = src[rows][cols], zeros up to ldd.
@@ -340,10 +368,11 @@ __global__ __launch_bounds__(256) void pack_transposed_kernel(u16* __restrict__ 
   }
 }
 
-// C[row][col] = sum over slabs, in slab order, of part[slab][row][col] (fp32), to fp32 or bf16.
+// C[row][col] = factor * sum over slabs, in slab order, of part[slab][row][col] (fp32), to fp32 or bf16.
 template <bool OUT_BF16>
 __global__ __launch_bounds__(256) void fold_slabs_kernel(void* __restrict__ C, int ldc, const float* __restrict__ part, int ldp,
-                                                         long long slab, int slabs, int rows, int cols) {
+                                                         long long slab, int slabs, int rows, int cols,
+                                                         const float* __restrict__ factor) {
   const size_t n = (size_t)rows * cols, step = (size_t)gridDim.x * 256;
   for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += step) {
     const size_t r = i / cols;
@@ -351,19 +380,20 @@ __global__ __launch_bounds__(256) void fold_slabs_kernel(void* __restrict__ C, i
     const float* src = part + r * ldp + c;
     float v = 0.0f;
     for (int k = 0; k < slabs; ++k) v += src[(size_t)k * slab];
+    if (factor) v *= *factor;
     if constexpr (OUT_BF16) reinterpret_cast<u16*>(C)[r * ldc + c] = f2bf(v);
     else reinterpret_cast<float*>(C)[r * ldc + c] = v;
   }
 }
 
-// out[c] = sum over blocks of part[block][c]
+// out[c] = factor * sum over blocks of part[block][c]
 __global__ __launch_bounds__(256) void fold_columns_kernel(float* __restrict__ out, const float* __restrict__ part, int ld,
-                                                           int blocks, int cols) {
+                                                           int blocks, int cols, const float* __restrict__ factor) {
   const int c = blockIdx.x * 256 + threadIdx.x;
   if (c >= cols) return;
   float v = 0.0f;
   for (int b = 0; b < blocks; ++b) v += part[(size_t)b * ld + c];
-  out[c] = v;
+  out[c] = factor ? v * *factor : v;
 }
 
 // ---- fp32 models ------------------------------------------------------------------------------------
@@ -462,7 +492,7 @@ ForwardPlan plan_forward(char* base, int M, int V, int K) {
   ForwardPlan f{};
   Carver c{base};
   f.Kp = (int)up(K, 64);
-  f.pack_cols = (int)std::min<size_t>(up(V, TB), std::max<size_t>(((size_t)1 << 24) / f.Kp / TB * TB, TB));
+  f.pack_cols = (int)std::min<size_t>(up(V, 64), std::max<size_t>(((size_t)1 << 24) / f.Kp / 256 * 256, 256));
   f.Xp = c.take<u16>((size_t)M * f.Kp);
   f.Wp = c.take<u16>((size_t)std::min(V, f.pack_cols) * f.Kp);
   f.zt = c.take<float>(M);
@@ -473,27 +503,36 @@ ForwardPlan plan_forward(char* base, int M, int V, int K) {
 
 struct BackwardPlan {
   int Kp, Mp, piece, splits_x, splits_w;
+  int tile;        // of the launch that makes g; Mp and the pieces are multiples of it
+  int tile_x, tile_w;
   bool sum_x;      // dX comes out of fp32 slabs
   u16 *Xp, *Xt, *Wp, *Wt, *G, *GT;
-  float *db_part, *x_part, *w_part;
+  float *top, *db_part, *x_part, *w_part;
   size_t bytes;
 };
-int splits_for(size_t rows, size_t cols, size_t steps) {
-  const size_t n = up(rows, TB) / TB * (up(cols, TB) / TB);
-  // enough workgroups for the 256 CUs, but at least eight K steps for each
-  return (int)std::max<size_t>(1, std::min<size_t>({(256 + n - 1) / n, steps / 8, 64}));
+// Tile and K splits of a product whose result is rows x cols: 256 x 256 tiles where they fill the CUs by
+// themselves, else 128 x 128 with the K steps dealt out to reach the 256 CUs, at least eight to each.
+void shape_product(size_t rows, size_t cols, size_t steps, int* tile, int* splits) {
+  *tile = tile_for(rows, cols);
+  *splits = 1;
+  if (*tile == 256) return;
+  const size_t n = (rows + 127) / 128 * ((cols + 127) / 128);
+  *splits = (int)std::max<size_t>(1, std::min<size_t>({(256 + n - 1) / n, steps / 8, 64}));
 }
 BackwardPlan plan_backward(char* base, int M, int V, int K) {
   BackwardPlan b{};
   Carver c{base};
   b.Kp = (int)up(K, 64);
-  b.Mp = (int)up(M, TB);
   // g and g^T of a piece take at most 2 x 512 MB, the copies of W's piece 256 MB each
-  const size_t most = std::min(((size_t)1 << 28) / b.Mp, ((size_t)1 << 27) / b.Kp) / 256 * 256;
-  b.piece = (int)std::min<size_t>(up(V, TB), std::max<size_t>(most, 256));
-  b.splits_x = splits_for(M, K, b.piece / 64);
-  b.splits_w = splits_for(b.piece, K, b.Mp / 64);
+  const size_t most = std::min(((size_t)1 << 28) / up(M, 256), ((size_t)1 << 27) / b.Kp) / 256 * 256;
+  const size_t widest = std::max<size_t>(most, 256);
+  b.tile = tile_for(M, std::min<size_t>(V, widest));
+  b.Mp = (int)up(M, b.tile);
+  b.piece = (int)std::min<size_t>(up(V, b.tile), widest);
+  shape_product(M, K, b.piece / 64, &b.tile_x, &b.splits_x);
+  shape_product(b.piece, K, b.Mp / 64, &b.tile_w, &b.splits_w);
   b.sum_x = b.splits_x > 1 || b.piece < V;
+  b.top = c.take<float>(1);
   b.Xp = c.take<u16>((size_t)M * b.Kp);
   b.Xt = c.take<u16>((size_t)K * b.Mp);
   b.Wp = c.take<u16>((size_t)std::min(V, b.piece) * b.Kp);
@@ -575,7 +614,7 @@ hipError_t xent_forward_bf16(int M, int V, int K, const u16* X, int ldx, const u
       w = f.Wp;
     }
     const EpiStats::Args e{bias ? bias + v0 : nullptr, target, v0, V, f.zt, f.part + (size_t)(v0 / 64) * M};
-    TRY(tiles<EpiStats>(X, ldx, w, w_direct ? ldw : f.Kp, M, cols, f.Kp, 1, e, s));
+    TRY(tiles<EpiStats>(tile_for(M, cols), X, ldx, w, w_direct ? ldw : f.Kp, M, cols, f.Kp, 1, e, s));
   }
   launch_kernel(xent_fold_kernel, dim3((M + 15) / 16), dim3(256), 0, s, (const float2*)f.part, (int)(up(V, 64) / 64), M, V,
                 target, (const float*)f.zt, loss, lse);
@@ -587,6 +626,11 @@ hipError_t xent_backward_bf16(int M, int V, int K, const u16* X, int ldx, const 
                               bool dw_bf16, void* dW, int lddw, float* db, void* ws, hipStream_t s) {
   const BackwardPlan b = plan_backward(static_cast<char*>(ws), M, V, K);
   const bool x_direct = direct(X, ldx, K), w_direct = direct(W, ldw, K);
+  const float* top = dloss ? b.top : nullptr;
+  if (dloss) {
+    launch_kernel(xent_top_kernel, dim3(1), dim3(1024), 0, s, dloss, target, M, V, b.top);
+    TRY(hipGetLastError());
+  }
   TRY(pack_transposed(b.Xt, X, M, K, ldx, b.Mp, s));
   if (!x_direct) {
     TRY(pack_rows(b.Xp, X, M, K, ldx, b.Kp, s));
@@ -594,7 +638,7 @@ hipError_t xent_backward_bf16(int M, int V, int K, const u16* X, int ldx, const 
     ldx = b.Kp;
   }
   for (int v0 = 0; v0 < V; v0 += b.piece) {
-    const int cols = std::min(b.piece, V - v0), padded = (int)up(cols, TB), steps = (int)up(cols, 64) / 64;
+    const int cols = std::min(b.piece, V - v0), padded = (int)up(cols, b.tile), steps = (int)up(cols, 64) / 64;
     const u16* w = W + (size_t)v0 * ldw;
     int ld_w = ldw;
     if (!w_direct) {
@@ -602,11 +646,11 @@ hipError_t xent_backward_bf16(int M, int V, int K, const u16* X, int ldx, const 
       w = b.Wp;
       ld_w = b.Kp;
     }
-    const EpiGrad::Args g{bias ? bias + v0 : nullptr, target, lse, dloss, v0, V, b.G, b.GT, padded, b.Mp, db ? b.db_part : nullptr};
-    TRY(tiles<EpiGrad>(X, ldx, w, ld_w, M, cols, b.Kp, 1, g, s));
+    const EpiGrad::Args g{bias ? bias + v0 : nullptr, target, lse, dloss, top, v0, V, b.G, b.GT, padded, b.Mp, db ? b.db_part : nullptr};
+    TRY(tiles<EpiGrad>(b.tile, X, ldx, w, ld_w, M, cols, b.Kp, 1, g, s));
     if (db) {
       launch_kernel(fold_columns_kernel, dim3((cols + 255) / 256), dim3(256), 0, s, db + v0, (const float*)b.db_part, padded,
-                    b.Mp / 64, cols);
+                    b.Mp / (b.tile / 2), cols, top);
       TRY(hipGetLastError());
     }
     // dX (+)= g W: the caller's transposed copy where whole 16-byte chunks of it can be read
@@ -619,37 +663,37 @@ hipError_t xent_backward_bf16(int M, int V, int K, const u16* X, int ldx, const 
     }
     if (b.sum_x) {
       const int splits = std::min(b.splits_x, steps);
-      const EpiOut<false>::Args e{b.x_part, (long long)M * b.Kp, b.Kp, 1, v0 > 0};
-      TRY(tiles<EpiOut<false>>(b.G, padded, wt, ld_t, M, K, steps * 64, splits, e, s));
+      const EpiOut<false>::Args e{b.x_part, (long long)M * b.Kp, b.Kp, 1, v0 > 0, nullptr};
+      TRY(tiles<EpiOut<false>>(b.tile_x, b.G, padded, wt, ld_t, M, K, steps * 64, splits, e, s));
     } else {
-      const EpiOut<true>::Args e{dX, 0, lddx, al16(dX) && lddx % 8 == 0, 0};
-      TRY(tiles<EpiOut<true>>(b.G, padded, wt, ld_t, M, K, steps * 64, 1, e, s));
+      const EpiOut<true>::Args e{dX, 0, lddx, al16(dX) && lddx % 8 == 0, 0, top};
+      TRY(tiles<EpiOut<true>>(b.tile_x, b.G, padded, wt, ld_t, M, K, steps * 64, 1, e, s));
     }
     // dW = g^T X
     void* dw = static_cast<char*>(dW) + (size_t)v0 * lddw * (dw_bf16 ? 2 : 4);
     if (b.splits_w > 1) {
-      const EpiOut<false>::Args e{b.w_part, (long long)b.piece * b.Kp, b.Kp, 1, 0};
-      TRY(tiles<EpiOut<false>>(b.GT, b.Mp, b.Xt, b.Mp, cols, K, b.Mp, b.splits_w, e, s));
+      const EpiOut<false>::Args e{b.w_part, (long long)b.piece * b.Kp, b.Kp, 1, 0, nullptr};
+      TRY(tiles<EpiOut<false>>(b.tile_w, b.GT, b.Mp, b.Xt, b.Mp, cols, K, b.Mp, b.splits_w, e, s));
       const dim3 grid(flat_grid((size_t)cols * K));
       if (dw_bf16)
         launch_kernel(fold_slabs_kernel<true>, grid, dim3(256), 0, s, dw, lddw, (const float*)b.w_part, b.Kp,
-                      (long long)b.piece * b.Kp, b.splits_w, cols, K);
+                      (long long)b.piece * b.Kp, b.splits_w, cols, K, top);
       else
         launch_kernel(fold_slabs_kernel<false>, grid, dim3(256), 0, s, dw, lddw, (const float*)b.w_part, b.Kp,
-                      (long long)b.piece * b.Kp, b.splits_w, cols, K);
+                      (long long)b.piece * b.Kp, b.splits_w, cols, K, top);
       TRY(hipGetLastError());
     } else if (dw_bf16) {
-      const EpiOut<true>::Args e{dw, 0, lddw, al16(dw) && lddw % 8 == 0, 0};
-      TRY(tiles<EpiOut<true>>(b.GT, b.Mp, b.Xt, b.Mp, cols, K, b.Mp, 1, e, s));
+      const EpiOut<true>::Args e{dw, 0, lddw, al16(dw) && lddw % 8 == 0, 0, top};
+      TRY(tiles<EpiOut<true>>(b.tile_w, b.GT, b.Mp, b.Xt, b.Mp, cols, K, b.Mp, 1, e, s));
     } else {
-      const EpiOut<false>::Args e{dw, 0, lddw, al16(dw) && lddw % 4 == 0, 0};
-      TRY(tiles<EpiOut<false>>(b.GT, b.Mp, b.Xt, b.Mp, cols, K, b.Mp, 1, e, s));
+      const EpiOut<false>::Args e{dw, 0, lddw, al16(dw) && lddw % 4 == 0, 0, top};
+      TRY(tiles<EpiOut<false>>(b.tile_w, b.GT, b.Mp, b.Xt, b.Mp, cols, K, b.Mp, 1, e, s));
     }
   }
   if (b.sum_x) {
     // the last piece may have had fewer splits than there are slabs; the first piece wrote them all
     launch_kernel(fold_slabs_kernel<true>, dim3(flat_grid((size_t)M * K)), dim3(256), 0, s, (void*)dX, lddx,
-                  (const float*)b.x_part, b.Kp, (long long)M * b.Kp, std::min(b.splits_x, (int)up(std::min(b.piece, V), 64) / 64), M, K);
+                  (const float*)b.x_part, b.Kp, (long long)M * b.Kp, std::min(b.splits_x, (int)up(std::min(b.piece, V), 64) / 64), M, K, top);
     TRY(hipGetLastError());
   }
   return hipSuccess;

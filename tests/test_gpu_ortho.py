@@ -141,6 +141,14 @@ def test_batch_with_strides(rows, cols, dtype):
         near(o, newton_schulz(g), OUT, 2.0 ** -8)
 
 
+@pytest.mark.parametrize("rows,cols", [(300, 520), (520, 300)])
+def test_large_tiles(rows, cols):
+    rng = np.random.default_rng(12)
+    G = np.stack([gradient(rng, rows, cols) for _ in range(70)])  # together enough 256 x 256 tiles to fill the device
+    for o, g in zip(run(G, capi.MI_F32), G):
+        near(o, newton_schulz(g), OUT, 2.0 ** -8)
+
+
 def test_singular_values_end_near_one():
     G = gradient(np.random.default_rng(8), 256, 400, "noise")
     s = np.linalg.svd(run(G[None], capi.MI_F32)[0], compute_uv=False)

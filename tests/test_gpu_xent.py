@@ -235,6 +235,16 @@ def test_fp32_logits_in_several_pieces():
     check_backward(p, capi.MI_F32)
 
 
+@pytest.mark.parametrize("M,V,K", [(4000, 3400, 64),    # the tiles of the logits fill the device
+                                   (300, 4090, 3600),   # those of the weight gradient do
+                                   (4090, 200, 3400)])  # those of the input gradient do
+def test_large_tiles(M, V, K):
+    p = Problem(capi.MI_BF16, M, V, K)
+    check_forward(p)
+    check_backward(p, capi.MI_BF16)
+    check_backward(p, capi.MI_F32, dloss=False)
+
+
 @pytest.mark.parametrize("dtype", [capi.MI_BF16, capi.MI_F32], ids=["bf16", "f32"])
 def test_classes_and_rows_that_are_switched_off(dtype):
     def tweak(X, W, b, t, d):
