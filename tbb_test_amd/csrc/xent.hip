@@ -368,11 +368,12 @@ __global__ __launch_bounds__(256) void pack_transposed_kernel(u16* __restrict__ 
   }
 }
 
-// C[row][col] = factor * sum over slabs, in slab order, of part[slab][row][col] (fp32), to fp32 or bf16.
+// C[row][col] = factor * sum over slabs, in slab order, of part[slab][row][col] (fp32), to fp32 (add: on top of what C
+// holds) or bf16.
 template <bool OUT_BF16>
 __global__ __launch_bounds__(256) void fold_slabs_kernel(void* __restrict__ C, int ldc, const float* __restrict__ part, int ldp,
                                                          long long slab, int slabs, int rows, int cols,
-                                                         const float* __restrict__ factor) {
+                                                         const float* __restrict__ factor, int add) {
   const size_t n = (size_t)rows * cols, step = (size_t)gridDim.x * 256;
   for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += step) {
     const size_t r = i / cols;
@@ -382,7 +383,7 @@ __global__ __launch_bounds__(256) void fold_slabs_kernel(void* __restrict__ C, i
     for (int k = 0; k < slabs; ++k) v += src[(size_t)k * slab];
     if (factor) v *= *factor;
     if constexpr (OUT_BF16) reinterpret_cast<u16*>(C)[r * ldc + c] = f2bf(v);
-    else reinterpret_cast<float*>(C)[r * ldc + c] = v;
+    else reinterpret_cast<float*>(C)[r * ldc + c] = add ? reinterpret_cast<float*>(C)[r * ldc + c] + v : v;
   }
 }
 
@@ -398,11 +399,22 @@ __global__ __launch_bounds__(256) void fold_columns_kernel(float* __restrict__ o
 
 // ---- fp32 models ------------------------------------------------------------------------------------
 
-// Statistics of one piece of logits Z [M x cols], joined to those of the pieces before (first: none).
-// One workgroup per row; `last` turns them into loss and lse.
+// dst[rows_p][cols_p] = src[rows][cols], zeros around it.
+__global__ __launch_bounds__(256) void pad_f32_kernel(float* __restrict__ dst, const float* __restrict__ src, int rows, int cols,
+                                                      int ld, int rows_p, int cols_p) {
+  const size_t n = (size_t)rows_p * cols_p, step = (size_t)gridDim.x * 256;
+  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += step) {
+    const int r = (int)(i / cols_p), c = (int)(i - (size_t)r * cols_p);
+    dst[i] = r < rows && c < cols ? src[(size_t)r * ld + c] : 0.0f;
+  }
+}
+
+// Statistics of one piece of products Z [M x cols] (the bias is added here), joined to those of the pieces
+// before (first = 0: none).  One workgroup per row, one pass; `last` turns them into loss and lse.
 __global__ __launch_bounds__(256) void xent_rows_f32_kernel(const float* __restrict__ Z, int ldz, int cols, int first, int vocab,
-                                                            int last, const int* __restrict__ target, float2* __restrict__ part,
-                                                            float* __restrict__ zt, float* __restrict__ loss, float* __restrict__ lse) {
+                                                            int last, const float* __restrict__ bias, const int* __restrict__ target,
+                                                            float2* __restrict__ part, float* __restrict__ zt,
+                                                            float* __restrict__ loss, float* __restrict__ lse) {
   __shared__ float2 red[256];
   const int row = blockIdx.x, tid = threadIdx.x;
   int t = target[row];
@@ -410,9 +422,19 @@ __global__ __launch_bounds__(256) void xent_rows_f32_kernel(const float* __restr
   t = counts ? t - first : -1;
   const float* z = Z + (size_t)row * ldz;
   float m = -__builtin_inff(), s = 0.0f;
-  for (int c = tid; c < cols; c += 256) {
-    if (c == t) continue;
-    join(m, s, z[c], __builtin_isinf(z[c]) ? (z[c] > 0.0f ? __builtin_inff() : 0.0f) : z[c] - z[c] + 1.0f);
+  for (int c = 4 * tid; c < cols; c += 1024) {
+    const f32x4 four = *reinterpret_cast<const f32x4*>(z + c);  // rows are padded to whole quadruples
+    float v[4], top = -__builtin_inff(), sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[i] = four[i] + (bias && c + i < cols ? bias[c + i] : 0.0f);
+      if (c + i >= cols || c + i == t) v[i] = -__builtin_inff();
+      top = fmaxf(top, v[i]);
+    }
+    const float ref = finite_or_zero(top);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum += __builtin_amdgcn_exp2f((v[i] - ref) * LOG2E);
+    join(m, s, top, sum);
   }
   red[tid] = float2{m, s};
   __syncthreads();
@@ -432,34 +454,42 @@ __global__ __launch_bounds__(256) void xent_rows_f32_kernel(const float* __restr
     join(before.x, before.y, all.x, all.y);
     all = before;
   }
-  if (t >= 0 && t < cols) zt[row] = z[t];
+  if (t >= 0 && t < cols) zt[row] = z[t] + (bias ? bias[t] : 0.0f);
   if (last) finish_row(all.x, all.y, counts, counts ? zt[row] : 0.0f, loss + row, lse + row);
   else part[row] = all;
 }
 
-__global__ __launch_bounds__(256) void xent_grad_f32_kernel(float* __restrict__ Z, int ldz, int M, int cols, int first, int vocab,
+// Products of one piece, class by class, Zt [rows_p x Mp] -> g^T in place, zeros around the rows x M that
+// are there; db = its row sums.  One wavefront per class.
+__global__ __launch_bounds__(256) void xent_grad_f32_kernel(float* __restrict__ Zt, int Mp, int M, int rows, int rows_p, int first,
+                                                            int vocab, const float* __restrict__ bias,
                                                             const int* __restrict__ target, const float* __restrict__ lse,
-                                                            const float* __restrict__ dloss) {
-  const size_t n = (size_t)M * cols, step = (size_t)gridDim.x * 256;
-  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += step) {
-    const size_t r = i / cols;
-    const int c = (int)(i - r * cols), t = target[r];
-    float g = 0.0f;
-    if (t >= 0 && t < vocab) {
-      const float x = Z[r * ldz + c] - lse[r];
-      g = (dloss ? dloss[r] : 1.0f) * (c == t - first ? expm1f(x) : expf(x));
+                                                            const float* __restrict__ dloss, float* __restrict__ db) {
+  const int j = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (j >= rows_p) return;
+  float* z = Zt + (size_t)j * Mp;
+  const float add = bias && j < rows ? bias[j] : 0.0f;
+  float sum = 0.0f;
+  for (int i = 4 * lane; i < Mp; i += 256) {
+    f32x4 v = *reinterpret_cast<const f32x4*>(z + i);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      float g = 0.0f;
+      if (j < rows && i + k < M) {
+        const int t = target[i + k];
+        if (t >= 0 && t < vocab) {
+          const float x = v[k] + add - lse[i + k];
+          g = (dloss ? dloss[i + k] : 1.0f) * (t == first + j ? expm1f(x) : __builtin_amdgcn_exp2f(x * LOG2E));
+        }
+      }
+      v[k] = g;
+      sum += g;
     }
-    Z[r * ldz + c] = g;
+    *reinterpret_cast<f32x4*>(z + i) = v;
   }
-}
-
-__global__ __launch_bounds__(256) void add_rows_kernel(float* __restrict__ dst, int ldd, const float* __restrict__ src, int rows,
-                                                       int cols) {
-  const size_t n = (size_t)rows * cols, step = (size_t)gridDim.x * 256;
-  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += step) {
-    const size_t r = i / cols;
-    dst[r * ldd + (i - r * cols)] += src[i];
-  }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
+  if (db && lane == 0 && j < rows) db[j] = sum;
 }
 
 // ---- sizes ------------------------------------------------------------------------------------------
@@ -546,20 +576,33 @@ BackwardPlan plan_backward(char* base, int M, int V, int K) {
   return b;
 }
 
+// fp32: the framework's fp32 GEMMs are fast on whole tiles of aligned operands only, so everything is padded to
+// them; what already is whole is used where it stands.
 struct F32Plan {
-  int piece;
-  float *Z, *zt, *x_part;
+  int Mp, Kp, piece;
+  int splits;       // of the classes, for dX
+  float *Xp, *Wp, *Z, *zt, *x_part, *w_part;
   float2* part;
   size_t bytes;
 };
+int whole_tiles(int n) { return (int)(n >= 128 ? up(n, 128) : up(n, 32)); }
 F32Plan plan_f32(char* base, int M, int V, int K, bool backward) {
   F32Plan f{};
   Carver c{base};
-  const size_t most = std::max<size_t>(((size_t)1 << 28) / M / 64 * 64, 64);  // a piece of logits takes at most 1 GB
-  f.piece = (int)std::min<size_t>(up(V, 64), most);
-  f.Z = c.take<float>((size_t)M * f.piece);
+  f.Mp = whole_tiles(M);
+  f.Kp = whole_tiles(K);
+  // a piece of products and a piece of W take at most 1 GB each
+  const size_t most = std::max<size_t>(((size_t)1 << 28) / std::max(f.Mp, f.Kp) / 128 * 128, 128);
+  f.piece = (int)std::min<size_t>(whole_tiles(V), most);
+  f.Xp = c.take<float>((size_t)f.Mp * f.Kp);
+  f.Wp = c.take<float>((size_t)f.piece * f.Kp);
+  f.Z = c.take<float>((size_t)f.Mp * f.piece);
   if (backward) {
-    if (f.piece < V) f.x_part = c.take<float>((size_t)M * K);
+    const size_t tiles = up(f.Mp, 128) / 128 * (up(f.Kp, 128) / 128);
+    f.splits = tiles > 128 ? 1 : tiles > 64 ? 2 : 4;
+    while (f.piece % (f.splits * 32) != 0) f.splits /= 2;
+    f.x_part = c.take<float>((size_t)f.splits * f.Mp * f.Kp);
+    f.w_part = c.take<float>((size_t)f.piece * f.Kp);
   } else {
     f.zt = c.take<float>(M);
     f.part = c.take<float2>(M);
@@ -677,10 +720,10 @@ hipError_t xent_backward_bf16(int M, int V, int K, const u16* X, int ldx, const 
       const dim3 grid(flat_grid((size_t)cols * K));
       if (dw_bf16)
         launch_kernel(fold_slabs_kernel<true>, grid, dim3(256), 0, s, dw, lddw, (const float*)b.w_part, b.Kp,
-                      (long long)b.piece * b.Kp, b.splits_w, cols, K, top);
+                      (long long)b.piece * b.Kp, b.splits_w, cols, K, top, 0);
       else
         launch_kernel(fold_slabs_kernel<false>, grid, dim3(256), 0, s, dw, lddw, (const float*)b.w_part, b.Kp,
-                      (long long)b.piece * b.Kp, b.splits_w, cols, K, top);
+                      (long long)b.piece * b.Kp, b.splits_w, cols, K, top, 0);
       TRY(hipGetLastError());
     } else if (dw_bf16) {
       const EpiOut<true>::Args e{dw, 0, lddw, al16(dw) && lddw % 8 == 0, 0, top};
@@ -693,42 +736,78 @@ hipError_t xent_backward_bf16(int M, int V, int K, const u16* X, int ldx, const 
   if (b.sum_x) {
     // the last piece may have had fewer splits than there are slabs; the first piece wrote them all
     launch_kernel(fold_slabs_kernel<true>, dim3(flat_grid((size_t)M * K)), dim3(256), 0, s, (void*)dX, lddx,
-                  (const float*)b.x_part, b.Kp, (long long)M * b.Kp, std::min(b.splits_x, (int)up(std::min(b.piece, V), 64) / 64), M, K, top);
+                  (const float*)b.x_part, b.Kp, (long long)M * b.Kp, std::min(b.splits_x, (int)up(std::min(b.piece, V), 64) / 64), M, K, top, 0);
     TRY(hipGetLastError());
   }
   return hipSuccess;
 }
+
+namespace {
+bool whole(const float* q, int ld, int rows, int rows_p, int cols, int cols_p) {
+  return rows == rows_p && cols == cols_p && al16(q) && ld % 4 == 0;
+}
+// An operand in whole tiles: where it stands, or copied to `room`.
+hipError_t whole_operand(const float*& q, int& ld, float* room, int rows, int cols, int rows_p, int cols_p, hipStream_t s) {
+  if (whole(q, ld, rows, rows_p, cols, cols_p)) return hipSuccess;
+  launch_kernel(pad_f32_kernel, dim3(flat_grid((size_t)rows_p * cols_p)), dim3(256), 0, s, room, q, rows, cols, ld, rows_p, cols_p);
+  q = room;
+  ld = cols_p;
+  return hipGetLastError();
+}
+}  // namespace
 
 hipError_t xent_forward_f32(int M, int V, int K, const float* X, int ldx, const float* W, int ldw, const float* bias,
                             const int* target, float* loss, float* lse, void* ws, hipStream_t s) {
   const F32Plan f = plan_f32(static_cast<char*>(ws), M, V, K, false);
+  TRY(whole_operand(X, ldx, f.Xp, M, K, f.Mp, f.Kp, s));
   for (int v0 = 0; v0 < V; v0 += f.piece) {
-    const int cols = std::min(f.piece, V - v0);
-    TRY(sgemm_nt(M, cols, K, X, ldx, W + (size_t)v0 * ldw, ldw, f.Z, f.piece, bias ? bias + v0 : nullptr, 0, s, 0));
-    launch_kernel(xent_rows_f32_kernel, dim3(M), dim3(256), 0, s, (const float*)f.Z, f.piece, cols, v0, V,
-                  (int)(v0 + cols == V), target, f.part, f.zt, loss, lse);
+    const int cols = std::min(f.piece, V - v0), cols_p = whole_tiles(cols);
+    const float* w = W + (size_t)v0 * ldw;
+    int ld_w = ldw;
+    TRY(whole_operand(w, ld_w, f.Wp, cols, K, cols_p, f.Kp, s));
+    TRY(sgemm_nt(f.Mp, cols_p, f.Kp, X, ldx, w, ld_w, f.Z, cols_p, nullptr, 0, s, 0));
+    launch_kernel(xent_rows_f32_kernel, dim3(M), dim3(256), 0, s, (const float*)f.Z, cols_p, cols, v0, V, (int)(v0 + cols == V),
+                  bias ? bias + v0 : nullptr, target, f.part, f.zt, loss, lse);
     TRY(hipGetLastError());
   }
   return hipSuccess;
 }
 
+// The products are made class by class, Z^T = W X^T, so that g^T is at hand as it is for dW = g^T X and as the
+// transposed operand of dX = (g^T)^T W, whose sum over the classes is dealt to `splits` entries of one launch
+// where dX has too few tiles to fill the device.
 hipError_t xent_backward_f32(int M, int V, int K, const float* X, int ldx, const float* W, int ldw, const float* bias,
                              const int* target, const float* lse, const float* dloss, float* dX, int lddx, float* dW, int lddw,
                              float* db, void* ws, hipStream_t s) {
   const F32Plan f = plan_f32(static_cast<char*>(ws), M, V, K, true);
+  TRY(whole_operand(X, ldx, f.Xp, M, K, f.Mp, f.Kp, s));
+  const bool dx_direct = f.splits == 1 && f.piece >= V && whole(dX, lddx, M, f.Mp, K, f.Kp);
   for (int v0 = 0; v0 < V; v0 += f.piece) {
-    const int cols = std::min(f.piece, V - v0);
+    const int cols = std::min(f.piece, V - v0), cols_p = whole_tiles(cols);
     const float* w = W + (size_t)v0 * ldw;
-    TRY(sgemm_nt(M, cols, K, X, ldx, w, ldw, f.Z, f.piece, bias ? bias + v0 : nullptr, 0, s, 0));
-    launch_kernel(xent_grad_f32_kernel, dim3(flat_grid((size_t)M * cols)), dim3(256), 0, s, f.Z, f.piece, M, cols, v0, V, target,
-                  lse, dloss);
+    int ld_w = ldw;
+    TRY(whole_operand(w, ld_w, f.Wp, cols, K, cols_p, f.Kp, s));
+    TRY(sgemm_nt(cols_p, f.Mp, f.Kp, w, ld_w, X, ldx, f.Z, f.Mp, nullptr, 0, s, 0));
+    launch_kernel(xent_grad_f32_kernel, dim3((cols_p + 3) / 4), dim3(256), 0, s, f.Z, f.Mp, M, cols, cols_p, v0, V,
+                  bias ? bias + v0 : nullptr, target, lse, dloss, db ? db + v0 : nullptr);
     TRY(hipGetLastError());
-    TRY(sgemm_nn(M, K, cols, f.Z, f.piece, w, ldw, v0 ? f.x_part : dX, v0 ? K : lddx, nullptr, 0, s, 0));
-    if (v0) {
-      launch_kernel(add_rows_kernel, dim3(flat_grid((size_t)M * K)), dim3(256), 0, s, dX, lddx, (const float*)f.x_part, M, K);
+    const int splits = cols_p % (f.splits * 32) == 0 ? f.splits : 1;
+    float* dx = dx_direct ? dX : f.x_part;
+    TRY(sgemm_tn(splits, f.Mp, f.Kp, cols_p / splits, f.Z, f.Mp, w, ld_w, dx, dx_direct ? lddx : f.Kp, (long long)f.Mp * f.Kp,
+                 nullptr, 0, s, 0));
+    if (!dx_direct) {
+      launch_kernel(fold_slabs_kernel<false>, dim3(flat_grid((size_t)M * K)), dim3(256), 0, s, (void*)dX, lddx,
+                    (const float*)f.x_part, f.Kp, (long long)f.Mp * f.Kp, splits, M, K, (const float*)nullptr, (int)(v0 > 0));
       TRY(hipGetLastError());
     }
-    TRY(sgemm_tn(1, cols, K, M, f.Z, f.piece, X, ldx, dW + (size_t)v0 * lddw, lddw, 0, db ? db + v0 : nullptr, 0, s, 0));
+    float* dw = dW + (size_t)v0 * lddw;
+    const bool dw_direct = whole(dw, lddw, cols, cols_p, K, f.Kp);
+    TRY(sgemm_nn(cols_p, f.Kp, f.Mp, f.Z, f.Mp, X, ldx, dw_direct ? dw : f.w_part, dw_direct ? lddw : f.Kp, nullptr, 0, s, 0));
+    if (!dw_direct) {
+      launch_kernel(fold_slabs_kernel<false>, dim3(flat_grid((size_t)cols * K)), dim3(256), 0, s, (void*)dw, lddw,
+                    (const float*)f.w_part, f.Kp, 0LL, 1, cols, K, (const float*)nullptr, 0);
+      TRY(hipGetLastError());
+    }
   }
   return hipSuccess;
 }
