@@ -15,6 +15,7 @@
 // X is near its limit, stays in fp32 too and joins the a X term; its rounding would be most of what is
 // left.  Together: 2e-4 .. 8e-4 of |O|.
 #include <hip/hip_runtime.h>
+#include <cstdlib>
 
 #include <algorithm>
 
@@ -308,6 +309,7 @@ Plan plan_ortho(char* base, int batch, int rows, int cols) {
   // large matrices: 256 x 256 tiles once even the smallest products (the triangle of m x m) fill the CUs
   const size_t t = up(q.m, 256) / 256;
   q.tile = batch * t * (t + 1) / 2 >= 200 ? 256 : 128;
+  { static int t = getenv("TT") ? atoi(getenv("TT")) : 0; if (t) q.tile = t; }
   q.mp = (int)up(q.m, q.tile);
   q.np = (int)up(q.n, q.tile);
   q.scale = 1.0f;

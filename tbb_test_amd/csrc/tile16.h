@@ -30,9 +30,9 @@ struct Tile16 {
   const u16* B;
   long long batchA, batchB;  // elements between the operands of consecutive batch entries
   int lda, ldb, M, N, K;
-  int tiles_m, tiles_n;
+  int tiles_m, tiles_n, tiles;  // tiles: of one entry and split
   int tile;       // rows and columns of a tile
-  int splits;     // the K steps are dealt to this many workgroups per tile; blockIdx.z = entry * splits + split
+  int splits;     // the K steps are dealt to this many workgroups per tile
   int symmetric;  // only tiles with tile_m >= tile_n are launched (square results, BM == BN)
 };
 
@@ -46,24 +46,36 @@ __device__ __forceinline__ unsigned pack16(float lo, float hi) {
 __device__ __forceinline__ float f16_lo(unsigned v) { return (float)__builtin_bit_cast(f16x2, v)[0]; }
 __device__ __forceinline__ float f16_hi(unsigned v) { return (float)__builtin_bit_cast(f16x2, v)[1]; }
 
-// Workgroup -> tile.  Workgroups go to the 8 XCDs round-robin; each XCD gets one contiguous range of an
-// order in which neighbours share operand panels: bands of eight tile rows, walked column by column (32
-// workgroups of an XCD in flight share eight A panels and four B panels), or the rows of the lower
-// triangle one after another.
-__device__ __forceinline__ void tile16_of_workgroup(const Tile16& p, int id, int total, int& tm, int& tn) {
-  const int xcd = id & 7, rest = total & 7;
-  id = xcd * (total >> 3) + (xcd < rest ? xcd : rest) + (id >> 3);
+// Workgroup -> batch entry, K split and tile.  Workgroups go to the 8 XCDs round-robin; each XCD gets one
+// contiguous range of an order in which neighbours share operand panels: entry by entry, split by split, and within
+// one bands of eight tile rows, walked column by column (32 workgroups of an XCD in flight share eight
+// A panels and four B panels), or the rows of the lower triangle one after another.
+__device__ __forceinline__ void tile16_of_workgroup(const Tile16& p, int& entry, int& split, int& tm, int& tn) {
+  const int total = gridDim.x, xcd = blockIdx.x & 7, rest = total & 7;
+  int id = xcd * (total >> 3) + (xcd < rest ? xcd : rest) + (blockIdx.x >> 3);
+  const int z = __builtin_amdgcn_readfirstlane(id / p.tiles);  // (divisions go through vector registers)
+  id -= z * p.tiles;
+  entry = __builtin_amdgcn_readfirstlane(z / p.splits);
+  split = z - entry * p.splits;
   if (p.symmetric) {
     tm = (int)((__builtin_sqrtf(8.0f * (float)id + 1.0f) - 1.0f) * 0.5f);
     while (tm * (tm + 1) / 2 > id) --tm;  // the root is good to a unit only
     while ((tm + 1) * (tm + 2) / 2 <= id) ++tm;
+    tm = __builtin_amdgcn_readfirstlane(tm);
     tn = id - tm * (tm + 1) / 2;
     return;
   }
-  const int band = id / (8 * p.tiles_n), within = id - band * 8 * p.tiles_n;
+  const int band = __builtin_amdgcn_readfirstlane(id / (8 * p.tiles_n)), within = id - band * 8 * p.tiles_n;
   const int height = p.tiles_m - band * 8 < 8 ? p.tiles_m - band * 8 : 8;
-  tn = within / height;
+  tn = __builtin_amdgcn_readfirstlane(within / height);
   tm = band * 8 + within - tn * height;
+}
+
+// The K steps of a split: first one and number of them.
+__device__ __forceinline__ void tile16_steps(const Tile16& p, int split, int& k0, int& nk) {
+  const int steps = p.K / 64;
+  k0 = __builtin_amdgcn_readfirstlane((int)((long long)steps * split / p.splits));
+  nk = __builtin_amdgcn_readfirstlane((int)((long long)steps * (split + 1) / p.splits)) - k0;
 }
 
 // Transposed store of a wavefront's WTM x 64 packed results: dst[col][row], `ld` elements per column,
@@ -99,9 +111,11 @@ __device__ __forceinline__ void store_transposed(u16* __restrict__ dst, size_t l
 }
 
 // The tile kernel.  WM x WN wavefronts of (BM / WM) x 64; a ring of STAGES LDS buffers filled by direct
-// global -> LDS loads, one barrier per K step of 64.  At the top of step t the tile of step t has landed
-// (the counter retires loads in order) and every wavefront is done with the buffer of step t - 1, which
-// takes the tile of step t + STAGES - 1.
+// global -> LDS loads, one barrier per K step of 64.  Step t multiplies buffer t % STAGES in two K chunks;
+// between them every wavefront has read what it needs of the buffer and the tile of step t + 1 has landed
+// (the counter retires loads in order), then the barrier, then the tile of step t + STAGES is requested
+// into the buffer just read out, and the first fragments of step t + 1 are read under the second chunk's
+// MFMAs.
 template <int BM, int BN, int WM, int WN, int STAGES>
 struct TileKernel {
   static constexpr int NW = WM * WN, QB = BM / WM / 16, BK = 64;
@@ -118,19 +132,17 @@ __global__ __launch_bounds__(WM* WN * 64) void tile16_kernel(Tile16 p, typename 
   using K_ = TileKernel<BM, BN, WM, WN, STAGES>;
   constexpr int NW = K_::NW, QB = K_::QB, BK = K_::BK;
   using frag = std::conditional_t<F16, f16x8, bf16x8>;
-  typedef __attribute__((address_space(3))) const frag lds_frag_t;
   extern __shared__ __attribute__((aligned(16))) u16 smem_t[];
   const unsigned lds_base = __builtin_amdgcn_readfirstlane((unsigned)(size_t)((__attribute__((address_space(3))) const void*)smem_t));
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int l16 = lane & 15, q = lane >> 4;
   const int wm0 = (wave / WN) * (BM / WM), wn0 = (wave % WN) * 64;
 
-  int tm, tn;
-  tile16_of_workgroup(p, blockIdx.x, gridDim.x, tm, tn);
+  int entry, split, tm, tn;
+  tile16_of_workgroup(p, entry, split, tm, tn);
   const int m0 = tm * BM, n0 = tn * BN;
-  const int entry = blockIdx.z / p.splits, split = blockIdx.z - entry * p.splits;
-  const int steps = p.K / BK;
-  const int k0 = (int)((long long)steps * split / p.splits), nk = (int)((long long)steps * (split + 1) / p.splits) - k0;
+  int k0, nk;
+  tile16_steps(p, split, k0, nk);
 
   unsigned offa[K_::NIA], offb[K_::NIB];
   const int lrow = lane >> 3, pc = lane & 7;
@@ -144,17 +156,26 @@ __global__ __launch_bounds__(WM* WN * 64) void tile16_kernel(Tile16 p, typename 
     const int row = (j * NW + wave) * 8 + lrow, real = n0 + row < p.N ? row : p.N - 1 - n0;
     offb[j] = 2u * ((unsigned)real * (unsigned)p.ldb + (unsigned)(pc ^ x32::swz_b(row)) * 8u);
   }
-  const u16* a = p.A + (size_t)entry * p.batchA + (size_t)m0 * p.lda + (size_t)k0 * BK;
-  const u16* b = p.B + (size_t)entry * p.batchB + (size_t)n0 * p.ldb + (size_t)k0 * BK;
-  auto issue = [&](int buf) __attribute__((always_inline)) {
-#pragma unroll
-    for (int j = 0; j < K_::NIA; ++j)
-      load_to_lds_uniform(a, offa[j], lds_base + 2u * (unsigned)(buf * K_::BUF + (j * NW + wave) * 8 * BK));
-#pragma unroll
-    for (int j = 0; j < K_::NIB; ++j)
-      load_to_lds_uniform(b, offb[j], lds_base + 2u * (unsigned)(buf * K_::BUF + K_::A_ELEMS + (j * NW + wave) * 8 * BK));
-    a += BK;
-    b += BK;
+  // the operand bases as scalar values, advanced with scalar additions
+  auto uniform64 = [](const void* q) {
+    const unsigned long long v = reinterpret_cast<unsigned long long>(q);
+    const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)v), hi = __builtin_amdgcn_readfirstlane((unsigned)(v >> 32));
+    return ((unsigned long long)hi << 32) | lo;
+  };
+  unsigned long long a = uniform64(p.A + (size_t)entry * p.batchA + (size_t)m0 * p.lda + (size_t)k0 * BK);
+  unsigned long long b = uniform64(p.B + (size_t)entry * p.batchB + (size_t)n0 * p.ldb + (size_t)k0 * BK);
+  auto to_lds = [](unsigned long long base, unsigned lane_off, unsigned lds) __attribute__((always_inline)) {
+    asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lds), "v"(lane_off), "s"(base) : "memory", "m0");
+  };
+  // load i of the tile that goes into buffer buf: A's, then B's; behind the last one on to the next K step
+  auto load = [&](auto i_c, int buf) __attribute__((always_inline)) {
+    constexpr int i = decltype(i_c)::value;
+    if constexpr (i < K_::NIA) to_lds(a, offa[i], lds_base + 2u * (unsigned)(buf * K_::BUF + (i * NW + wave) * 8 * BK));
+    else to_lds(b, offb[i - K_::NIA], lds_base + 2u * (unsigned)(buf * K_::BUF + K_::A_ELEMS + ((i - K_::NIA) * NW + wave) * 8 * BK));
+    if constexpr (i == K_::INSTR - 1) {
+      a += 2 * BK;
+      b += 2 * BK;
+    }
   };
 
   unsigned qa[2], pa[2];
@@ -170,37 +191,78 @@ __global__ __launch_bounds__(WM* WN * 64) void tile16_kernel(Tile16 p, typename 
 #pragma unroll
     for (int ip = 0; ip < 4; ++ip) acc[jq][ip] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
+  // Fragments of one K chunk of 32, two sets: one multiplied while the other is read.  A chunk is written out as
+  // volatile asm, which keeps its order: MFMAs that accumulate in place (left to itself the compiler rotates the
+  // accumulators through a spare quadruple, four moves and a wait around every MFMA), a fragment read behind each of
+  // the first ones, the tile loads behind the later ones.
+  frag fq[2][QB], fp[2][4];
+  auto read = [&](auto r_c, auto kc_c, unsigned off) __attribute__((always_inline)) {
+    constexpr int r = decltype(r_c)::value, kc = decltype(kc_c)::value;
+    auto& fq_ = fq; auto& fp_ = fp; auto& qa_ = qa; auto& pa_ = pa;  // (named so that the lambda captures them: operands of asm statements alone do not)
+    if constexpr (r < 4)
+      asm volatile("ds_read_b128 %0, %1 offset:%2" : "=&v"(fp_[kc][r]) : "v"(pa_[kc] + off), "i"(2 * (32 * (r >> 1) + 4 * (r & 1)) * BK));
+    else
+      asm volatile("ds_read_b128 %0, %1 offset:%2" : "=&v"(fq_[kc][r - 4]) : "v"(qa_[kc] + off), "i"(2 * (r - 4) * 16 * BK));
+  };
+  constexpr int READS = QB + 4, MFMAS = QB * 4;
+  // multiplies set kc, reads the other set from byte offset `off` and, where asked, requests a tile into buffer `buf`
+  auto chunk = [&](auto kc_c, unsigned off, auto fill_c, int buf) __attribute__((always_inline)) {
+    constexpr int kc = decltype(kc_c)::value;
+    constexpr bool fill = decltype(fill_c)::value;
+    auto& fq_ = fq; auto& fp_ = fp; auto& acc_ = acc;
+    static_for_h<MFMAS>([&](auto i_c) {
+      constexpr int i = decltype(i_c)::value, jq = i / 4, ip = i % 4;
+      if constexpr (F16) asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+v"(acc_[jq][ip]) : "v"(fp_[kc][ip]), "v"(fq_[kc][jq]));
+      else asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+v"(acc_[jq][ip]) : "v"(fp_[kc][ip]), "v"(fq_[kc][jq]));
+      static_for_h<(READS + MFMAS - 1) / MFMAS>([&](auto j_c) {
+        constexpr int r = decltype(j_c)::value * MFMAS + i;
+        if constexpr (r < READS) read(std::integral_constant<int, r>{}, std::integral_constant<int, kc ^ 1>{}, off);
+      });
+      if constexpr (fill)
+          static_for_h<K_::INSTR>([&](auto l_c) {
+            constexpr int l = decltype(l_c)::value;
+            if constexpr (l * MFMAS / K_::INSTR == i) load(l_c, buf);
+          });
+    });
+  };
+  using C0 = std::integral_constant<int, 0>;
+  using C1 = std::integral_constant<int, 1>;
 #pragma unroll
-  for (int s = 0; s < STAGES - 1; ++s)
-    if (s < nk) issue(s);
+  for (int s = 0; s < STAGES; ++s)
+    if (s < nk) static_for_h<K_::INSTR>([&](auto l_c) { load(l_c, s); });
+  if (nk >= STAGES) __builtin_amdgcn_s_waitcnt(vmcnt_imm((STAGES - 1) * K_::INSTR));
+  else __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+  ring_barrier();
+  static_for_h<READS>([&](auto r_c) { read(r_c, C0{}, 0u); });
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   int cur = 0;
-  for (int t = 0; t < nk; ++t) {
-    if (t + STAGES - 1 <= nk) __builtin_amdgcn_s_waitcnt(vmcnt_imm((STAGES - 2) * K_::INSTR));
-    else __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+  auto step = [&](auto fill_c) __attribute__((always_inline)) {
+    constexpr bool fill = decltype(fill_c)::value;  // the tile STAGES steps ahead exists
+    const int next = cur + 1 == STAGES ? 0 : cur + 1;
+    chunk(C0{}, 2u * (unsigned)(cur * K_::BUF), std::false_type{}, 0);
+    // the second set is in registers, so this wavefront is done with the buffer, and the next tile has landed
+    if constexpr (fill) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "i"((STAGES - 2) * K_::INSTR) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     ring_barrier();
-    if (t + STAGES - 1 < nk) issue(cur == 0 ? STAGES - 1 : cur - 1);
-    const unsigned off = 2u * (unsigned)(cur * K_::BUF);
+    // after the last tile: a harmless read of ring memory
+    chunk(C1{}, 2u * (unsigned)(next * K_::BUF), fill_c, cur);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    cur = next;
+  };
+  int t = 0;
+  for (; t + STAGES < nk; ++t) step(std::true_type{});
+  for (; t < nk; ++t) step(std::false_type{});
+  // what the last step read is used by nothing: kept until it has arrived, lest its registers are given away before
 #pragma unroll
-    for (int kc = 0; kc < 2; ++kc) {
-      frag fp[4];
+  for (int ip = 0; ip < 4; ++ip) asm volatile("" : : "v"(fp[0][ip]));
 #pragma unroll
-      for (int ip = 0; ip < 4; ++ip)
-        fp[ip] = *reinterpret_cast<lds_frag_t*>((__attribute__((address_space(3))) const char*)(size_t)(
-            pa[kc] + off + 2u * (unsigned)((32 * (ip >> 1) + 4 * (ip & 1)) * BK)));
+  for (int jq = 0; jq < QB; ++jq) asm volatile("" : : "v"(fq[0][jq]));
+  // the compiler does not know that MFMAs have just written the accumulators: wait, then hand them over
+  asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
 #pragma unroll
-      for (int jq = 0; jq < QB; ++jq) {
-        const frag fq = *reinterpret_cast<lds_frag_t*>((__attribute__((address_space(3))) const char*)(size_t)(
-            qa[kc] + off + 2u * (unsigned)(jq * 16 * BK)));
+  for (int jq = 0; jq < QB; ++jq)
 #pragma unroll
-        for (int ip = 0; ip < 4; ++ip) {
-          if constexpr (F16) acc[jq][ip] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fp[ip], fq, acc[jq][ip], 0, 0, 0);
-          else acc[jq][ip] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fp[ip], fq, acc[jq][ip], 0, 0, 0);
-        }
-      }
-    }
-    __builtin_amdgcn_sched_barrier(0);  // this step's reads have returned (its MFMAs are issued) before the next barrier
-    cur = cur + 1 == STAGES ? 0 : cur + 1;
-  }
+    for (int ip = 0; ip < 4; ++ip) asm volatile("" : "+v"(acc[jq][ip]));
   __syncthreads();  // every wavefront is done with the operand tiles: the epilogue may use the LDS
   unsigned char* stage = reinterpret_cast<unsigned char*>(smem_t) + (size_t)wave * K_::STAGE_REGION;
   auto get = [&](int jq, int h, int i) __attribute__((always_inline)) { return acc[jq][2 * h + (i >> 2)][i & 3]; };
@@ -213,12 +275,11 @@ __global__ __launch_bounds__(x32::W4_NW * 64) void tile256_kernel(Tile16 p, type
   extern __shared__ __attribute__((aligned(16))) u16 smem_t[];
   const unsigned lds_base = __builtin_amdgcn_readfirstlane((unsigned)(size_t)((__attribute__((address_space(3))) const void*)smem_t));
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  int tm, tn;
-  tile16_of_workgroup(p, blockIdx.x, gridDim.x, tm, tn);
+  int entry, split, tm, tn;
+  tile16_of_workgroup(p, entry, split, tm, tn);
   const int m0 = tm * x32::BM, n0 = tn * x32::BN;
-  const int entry = blockIdx.z / p.splits, split = blockIdx.z - entry * p.splits;
-  const int steps = p.K / x32::BK;
-  const int k0 = (int)((long long)steps * split / p.splits), nk = (int)((long long)steps * (split + 1) / p.splits) - k0;
+  int k0, nk;
+  tile16_steps(p, split, k0, nk);
   f32x4 acc[2][x32::QB][4];
   const x32::W4Operands op{p.A + (size_t)entry * p.batchA + (size_t)m0 * p.lda + (size_t)k0 * x32::BK,
                            p.B + (size_t)entry * p.batchB + (size_t)n0 * p.ldb + (size_t)k0 * x32::BK,
@@ -243,28 +304,48 @@ __global__ __launch_bounds__(x32::W4_NW * 64) void tile256_kernel(Tile16 p, type
   half(std::integral_constant<int, 1>{});
 }
 
-// p.tile: 128 or 256.
+template <bool F16, int BM, int WM, int WN, int STAGES, class Epi>
+hipError_t launch_ring(const Tile16& p, const typename Epi::Args& e, dim3 grid, hipStream_t s) {
+  using K_ = TileKernel<BM, BM, WM, WN, STAGES>;
+  auto kern = tile16_kernel<F16, BM, BM, WM, WN, STAGES, Epi>;
+  static LdsOptIn opt_in;
+  if (hipError_t err = opt_in.ensure(reinterpret_cast<const void*>(kern), K_::LDS); err != hipSuccess) return err;
+  launch_kernel(kern, grid, dim3(WM * WN * 64), K_::LDS, s, p, e);
+  return hipGetLastError();
+}
+
+// p.tile: 64, 128 or 256.
 template <bool F16, class Epi>
 hipError_t launch_tile16(Tile16 p, const typename Epi::Args& e, int batch, hipStream_t s) {
   p.tiles_m = (p.M + p.tile - 1) / p.tile;
   p.tiles_n = (p.N + p.tile - 1) / p.tile;
-  const long long total = p.symmetric ? (long long)p.tiles_m * (p.tiles_m + 1) / 2 : (long long)p.tiles_m * p.tiles_n;
-  if (total <= 0 || batch <= 0) return hipSuccess;
-  if (total > 0x3fffffff || (long long)batch * p.splits > 65535) return hipErrorInvalidValue;
-  const dim3 grid((unsigned)total, 1, batch * p.splits);
+  const long long tiles = p.symmetric ? (long long)p.tiles_m * (p.tiles_m + 1) / 2 : (long long)p.tiles_m * p.tiles_n;
+  const long long total = tiles * batch * p.splits;
+  if (total <= 0) return hipSuccess;
+  if (tiles > (1 << 27) || total > (1 << 27)) return hipErrorInvalidValue;
+  p.tiles = (int)tiles;
+  const dim3 grid((unsigned)total);
+  static int cfg128 = getenv("T128") ? atoi(getenv("T128")) : 0, cfg64 = getenv("T64") ? atoi(getenv("T64")) : 0;
   if (p.tile == 256) {
     auto kern = tile256_kernel<F16, Epi>;
     static LdsOptIn opt_in;
     if (hipError_t err = opt_in.ensure(reinterpret_cast<const void*>(kern), x32::LDS_BYTES); err != hipSuccess) return err;
     launch_kernel(kern, grid, dim3(x32::W4_NW * 64), x32::LDS_BYTES, s, p, e);
-  } else {
-    using K_ = TileKernel<128, 128, 2, 2, 2>;
-    auto kern = tile16_kernel<F16, 128, 128, 2, 2, 2, Epi>;
-    static LdsOptIn opt_in;
-    if (hipError_t err = opt_in.ensure(reinterpret_cast<const void*>(kern), K_::LDS); err != hipSuccess) return err;
-    launch_kernel(kern, grid, dim3(256), K_::LDS, s, p, e);
+    return hipGetLastError();
   }
-  return hipGetLastError();
+  if (p.tile == 128) {
+    if (cfg128 == 5) return launch_ring<F16, 128, 1, 2, 2, Epi>(p, e, grid, s);
+    if (cfg128 == 1) return launch_ring<F16, 128, 2, 2, 4, Epi>(p, e, grid, s);
+    if (cfg128 == 2) return launch_ring<F16, 128, 4, 2, 4, Epi>(p, e, grid, s);
+    if (cfg128 == 3) return launch_ring<F16, 128, 4, 2, 2, Epi>(p, e, grid, s);
+    if (cfg128 == 4) return launch_ring<F16, 128, 4, 2, 3, Epi>(p, e, grid, s);
+    return launch_ring<F16, 128, 2, 2, 2, Epi>(p, e, grid, s);
+  }
+  if (cfg64 == 2) return launch_ring<F16, 64, 2, 1, 4, Epi>(p, e, grid, s);
+  if (cfg64 == 3) return launch_ring<F16, 64, 2, 1, 8, Epi>(p, e, grid, s);
+  if (cfg64 == 4) return launch_ring<F16, 64, 1, 1, 4, Epi>(p, e, grid, s);
+  if (cfg64 == 1) return launch_ring<F16, 64, 4, 1, 4, Epi>(p, e, grid, s);
+  return launch_ring<F16, 64, 4, 1, 8, Epi>(p, e, grid, s);
 }
 
 }  // namespace mi

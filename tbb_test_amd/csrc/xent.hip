@@ -12,6 +12,7 @@
 // term) in both orders that the next two products read, g for dX += g W and g^T for dW = g^T X.
 // fp32 models: the same pieces through the framework's fp32 GEMMs, with the softmax between them.
 #include <hip/hip_runtime.h>
+#include <cstdlib>
 
 #include <algorithm>
 
