@@ -9,13 +9,12 @@
 // bits less, which this iteration turns into errors of 1e-2 (flat spectra) to 3e-1 (a few strong
 // directions over a floor) of |O|; everything here is bounded, so fp16's range is enough: |X|_F = 1 at
 // the start and no singular value ever passes 1.21, hence |A_ij| < 1.5 and |b A + c A^2| < 2.9.
-// X is kept in fp32 beside its fp16 copy, because the a X term carries every direction from one
-// iteration to the next and grows small ones 3.4 times each: with the fp16 copy in that term its white
-// rounding noise grows along (4e-2 for a floor of 1e-2).  The diagonal of b A + c A^2, near b + c once
+// X is kept to 22 bits, because the a X term carries every direction from one iteration to the next and
+// grows small ones 3.4 times each: with the fp16 operand in that term its white rounding noise grows along
+// (4e-2 for a floor of 1e-2).  The diagonal of b A + c A^2, near b + c once
 // X is near its limit, stays in fp32 too and joins the a X term; its rounding would be most of what is
 // left.  Together: 2e-4 .. 8e-4 of |O|.
 #include <hip/hip_runtime.h>
-#include <cstdlib>
 
 #include <algorithm>
 
@@ -30,6 +29,7 @@ constexpr float NS_A = 3.4445f, NS_B = -4.7750f, NS_C = 2.0315f;
 constexpr float GRAM_SCALE = 4096.0f;  // A and b A + c A^2 are stored times this: off-diagonal entries start near 1 / (m sqrt n)
 
 inline size_t up(size_t x, size_t a) { return (x + a - 1) / a * a; }
+inline bool fours(const void* q, int bytes) { return reinterpret_cast<uintptr_t>(q) % bytes == 0; }  // null too
 
 // ---- U, its norm, X_0 -------------------------------------------------------------------------------
 
@@ -44,47 +44,82 @@ struct GatherArgs {
   long long strideM;
   float mu;
   int nesterov;
-  float* X;              // [batch][mp x np], in working orientation
+  float* U;              // [batch][mp x np], in working orientation
   int mp, np;
+  int vec;               // rows of G (and momentum) start at whole 16 bytes (bf16: 8)
   double* sumsq;         // [batch][workgroups of an entry]
 };
 
 // U in working orientation, zero padded, and the sum of its squares per workgroup.  64 x 64 tiles of the
-// gradient; FLIP turns them through LDS.
+// gradient, four consecutive elements per thread and row (16-byte loads where rows allow it: `vec`); FLIP
+// turns them through LDS.
 template <bool BF16, bool FLIP>
 __global__ __launch_bounds__(256) void ortho_gather_kernel(GatherArgs p) {
   __shared__ float tile[FLIP ? 64 : 1][65];
   __shared__ double red[256];
-  const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
+  const int tx = (threadIdx.x & 15) * 4, ty = threadIdx.x >> 4;
   const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64, col = c0 + tx;
-  float* X = p.X + (size_t)blockIdx.z * p.mp * p.np;
+  float* U = p.U + (size_t)blockIdx.z * p.mp * p.np;
   double acc = 0.0;
-  for (int i = ty; i < 64; i += 4) {
-    const int row = r0 + i;
-    float u = 0.0f;
-    if (row < p.rows && col < p.cols) {
+#pragma unroll
+  for (int pass = 0; pass < 4; ++pass) {
+    const int i = pass * 16 + ty, row = r0 + i;
+    f32x4 u = {0.0f, 0.0f, 0.0f, 0.0f};
+    const int n = row < p.rows ? min(p.cols - col, 4) : 0;  // elements that are there
+    if (n > 0) {
       const size_t at = (size_t)blockIdx.z * p.strideG + (size_t)row * p.ldg + col;
-      if constexpr (BF16) u = bf2f(static_cast<const u16*>(p.G)[at]);
-      else {
+      const bool whole = p.vec && n == 4;
+      if constexpr (BF16) {
+        const u16* g = static_cast<const u16*>(p.G) + at;
+        if (whole) {
+          const u32x2 two = *reinterpret_cast<const u32x2*>(g);
+          u = f32x4{__uint_as_float(two[0] << 16), __uint_as_float(two[0] & 0xffff0000u), __uint_as_float(two[1] << 16), __uint_as_float(two[1] & 0xffff0000u)};
+        } else {
+          for (int k = 0; k < n; ++k) u[k] = bf2f(g[k]);
+        }
+      } else {
         const float* g = static_cast<const float*>(p.G) + at;
-        u = g[0];
-        for (int r = 1; r < p.R; ++r) u += g[(size_t)r * p.replica_stride];
+        if (whole) {
+          u = *reinterpret_cast<const f32x4*>(g);
+          for (int r = 1; r < p.R; ++r) u += *reinterpret_cast<const f32x4*>(g + (size_t)r * p.replica_stride);
+        } else {
+          for (int k = 0; k < n; ++k) {
+            u[k] = g[k];
+            for (int r = 1; r < p.R; ++r) u[k] += g[(size_t)r * p.replica_stride + k];
+          }
+        }
       }
       if (p.momentum) {
         float* m = p.momentum + (size_t)blockIdx.z * p.strideM + (size_t)row * p.cols + col;
-        const float now = fmaf(p.mu, *m, u);
-        *m = now;
-        u = p.nesterov ? fmaf(p.mu, now, u) : now;
+        f32x4 now = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (whole) now = *reinterpret_cast<const f32x4*>(m);
+        else for (int k = 0; k < n; ++k) now[k] = m[k];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          now[k] = fmaf(p.mu, now[k], u[k]);
+          u[k] = p.nesterov ? fmaf(p.mu, now[k], u[k]) : now[k];
+        }
+        if (whole) *reinterpret_cast<f32x4*>(m) = now;
+        else for (int k = 0; k < n; ++k) m[k] = now[k];
       }
     }
-    acc += (double)u * (double)u;
-    if constexpr (FLIP) tile[i][tx] = u;
-    else X[(size_t)row * p.np + col] = u;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) acc += (double)u[k] * (double)u[k];
+    if constexpr (FLIP) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) tile[i][tx + k] = u[k];
+    } else {
+      *reinterpret_cast<f32x4*>(U + (size_t)row * p.np + col) = u;
+    }
   }
   red[threadIdx.x] = acc;
   __syncthreads();
   if constexpr (FLIP) {
-    for (int i = ty; i < 64; i += 4) X[(size_t)(c0 + i) * p.np + r0 + tx] = tile[tx][i];
+#pragma unroll
+    for (int pass = 0; pass < 4; ++pass) {
+      const int i = pass * 16 + ty;
+      *reinterpret_cast<f32x4*>(U + (size_t)(c0 + i) * p.np + r0 + tx) = f32x4{tile[tx][i], tile[tx + 1][i], tile[tx + 2][i], tile[tx + 3][i]};
+    }
   }
   for (int off = 128; off > 0; off >>= 1) {
     if ((int)threadIdx.x < off) red[threadIdx.x] += red[threadIdx.x + off];
@@ -96,9 +131,13 @@ __global__ __launch_bounds__(256) void ortho_gather_kernel(GatherArgs p) {
 // inv[entry] = 1 / |U|_F; 0 for U = 0, NaN where |U|_F is not finite.
 __global__ __launch_bounds__(256) void ortho_norm_kernel(const double* __restrict__ sumsq, int blocks, double* __restrict__ inv) {
   __shared__ double red[256];
-  double acc = 0.0;
-  for (int i = threadIdx.x; i < blocks; i += 256) acc += sumsq[(size_t)blockIdx.x * blocks + i];
-  red[threadIdx.x] = acc;
+  double part[8] = {};
+  int i = threadIdx.x;
+  for (; i + 7 * 256 < blocks; i += 8 * 256)
+#pragma unroll
+    for (int k = 0; k < 8; ++k) part[k] += sumsq[(size_t)blockIdx.x * blocks + i + 256 * k];
+  for (; i < blocks; i += 256) part[0] += sumsq[(size_t)blockIdx.x * blocks + i];
+  red[threadIdx.x] = ((part[0] + part[1]) + (part[2] + part[3])) + ((part[4] + part[5]) + (part[6] + part[7]));
   __syncthreads();
   for (int off = 128; off > 0; off >>= 1) {
     if ((int)threadIdx.x < off) red[threadIdx.x] += red[threadIdx.x + off];
@@ -110,29 +149,51 @@ __global__ __launch_bounds__(256) void ortho_norm_kernel(const double* __restric
   }
 }
 
-// X <- X / |U|_F, Xh = fp16(scale X), XhT its transpose.  64 x 64 tiles.
-__global__ __launch_bounds__(256) void ortho_scale_kernel(float* __restrict__ X, u16* __restrict__ Xh, u16* __restrict__ XhT, int mp,
-                                                          int np, const double* __restrict__ inv, float scale) {
+// X = scale * x is kept as two fp16 numbers, x rounded and 2^11 times what the rounding left: 22 bits, as much
+// traffic as fp32, and the first half is the operand of the products.
+constexpr float LOW_SCALE = 2048.0f;
+__device__ __forceinline__ float joined(float high, float low) { return fmaf(low, 1.0f / LOW_SCALE, high); }
+
+// X_0 = scale * U / |U|_F as two halves, and the first half transposed.  64 x 64 tiles.
+__global__ __launch_bounds__(256) void ortho_scale_kernel(const float* __restrict__ U, u16* __restrict__ Xh, u16* __restrict__ Xl,
+                                                          u16* __restrict__ XhT, int mp, int np, const double* __restrict__ inv,
+                                                          float scale) {
   __shared__ u16 tile[64][66];
   const size_t base = (size_t)blockIdx.z * mp * np;
-  const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6, r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;
-  const double f = inv[blockIdx.z];
-  for (int i = ty; i < 64; i += 4) {
+  const int tx = (threadIdx.x & 15) * 4, ty = threadIdx.x >> 4, r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;
+  const double f = inv[blockIdx.z] * (double)scale;
+#pragma unroll
+  for (int pass = 0; pass < 4; ++pass) {
+    const int i = pass * 16 + ty;
     const size_t at = base + (size_t)(r0 + i) * np + c0 + tx;
-    const float x = (float)((double)X[at] * f);
-    X[at] = x;
-    const u16 h = __builtin_bit_cast(u16, (_Float16)(scale * x));
-    Xh[at] = h;
-    tile[i][tx] = h;
+    const f32x4 u = *reinterpret_cast<const f32x4*>(U + at);
+    float x[4];
+    u32x2 high, low;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) x[k] = (float)((double)u[k] * f);
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      high[k] = pack16<true>(x[2 * k], x[2 * k + 1]);
+      low[k] = pack16<true>(LOW_SCALE * (x[2 * k] - f16_lo(high[k])), LOW_SCALE * (x[2 * k + 1] - f16_hi(high[k])));
+    }
+    *reinterpret_cast<u32x2*>(Xh + at) = high;
+    *reinterpret_cast<u32x2*>(Xl + at) = low;
+    *reinterpret_cast<unsigned*>(&tile[i][tx]) = high[0];
+    *reinterpret_cast<unsigned*>(&tile[i][tx + 2]) = high[1];
   }
   __syncthreads();
-  for (int i = ty; i < 64; i += 4) XhT[base + (size_t)(c0 + i) * mp + r0 + tx] = tile[tx][i];
+#pragma unroll
+  for (int pass = 0; pass < 4; ++pass) {
+    const int i = pass * 16 + ty;
+    *reinterpret_cast<u32x2*>(XhT + base + (size_t)(c0 + i) * mp + r0 + tx) =
+        u32x2{tile[tx][i] | (unsigned)tile[tx + 1][i] << 16, tile[tx + 2][i] | (unsigned)tile[tx + 3][i] << 16};
+  }
 }
 
 // ---- the products -----------------------------------------------------------------------------------
 
 // A = X X^T (times GRAM_SCALE, fp16): a tile of the lower triangle and its mirror image.
-struct EpiGram {
+struct EpiGram : NoPre {
   struct Args {
     u16* A;
     int ld;
@@ -140,8 +201,8 @@ struct EpiGram {
     float scale;
   };
   template <int QB, class Get>
-  static __device__ __forceinline__ void run(const Args& e, const Tile16& p, Get get, int row0, int colw, int lane,
-                                             unsigned char* stage, int entry, int) {
+  static __device__ __forceinline__ void run(const Args& e, const Tile16& p, const Pre<QB>& pre, Get get, int row0, int colw, int lane,
+                                             unsigned char* stage, int entry) {
     u16* A = e.A + (size_t)entry * e.batch;
     const int l16 = lane & 15, col = colw + 8 * (lane >> 4);
     u32x4 pk[QB][2];
@@ -166,17 +227,26 @@ struct EpiPoly {
     int ld;
     long long batch;
   };
-  template <int QB, class Get>
-  static __device__ __forceinline__ void run(const Args& e, const Tile16& p, Get get, int row0, int colw, int lane,
-                                             unsigned char* stage, int entry, int) {
-    const u16* A = e.A + (size_t)entry * e.batch;
-    u16* P = e.P + (size_t)entry * e.batch;
-    const int l16 = lane & 15, col = colw + 8 * (lane >> 4);
-    u32x4 pk[QB][2];
+  template <int QB>
+  struct Pre {
+    u32x4 a[QB][2];
+  };
+  template <int QB>
+  static __device__ __forceinline__ Pre<QB> before(const Args& e, const Tile16&, int row0, int colw, int lane, int entry) {
+    const u16* A = e.A + (size_t)entry * e.batch + (size_t)(row0 + (lane & 15)) * e.ld + colw + 8 * (lane >> 4);
+    Pre<QB> v;
 #pragma unroll
     for (int jq = 0; jq < QB; ++jq)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) pk[jq][h] = *reinterpret_cast<const u32x4*>(A + (size_t)(row0 + 16 * jq + l16) * e.ld + col + 32 * h);
+      for (int h = 0; h < 2; ++h) v.a[jq][h] = *reinterpret_cast<const u32x4*>(A + (size_t)(16 * jq) * e.ld + 32 * h);
+    return v;
+  }
+  template <int QB, class Get>
+  static __device__ __forceinline__ void run(const Args& e, const Tile16& p, const Pre<QB>& pre, Get get, int row0, int colw, int lane,
+                                             unsigned char* stage, int entry) {
+    u16* P = e.P + (size_t)entry * e.batch;
+    const int l16 = lane & 15, col = colw + 8 * (lane >> 4);
+    u32x4 pk[QB][2];
     const bool on_diagonal = row0 / p.tile == colw / p.tile;
 #pragma unroll
     for (int jq = 0; jq < QB; ++jq)
@@ -186,7 +256,7 @@ struct EpiPoly {
         float v[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const unsigned w = pk[jq][h][i >> 1];
+          const unsigned w = pre.a[jq][h][i >> 1];
           v[i] = fmaf(NS_C / GRAM_SCALE, get(jq, h, i), NS_B * ((i & 1) ? f16_hi(w) : f16_lo(w)));
         }
         if (on_diagonal) {
@@ -205,40 +275,62 @@ struct EpiPoly {
   }
 };
 
-// X <- (a + diag) X + P X; the fp16 copy and its transpose for the next iteration (null: last one).
+// X <- (a + diag) X + P X, in place, and the first half's transpose for the next iteration (null: last one).
 struct EpiStep {
   struct Args {
-    float* X;
     const float* diag;
-    u16 *Xh, *XhT;
+    u16 *Xh, *Xl, *XhT;
     int mp, np;
-    float unscale, scale;  // accumulator -> X, X -> fp16 copy
+    float unscale;  // of the products, to scale * x
   };
-  template <int QB, class Get>
-  static __device__ __forceinline__ void run(const Args& e, const Tile16& p, Get get, int row0, int colw, int lane,
-                                             unsigned char* stage, int entry, int) {
-    const size_t base = (size_t)entry * e.mp * e.np;
-    const int l16 = lane & 15, col = colw + 8 * (lane >> 4);
-    u32x4 pk[QB][2];
+  template <int QB>
+  struct Pre {
+    u32x4 high[QB][2], low[QB][2];
+    float keep[QB];
+  };
+  template <int QB>
+  static __device__ __forceinline__ Pre<QB> before(const Args& e, const Tile16&, int row0, int colw, int lane, int entry) {
+    const int row = row0 + (lane & 15);
+    const size_t at = (size_t)entry * e.mp * e.np + (size_t)row * e.np + colw + 8 * (lane >> 4);
+    Pre<QB> v;
 #pragma unroll
     for (int jq = 0; jq < QB; ++jq) {
-      const int row = row0 + 16 * jq + l16;
-      const float keep = NS_A + e.diag[(size_t)entry * e.mp + row];
+      v.keep[jq] = NS_A + e.diag[(size_t)entry * e.mp + row + 16 * jq];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        f32x4* x = reinterpret_cast<f32x4*>(e.X + base + (size_t)row * e.np + col + 32 * h);
-        f32x4 v[2] = {x[0], x[1]};
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i >> 2][i & 3] = fmaf(keep, v[i >> 2][i & 3], e.unscale * get(jq, h, i));
-        x[0] = v[0];
-        x[1] = v[1];
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          pk[jq][h][k] = pack16<true>(e.scale * v[k >> 1][2 * (k & 1)], e.scale * v[k >> 1][2 * (k & 1) + 1]);
-        if (e.Xh) *reinterpret_cast<u32x4*>(e.Xh + base + (size_t)row * e.np + col + 32 * h) = pk[jq][h];
+        v.high[jq][h] = *reinterpret_cast<const u32x4*>(e.Xh + at + (size_t)(16 * jq) * e.np + 32 * h);
+        v.low[jq][h] = *reinterpret_cast<const u32x4*>(e.Xl + at + (size_t)(16 * jq) * e.np + 32 * h);
       }
     }
-    if (e.XhT) store_transposed<QB>(e.XhT + base + (size_t)colw * e.mp + row0, e.mp, pk, lane, stage);
+    return v;
+  }
+  template <int QB, class Get>
+  static __device__ __forceinline__ void run(const Args& e, const Tile16& p, const Pre<QB>& pre, Get get, int row0, int colw, int lane,
+                                             unsigned char* stage, int entry) {
+    const size_t base = (size_t)entry * e.mp * e.np;
+    const int l16 = lane & 15, col = colw + 8 * (lane >> 4);
+    u32x4 high[QB][2];
+    // (all of the tile's X is requested before anything is stored: a load behind a store waits for that store)
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int jq = 0; jq < QB; ++jq)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const size_t at = base + (size_t)(row0 + 16 * jq + l16) * e.np + col + 32 * h;
+        u32x4 low;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const unsigned hi = pre.high[jq][h][k], lo = pre.low[jq][h][k];
+          const float x0 = fmaf(pre.keep[jq], joined(f16_lo(hi), f16_lo(lo)), e.unscale * get(jq, h, 2 * k));
+          const float x1 = fmaf(pre.keep[jq], joined(f16_hi(hi), f16_hi(lo)), e.unscale * get(jq, h, 2 * k + 1));
+          const unsigned now = pack16<true>(x0, x1);
+          high[jq][h][k] = now;
+          low[k] = pack16<true>(LOW_SCALE * (x0 - f16_lo(now)), LOW_SCALE * (x1 - f16_hi(now)));
+        }
+        *reinterpret_cast<u32x4*>(e.Xh + at) = high[jq][h];
+        *reinterpret_cast<u32x4*>(e.Xl + at) = low;
+      }
+    if (e.XhT) store_transposed<QB>(e.XhT + base + (size_t)colw * e.mp + row0, e.mp, high, lane, stage);
   }
 };
 
@@ -246,7 +338,8 @@ struct EpiStep {
 
 struct FinishArgs {
   int rows, cols;
-  const float* X;  // [batch][mp x np]
+  const u16 *Xh, *Xl;  // [batch][mp x np]
+  float unscale;       // of X
   int mp, np;
   u16* O;          // bf16 result, or null
   int ldo;
@@ -255,49 +348,87 @@ struct FinishArgs {
   u16 *W16, *Wt16;
   long long strideW;
   float keep, step;  // W <- keep W - step O
+  int vec, vec_t;    // rows of O, W and W16 (of Wt16) start at whole 16 or 8 bytes
 };
 
 template <bool FLIP>
 __global__ __launch_bounds__(256) void ortho_finish_kernel(FinishArgs p) {
   __shared__ float turned[FLIP ? 64 : 1][65];
   __shared__ u16 tile[64][66];
-  const float* X = p.X + (size_t)blockIdx.z * p.mp * p.np;
-  const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6, r0 = blockIdx.y * 64, c0 = blockIdx.x * 64, col = c0 + tx;
-  if constexpr (FLIP) {  // X is padded to whole 64 x 64 tiles
-    for (int i = ty; i < 64; i += 4) turned[i][tx] = X[(size_t)(c0 + i) * p.np + r0 + tx];
+  const size_t base = (size_t)blockIdx.z * p.mp * p.np;
+  const int tx = (threadIdx.x & 15) * 4, ty = threadIdx.x >> 4, r0 = blockIdx.y * 64, c0 = blockIdx.x * 64, col = c0 + tx;
+  auto x_at = [&](size_t at) {  // four elements (X is padded to whole 64 x 64 tiles)
+    const u32x2 high = *reinterpret_cast<const u32x2*>(p.Xh + base + at), low = *reinterpret_cast<const u32x2*>(p.Xl + base + at);
+    return f32x4{p.unscale * joined(f16_lo(high[0]), f16_lo(low[0])), p.unscale * joined(f16_hi(high[0]), f16_hi(low[0])),
+                 p.unscale * joined(f16_lo(high[1]), f16_lo(low[1])), p.unscale * joined(f16_hi(high[1]), f16_hi(low[1]))};
+  };
+  if constexpr (FLIP) {
+#pragma unroll
+    for (int pass = 0; pass < 4; ++pass) {
+      const f32x4 x = x_at((size_t)(c0 + pass * 16 + ty) * p.np + r0 + tx);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) turned[pass * 16 + ty][tx + k] = x[k];
+    }
     __syncthreads();
   }
-  for (int i = ty; i < 64; i += 4) {
-    const int row = r0 + i;
-    if (row >= p.rows || col >= p.cols) continue;
-    const float o = FLIP ? turned[tx][i] : X[(size_t)row * p.np + col];
-    if (p.O) p.O[(size_t)blockIdx.z * p.strideO + (size_t)row * p.ldo + col] = f2bf(o);
+#pragma unroll
+  for (int pass = 0; pass < 4; ++pass) {
+    const int i = pass * 16 + ty, row = r0 + i;
+    const int n = row < p.rows ? min(p.cols - col, 4) : 0;
+    if (n <= 0) continue;
+    const f32x4 o = FLIP ? f32x4{turned[tx][i], turned[tx + 1][i], turned[tx + 2][i], turned[tx + 3][i]} : x_at((size_t)row * p.np + col);
+    const bool whole = p.vec && n == 4;
+    if (p.O) {
+      u16* out = p.O + (size_t)blockIdx.z * p.strideO + (size_t)row * p.ldo + col;
+      if (whole) *reinterpret_cast<u32x2*>(out) = u32x2{pack16<false>(o[0], o[1]), pack16<false>(o[2], o[3])};
+      else for (int k = 0; k < n; ++k) out[k] = f2bf(o[k]);
+    }
     if (p.W) {
       const size_t at = (size_t)blockIdx.z * p.strideW + (size_t)row * p.cols + col;
-      const float w = fmaf(-p.step, o, p.keep * p.W[at]);
-      p.W[at] = w;
-      const u16 h = f2bf(w);
-      if (p.W16) p.W16[at] = h;
-      tile[i][tx] = h;
+      f32x4 w = {0.0f, 0.0f, 0.0f, 0.0f};
+      if (whole) w = *reinterpret_cast<const f32x4*>(p.W + at);
+      else for (int k = 0; k < n; ++k) w[k] = p.W[at + k];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) w[k] = fmaf(-p.step, o[k], p.keep * w[k]);
+      const u32x2 h = {pack16<false>(w[0], w[1]), pack16<false>(w[2], w[3])};
+      if (whole) {
+        *reinterpret_cast<f32x4*>(p.W + at) = w;
+        if (p.W16) *reinterpret_cast<u32x2*>(p.W16 + at) = h;
+      } else {
+        for (int k = 0; k < n; ++k) {
+          p.W[at + k] = w[k];
+          if (p.W16) p.W16[at + k] = f2bf(w[k]);
+        }
+      }
+      *reinterpret_cast<unsigned*>(&tile[i][tx]) = h[0];
+      *reinterpret_cast<unsigned*>(&tile[i][tx + 2]) = h[1];
     }
   }
   if (!p.Wt16) return;
   __syncthreads();
-  for (int i = ty; i < 64; i += 4)
-    if (c0 + i < p.cols && r0 + tx < p.rows)
-      p.Wt16[(size_t)blockIdx.z * p.strideW + (size_t)(c0 + i) * p.rows + r0 + tx] = tile[tx][i];
+#pragma unroll
+  for (int pass = 0; pass < 4; ++pass) {
+    const int i = pass * 16 + ty;
+    const int n = c0 + i < p.cols ? min(p.rows - r0 - tx, 4) : 0;
+    if (n <= 0) continue;
+    u16* out = p.Wt16 + (size_t)blockIdx.z * p.strideW + (size_t)(c0 + i) * p.rows + r0 + tx;
+    if (p.vec_t && n == 4)
+      *reinterpret_cast<u32x2*>(out) = u32x2{tile[tx][i] | (unsigned)tile[tx + 1][i] << 16, tile[tx + 2][i] | (unsigned)tile[tx + 3][i] << 16};
+    else
+      for (int k = 0; k < n; ++k) out[k] = tile[tx + k][i];
+  }
 }
 
 // ---- sizes ------------------------------------------------------------------------------------------
 
 struct Plan {
   int m, n, mp, np;
-  int tile;    // of the products; m and n are padded to multiples of it
   bool flip;
-  float scale;  // of the fp16 copies of X: a power of two near sqrt(n), so that typical entries start near 1 / sqrt(m)
-  float* X;
-  u16 *Xh, *XhT[2], *A, *P;
-  float* diag;
+  float scale;  // of X: a power of two near sqrt(n), so that typical entries start near 1 / sqrt(m)
+  Tile16Shape gram, poly, step;
+  float* U;
+  u16 *Xh, *Xl, *XhT[2], *A, *P;
+  float *diag, *part;
   double *sumsq, *inv;
   size_t bytes;
 };
@@ -306,12 +437,18 @@ Plan plan_ortho(char* base, int batch, int rows, int cols) {
   q.flip = rows > cols;
   q.m = std::min(rows, cols);
   q.n = std::max(rows, cols);
-  // large matrices: 256 x 256 tiles once even the smallest products (the triangle of m x m) fill the CUs
-  const size_t t = up(q.m, 256) / 256;
-  q.tile = batch * t * (t + 1) / 2 >= 200 ? 256 : 128;
-  { static int t = getenv("TT") ? atoi(getenv("TT")) : 0; if (t) q.tile = t; }
-  q.mp = (int)up(q.m, q.tile);
-  q.np = (int)up(q.n, q.tile);
+  // padded to whole tiles of the largest size that wastes little
+  auto pad = [](int v) {
+    for (int t : {256, 128})
+      if (up(v, t) - v <= (size_t)v / 32) return (int)up(v, t);
+    return (int)up(v, 64);
+  };
+  q.mp = pad(q.m);
+  q.np = pad(q.n);
+  auto largest = [](int v) { return v % 256 == 0 ? 256 : v % 128 == 0 ? 128 : 64; };
+  q.gram = tile16_shape(q.mp, q.mp, q.np, true, batch, 64, largest(q.mp), true);
+  q.poly = tile16_shape(q.mp, q.mp, q.mp, true, batch, 64, largest(q.mp), true);
+  q.step = tile16_shape(q.mp, q.np, q.mp, false, batch, 64, std::min(largest(q.mp), largest(q.np)), true);
   q.scale = 1.0f;
   while (q.scale * q.scale < (float)q.n && q.scale < 256.0f) q.scale *= 2.0f;
   size_t used = 0;
@@ -321,13 +458,15 @@ Plan plan_ortho(char* base, int batch, int rows, int cols) {
     return at;
   };
   const size_t x = (size_t)batch * q.mp * q.np, a = (size_t)batch * q.mp * q.mp;
-  q.X = (float*)take(x * 4);
+  q.U = (float*)take(x * 4);
   q.Xh = (u16*)take(x * 2);
+  q.Xl = (u16*)take(x * 2);
   q.XhT[0] = (u16*)take(x * 2);
   q.XhT[1] = (u16*)take(x * 2);
   q.A = (u16*)take(a * 2);
   q.P = (u16*)take(a * 2);
   q.diag = (float*)take((size_t)batch * q.mp * 4);
+  q.part = (float*)take(std::max({q.gram.part_floats, q.poly.part_floats, q.step.part_floats}) * 4);
   q.sumsq = (double*)take((size_t)batch * (q.mp / 64) * (q.np / 64) * 8);
   q.inv = (double*)take((size_t)batch * 8);
   q.bytes = used;
@@ -335,15 +474,14 @@ Plan plan_ortho(char* base, int batch, int rows, int cols) {
 }
 
 template <class Epi>
-hipError_t tiles(int tile, const u16* A, const u16* B, int M, int N, int K, long long batchA, long long batchB, int batch, bool symmetric,
+hipError_t tiles(const Plan& q, const Tile16Shape& shape, const u16* A, const u16* B, int M, int N, int K, int batch, bool symmetric,
                  const typename Epi::Args& e, hipStream_t s) {
   Tile16 p{};
   p.A = A; p.B = B; p.lda = K; p.ldb = K; p.M = M; p.N = N; p.K = K;
-  p.batchA = batchA; p.batchB = batchB;
-  p.splits = 1;
+  p.batchA = (long long)M * K; p.batchB = (long long)N * K;
+  p.batch = batch;
   p.symmetric = symmetric;
-  p.tile = tile;
-  return launch_tile16<true, Epi>(p, e, batch, s);
+  return launch_tile16<true, Epi>(p, shape, q.part, e, s);
 }
 
 #define TRY(call)                          \
@@ -352,9 +490,9 @@ hipError_t tiles(int tile, const u16* A, const u16* B, int M, int N, int K, long
     if (e_ != hipSuccess) return e_;       \
   } while (0)
 
-// U (gathered by `g`) -> X of the last iteration, in q.X.
+// U (gathered by `g`) -> scale * X of the last iteration, in q.Xh and q.Xl.
 hipError_t newton_schulz(const Plan& q, GatherArgs g, bool bf16, int batch, int steps, hipStream_t s) {
-  g.X = q.X;
+  g.U = q.U;
   g.mp = q.mp;
   g.np = q.np;
   g.sumsq = q.sumsq;
@@ -370,24 +508,25 @@ hipError_t newton_schulz(const Plan& q, GatherArgs g, bool bf16, int batch, int 
   TRY(hipGetLastError());
   launch_kernel(ortho_norm_kernel, dim3(batch), dim3(256), 0, s, (const double*)q.sumsq, (q.mp / 64) * (q.np / 64), q.inv);
   TRY(hipGetLastError());
-  launch_kernel(ortho_scale_kernel, tiles64, dim3(256), 0, s, q.X, q.Xh, q.XhT[0], q.mp, q.np, (const double*)q.inv, q.scale);
+  launch_kernel(ortho_scale_kernel, tiles64, dim3(256), 0, s, (const float*)q.U, q.Xh, q.Xl, q.XhT[0], q.mp, q.np,
+                (const double*)q.inv, q.scale);
   TRY(hipGetLastError());
-  const long long x = (long long)q.mp * q.np, a = (long long)q.mp * q.mp;
+  const long long a = (long long)q.mp * q.mp;
   for (int k = 0; k < steps; ++k) {
-    const bool last = k + 1 == steps;
     const EpiGram::Args gram{q.A, q.mp, a, GRAM_SCALE / (q.scale * q.scale)};
-    TRY(tiles<EpiGram>(q.tile, q.Xh, q.Xh, q.mp, q.mp, q.np, x, x, batch, true, gram, s));
+    TRY(tiles<EpiGram>(q, q.gram, q.Xh, q.Xh, q.mp, q.mp, q.np, batch, true, gram, s));
     const EpiPoly::Args poly{q.A, q.P, q.diag, q.mp, a};
-    TRY(tiles<EpiPoly>(q.tile, q.A, q.A, q.mp, q.mp, q.mp, a, a, batch, true, poly, s));
-    const EpiStep::Args step{q.X, q.diag, last ? nullptr : q.Xh, last ? nullptr : q.XhT[(k + 1) & 1], q.mp, q.np,
-                             1.0f / (GRAM_SCALE * q.scale), q.scale};
-    TRY(tiles<EpiStep>(q.tile, q.P, q.XhT[k & 1], q.mp, q.np, q.mp, a, x, batch, false, step, s));
+    TRY(tiles<EpiPoly>(q, q.poly, q.A, q.A, q.mp, q.mp, q.mp, batch, true, poly, s));
+    const EpiStep::Args step{q.diag, q.Xh, q.Xl, k + 1 == steps ? nullptr : q.XhT[(k + 1) & 1], q.mp, q.np, 1.0f / GRAM_SCALE};
+    TRY(tiles<EpiStep>(q, q.step, q.P, q.XhT[k & 1], q.mp, q.np, q.mp, batch, false, step, s));
   }
   return hipSuccess;
 }
 
 hipError_t finish(const Plan& q, FinishArgs f, int batch, hipStream_t s) {
-  f.X = q.X;
+  f.Xh = q.Xh;
+  f.Xl = q.Xl;
+  f.unscale = 1.0f / q.scale;
   f.mp = q.mp;
   f.np = q.np;
   const dim3 grid((f.cols + 63) / 64, (f.rows + 63) / 64, batch);
@@ -405,9 +544,11 @@ hipError_t orthogonalize(bool bf16, int batch, int rows, int cols, const void* G
   const Plan q = plan_ortho(static_cast<char*>(ws), batch, rows, cols);
   GatherArgs g{};
   g.rows = rows; g.cols = cols; g.G = G; g.ldg = ldg; g.strideG = strideG; g.R = 1;
+  g.vec = fours(G, bf16 ? 8 : 16) && ldg % 4 == 0 && strideG % 4 == 0;
   TRY(newton_schulz(q, g, bf16, batch, steps, s));
   FinishArgs f{};
   f.rows = rows; f.cols = cols; f.O = O; f.ldo = ldo; f.strideO = strideO;
+  f.vec = fours(O, 8) && ldo % 4 == 0 && strideO % 4 == 0;
   return finish(q, f, batch, s);
 }
 
@@ -419,11 +560,15 @@ hipError_t ortho_update(int batch, int rows, int cols, float* W, u16* W16, u16* 
   g.rows = rows; g.cols = cols; g.G = G; g.ldg = cols; g.strideG = (long long)layer_stride;
   g.replica_stride = replica_stride; g.R = R;
   g.momentum = momentum; g.strideM = (long long)layer_stride; g.mu = mu; g.nesterov = nesterov;
+  const bool strides = (batch == 1 || layer_stride % 4 == 0) && (R == 1 || replica_stride % 4 == 0);
+  g.vec = fours(G, 16) && fours(momentum, 16) && cols % 4 == 0 && strides;
   TRY(newton_schulz(q, g, false, batch, steps, s));
   FinishArgs f{};
   f.rows = rows; f.cols = cols; f.W = W; f.W16 = W16; f.Wt16 = Wt16; f.strideW = (long long)layer_stride;
   f.keep = 1.0f - lr * decay;
   f.step = lr * scale;
+  f.vec = fours(W, 16) && fours(W16, 8) && cols % 4 == 0 && strides;
+  f.vec_t = fours(Wt16, 8) && rows % 4 == 0 && strides;
   return finish(q, f, batch, s);
 }
 

@@ -30,10 +30,14 @@ struct Tile16 {
   const u16* B;
   long long batchA, batchB;  // elements between the operands of consecutive batch entries
   int lda, ldb, M, N, K;
-  int tiles_m, tiles_n, tiles;  // tiles: of one entry and split
-  int tile;       // rows and columns of a tile
-  int splits;     // the K steps are dealt to this many workgroups per tile
-  int symmetric;  // only tiles with tile_m >= tile_n are launched (square results, BM == BN)
+  int batch;
+  int symmetric;  // only tiles with tile_m >= tile_n are launched (square results)
+  int tile;       // rows and columns of a tile: 64, 128 or 256
+  // The tiles of all entries, entry by entry, are numbered through.  The first `full` are one workgroup each; the K
+  // steps of each of the others are dealt to `splits` workgroups, whose sums go to `part` and through a second launch.
+  int full, joined, splits;  // joined: how many are split
+  float* part;
+  int tiles_m, tiles_n, tiles;  // set by the launch; tiles: of one entry
 };
 
 // Two values rounded to nearest even, packed (low half first).
@@ -46,17 +50,12 @@ __device__ __forceinline__ unsigned pack16(float lo, float hi) {
 __device__ __forceinline__ float f16_lo(unsigned v) { return (float)__builtin_bit_cast(f16x2, v)[0]; }
 __device__ __forceinline__ float f16_hi(unsigned v) { return (float)__builtin_bit_cast(f16x2, v)[1]; }
 
-// Workgroup -> batch entry, K split and tile.  Workgroups go to the 8 XCDs round-robin; each XCD gets one
-// contiguous range of an order in which neighbours share operand panels: entry by entry, split by split, and within
-// one bands of eight tile rows, walked column by column (32 workgroups of an XCD in flight share eight
-// A panels and four B panels), or the rows of the lower triangle one after another.
-__device__ __forceinline__ void tile16_of_workgroup(const Tile16& p, int& entry, int& split, int& tm, int& tn) {
-  const int total = gridDim.x, xcd = blockIdx.x & 7, rest = total & 7;
-  int id = xcd * (total >> 3) + (xcd < rest ? xcd : rest) + (blockIdx.x >> 3);
-  const int z = __builtin_amdgcn_readfirstlane(id / p.tiles);  // (divisions go through vector registers)
-  id -= z * p.tiles;
-  entry = __builtin_amdgcn_readfirstlane(z / p.splits);
-  split = z - entry * p.splits;
+// Number `item` -> batch entry and tile, in an order in which neighbours share operand panels: within an entry
+// bands of eight tile rows, walked column by column (32 workgroups of an XCD in flight share eight A panels
+// and four B panels), or the rows of the lower triangle one after another.
+__device__ __forceinline__ void tile16_of_item(const Tile16& p, int item, int& entry, int& tm, int& tn) {
+  entry = __builtin_amdgcn_readfirstlane(item / p.tiles);  // (divisions go through vector registers)
+  const int id = item - entry * p.tiles;
   if (p.symmetric) {
     tm = (int)((__builtin_sqrtf(8.0f * (float)id + 1.0f) - 1.0f) * 0.5f);
     while (tm * (tm + 1) / 2 > id) --tm;  // the root is good to a unit only
@@ -71,11 +70,39 @@ __device__ __forceinline__ void tile16_of_workgroup(const Tile16& p, int& entry,
   tm = band * 8 + within - tn * height;
 }
 
-// The K steps of a split: first one and number of them.
-__device__ __forceinline__ void tile16_steps(const Tile16& p, int split, int& k0, int& nk) {
+// What a workgroup does: its item and the K steps of it.  split < 0: all of them.  Workgroups go to the 8 XCDs
+// round-robin; each XCD gets one contiguous range of the items.
+struct Tile16Job {
+  int item, split, entry, tm, tn, k0, nk;
+};
+__device__ __forceinline__ Tile16Job tile16_job(const Tile16& p) {
+  Tile16Job j;
   const int steps = p.K / 64;
-  k0 = __builtin_amdgcn_readfirstlane((int)((long long)steps * split / p.splits));
-  nk = __builtin_amdgcn_readfirstlane((int)((long long)steps * (split + 1) / p.splits)) - k0;
+  int id = blockIdx.x;
+  if (id < p.full) {
+    const int xcd = id & 7, rest = p.full & 7;
+    j.item = xcd * (p.full >> 3) + (xcd < rest ? xcd : rest) + (id >> 3);
+    j.split = -1;
+    j.k0 = 0;
+    j.nk = steps;
+  } else {
+    // split by split, so that the workgroups of an XCD share the operands' columns
+    id -= p.full;  // (a multiple of 8: id & 7 is still the XCD)
+    const int total = p.joined * p.splits, xcd = id & 7, rest = total & 7;
+    id = xcd * (total >> 3) + (xcd < rest ? xcd : rest) + (id >> 3);
+    j.split = __builtin_amdgcn_readfirstlane(id / p.joined);
+    j.item = p.full + id - j.split * p.joined;
+    j.k0 = __builtin_amdgcn_readfirstlane((int)((long long)steps * j.split / p.splits));
+    j.nk = __builtin_amdgcn_readfirstlane((int)((long long)steps * (j.split + 1) / p.splits)) - j.k0;
+  }
+  tile16_of_item(p, j.item, j.entry, j.tm, j.tn);
+  return j;
+}
+
+// Sums of a split: per block of 16 rows x 64 columns of the tile, row blocks first, the four n blocks of each lane.
+__device__ __forceinline__ f32x4* tile16_part(const Tile16& p, int item, int split, int row_in_tile, int col_in_tile, int lane) {
+  const int block = (row_in_tile >> 4) * (p.tile >> 6) + (col_in_tile >> 6), blocks = (p.tile >> 4) * (p.tile >> 6);
+  return reinterpret_cast<f32x4*>(p.part) + (((size_t)(item - p.full) * p.splits + split) * blocks + block) * 256 + lane;
 }
 
 // Transposed store of a wavefront's WTM x 64 packed results: dst[col][row], `ld` elements per column,
@@ -138,11 +165,8 @@ __global__ __launch_bounds__(WM* WN * 64) void tile16_kernel(Tile16 p, typename 
   const int l16 = lane & 15, q = lane >> 4;
   const int wm0 = (wave / WN) * (BM / WM), wn0 = (wave % WN) * 64;
 
-  int entry, split, tm, tn;
-  tile16_of_workgroup(p, entry, split, tm, tn);
-  const int m0 = tm * BM, n0 = tn * BN;
-  int k0, nk;
-  tile16_steps(p, split, k0, nk);
+  const Tile16Job job = tile16_job(p);
+  const int m0 = job.tm * BM, n0 = job.tn * BN, nk = job.nk;
 
   unsigned offa[K_::NIA], offb[K_::NIB];
   const int lrow = lane >> 3, pc = lane & 7;
@@ -162,11 +186,15 @@ __global__ __launch_bounds__(WM* WN * 64) void tile16_kernel(Tile16 p, typename 
     const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)v), hi = __builtin_amdgcn_readfirstlane((unsigned)(v >> 32));
     return ((unsigned long long)hi << 32) | lo;
   };
-  unsigned long long a = uniform64(p.A + (size_t)entry * p.batchA + (size_t)m0 * p.lda + (size_t)k0 * BK);
-  unsigned long long b = uniform64(p.B + (size_t)entry * p.batchB + (size_t)n0 * p.ldb + (size_t)k0 * BK);
+  unsigned long long a = uniform64(p.A + (size_t)job.entry * p.batchA + (size_t)m0 * p.lda + (size_t)job.k0 * BK);
+  unsigned long long b = uniform64(p.B + (size_t)job.entry * p.batchB + (size_t)n0 * p.ldb + (size_t)job.k0 * BK);
   auto to_lds = [](unsigned long long base, unsigned lane_off, unsigned lds) __attribute__((always_inline)) {
     asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(lds), "v"(lane_off), "s"(base) : "memory", "m0");
   };
+  // what the epilogue reads at the result's place, requested ahead of the K loop (older than the tile loads it counts)
+  typename Epi::template Pre<QB> pre;
+  if (job.split < 0) pre = Epi::template before<QB>(e, p, m0 + wm0, n0 + wn0, lane, job.entry);
+
   // load i of the tile that goes into buffer buf: A's, then B's; behind the last one on to the next K step
   auto load = [&](auto i_c, int buf) __attribute__((always_inline)) {
     constexpr int i = decltype(i_c)::value;
@@ -263,10 +291,17 @@ __global__ __launch_bounds__(WM* WN * 64) void tile16_kernel(Tile16 p, typename 
   for (int jq = 0; jq < QB; ++jq)
 #pragma unroll
     for (int ip = 0; ip < 4; ++ip) asm volatile("" : "+v"(acc[jq][ip]));
+  if (job.split >= 0) {
+#pragma unroll
+    for (int jq = 0; jq < QB; ++jq)
+#pragma unroll
+      for (int ip = 0; ip < 4; ++ip) tile16_part(p, job.item, job.split, wm0 + 16 * jq, wn0, lane)[64 * ip] = acc[jq][ip];
+    return;
+  }
   __syncthreads();  // every wavefront is done with the operand tiles: the epilogue may use the LDS
   unsigned char* stage = reinterpret_cast<unsigned char*>(smem_t) + (size_t)wave * K_::STAGE_REGION;
   auto get = [&](int jq, int h, int i) __attribute__((always_inline)) { return acc[jq][2 * h + (i >> 2)][i & 3]; };
-  Epi::template run<QB>(e, p, get, m0 + wm0, n0 + wn0, lane, stage, entry, split);
+  Epi::template run<QB>(e, p, pre, get, m0 + wm0, n0 + wn0, lane, stage, job.entry);
 }
 
 // The same on tiles of 256 x 256 with four wavefronts of 128 x 128 and the hand-ordered K loop.
@@ -275,77 +310,189 @@ __global__ __launch_bounds__(x32::W4_NW * 64) void tile256_kernel(Tile16 p, type
   extern __shared__ __attribute__((aligned(16))) u16 smem_t[];
   const unsigned lds_base = __builtin_amdgcn_readfirstlane((unsigned)(size_t)((__attribute__((address_space(3))) const void*)smem_t));
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  int entry, split, tm, tn;
-  tile16_of_workgroup(p, entry, split, tm, tn);
-  const int m0 = tm * x32::BM, n0 = tn * x32::BN;
-  int k0, nk;
-  tile16_steps(p, split, k0, nk);
+  const Tile16Job job = tile16_job(p);
+  const int m0 = job.tm * x32::BM, n0 = job.tn * x32::BN;
   f32x4 acc[2][x32::QB][4];
-  const x32::W4Operands op{p.A + (size_t)entry * p.batchA + (size_t)m0 * p.lda + (size_t)k0 * x32::BK,
-                           p.B + (size_t)entry * p.batchB + (size_t)n0 * p.ldb + (size_t)k0 * x32::BK,
+  const x32::W4Operands op{p.A + (size_t)job.entry * p.batchA + (size_t)m0 * p.lda + (size_t)job.k0 * x32::BK,
+                           p.B + (size_t)job.entry * p.batchB + (size_t)n0 * p.ldb + (size_t)job.k0 * x32::BK,
                            p.lda, p.ldb, p.M - m0, p.N - n0};
-  x32::w4_loop<false, F16, true>(op, nk, lds_base, wave, lane, acc);
-  __syncthreads();  // every wavefront is done with the operand tiles: the epilogue may use the LDS
-  unsigned char* stage = reinterpret_cast<unsigned char*>(smem_t) + (size_t)wave * x32::STAGE_REGION;
+  x32::w4_loop<false, F16, true>(op, job.nk, lds_base, wave, lane, acc);
   // made opaque, so that none of the epilogue's addresses is computed ahead of the K loop and kept through it
-  int lane_e = lane, row_e = m0 + wave / x32::W4_WN * x32::WTM, col_e = n0 + wave % x32::W4_WN * x32::W4_WTN;
+  int lane_e = lane, row_e = wave / x32::W4_WN * x32::WTM, col_e = wave % x32::W4_WN * x32::W4_WTN;
   asm volatile("" : "+v"(lane_e), "+s"(row_e), "+s"(col_e));
   // the accumulators are read out of the AGPRs where they are used (one register each, not 256 at once)
-  auto half = [&](auto h_c) __attribute__((always_inline)) {
-    constexpr int hc = decltype(h_c)::value;
-    auto get = [&](int jq, int h, int i) __attribute__((always_inline)) {
-      float v;
-      asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(v) : "a"(acc[hc][jq][2 * h + (i >> 2)][i & 3]));
-      return v;
-    };
-    Epi::template run<x32::QB>(e, p, get, row_e, col_e + 64 * hc, lane_e, stage, entry, split);
+  auto value = [&](auto h_c, int jq, int ip, int i) __attribute__((always_inline)) {
+    float v;
+    asm volatile("v_accvgpr_read_b32 %0, %1" : "=v"(v) : "a"(acc[decltype(h_c)::value][jq][ip][i]));
+    return v;
   };
-  half(std::integral_constant<int, 0>{});
-  half(std::integral_constant<int, 1>{});
+  using H0 = std::integral_constant<int, 0>;
+  using H1 = std::integral_constant<int, 1>;
+  if (job.split >= 0) {
+    auto half = [&](auto h_c) __attribute__((always_inline)) {
+#pragma unroll
+      for (int jq = 0; jq < x32::QB; ++jq)
+#pragma unroll
+        for (int ip = 0; ip < 4; ++ip)
+          tile16_part(p, job.item, job.split, row_e + 16 * jq, col_e + 64 * decltype(h_c)::value, lane_e)[64 * ip] =
+              f32x4{value(h_c, jq, ip, 0), value(h_c, jq, ip, 1), value(h_c, jq, ip, 2), value(h_c, jq, ip, 3)};
+    };
+    half(H0{});
+    half(H1{});
+    return;
+  }
+  __syncthreads();  // every wavefront is done with the operand tiles: the epilogue may use the LDS
+  unsigned char* stage = reinterpret_cast<unsigned char*>(smem_t) + (size_t)wave * x32::STAGE_REGION;
+  auto half = [&](auto h_c) __attribute__((always_inline)) {
+    auto get = [&](int jq, int h, int i) __attribute__((always_inline)) { return value(h_c, jq, 2 * h + (i >> 2), i & 3); };
+    const int row = m0 + row_e, col = n0 + col_e + 64 * decltype(h_c)::value;
+    const auto pre = Epi::template before<x32::QB>(e, p, row, col, lane_e, job.entry);
+    Epi::template run<x32::QB>(e, p, pre, get, row, col, lane_e, stage, job.entry);
+  };
+  half(H0{});
+  half(H1{});
+}
+
+// Second launch: the sums of the split tiles, in split order, and their epilogue, a block of 16 x 64 per wavefront.
+template <class Epi>
+__global__ __launch_bounds__(256) void tile16_join_kernel(Tile16 p, typename Epi::Args e) {
+  __shared__ __attribute__((aligned(16))) unsigned char stage[4][32 * (16 * 2 + 8)];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int blocks = (p.tile >> 4) * (p.tile >> 6), groups = blocks / 4;
+  const int n = __builtin_amdgcn_readfirstlane((int)blockIdx.x / groups), block = ((int)blockIdx.x - n * groups) * 4 + wave;
+  const int row = block / (p.tile >> 6) * 16, col = block % (p.tile >> 6) * 64;
+  int entry, tm, tn;
+  tile16_of_item(p, p.full + n, entry, tm, tn);
+  const f32x4* src = tile16_part(p, p.full + n, 0, row, col, lane);
+  f32x4 acc[4];
+#pragma unroll
+  for (int ip = 0; ip < 4; ++ip) acc[ip] = src[64 * ip];
+#pragma unroll 4
+  for (int k = 1; k < p.splits; ++k) {
+    src += (size_t)blocks * 256;
+#pragma unroll
+    for (int ip = 0; ip < 4; ++ip) acc[ip] += src[64 * ip];
+  }
+  auto get = [&](int, int h, int i) __attribute__((always_inline)) { return acc[2 * h + (i >> 2)][i & 3]; };
+  const auto pre = Epi::template before<1>(e, p, tm * p.tile + row, tn * p.tile + col, lane, entry);
+  Epi::template run<1>(e, p, pre, get, tm * p.tile + row, tn * p.tile + col, lane, stage[wave], entry);
+}
+
+// For epilogues that read nothing at the result's place.
+struct NoPre {
+  template <int QB>
+  struct Pre {};
+  template <int QB, class Args>
+  static __device__ __forceinline__ Pre<QB> before(const Args&, const Tile16&, int, int, int, int) {
+    return {};
+  }
+};
+
+// ---- host side --------------------------------------------------------------------------------------
+
+struct Tile16Shape {
+  int tile = 128, full = 0, splits = 1;
+  size_t part_floats = 0;
+};
+inline long long tile16_count(long long rows, long long cols, int tile, bool symmetric, int batch) {
+  const long long m = (rows + tile - 1) / tile, n = (cols + tile - 1) / tile;
+  return batch * (symmetric ? m * (m + 1) / 2 : m * n);
+}
+
+// Tile and split of a product, from an estimate in microseconds.  largest / smallest: the tiles allowed; may_split: the
+// epilogue can run on 16-row blocks in a second launch.  The estimate's constants are measured, on random data: a
+// K step of a 256 x 256 tile takes 1.5 us (one workgroup per CU), one of 128 x 128 0.32 us alone on a CU and
+// 0.96 us with a second workgroup beside it, one of 64 x 64 0.17 us alone, four together 0.8 us; a launch
+// starts and ends in 3-8 us; a join costs 4 us and the sums' way to memory and back at 4 TB/s.
+inline Tile16Shape tile16_shape(long long rows, long long cols, int K, bool symmetric, int batch, int smallest, int largest,
+                                bool may_split) {
+  const int steps = K / 64;
+  Tile16Shape best;
+  double best_us = 1e30;
+  for (int tile = smallest; tile <= largest; tile *= 2) {
+    const long long items = tile16_count(rows, cols, tile, symmetric, batch);
+    const double step = tile == 256 ? 1.5 : tile == 128 ? 0.32 : 0.17;
+    const int at_once = tile == 256 ? 1 : tile == 128 ? 2 : 4;  // workgroups of a CU
+    const double crowded = tile == 256 ? 1.5 : tile == 128 ? 0.48 : 0.20;  // a step's share of the CU when it is full
+    const double ends = tile == 256 ? 8.0 : tile == 128 ? 5.0 : 3.5;
+    auto rounds = [&](long long n, double k) {  // n workgroups of k steps
+      if (n <= 0) return 0.0;
+      if (n <= 256) return k * step + ends;
+      const long long whole = n / (256 * at_once), rest = n - whole * 256 * at_once;
+      const double last = rest == 0 ? 0.0 : rest <= 256 ? k * step + ends : k * crowded * (double)((rest + 255) / 256) + ends;
+      return (double)whole * (k * crowded * at_once + ends) + last;
+    };
+    const double plain = rounds(items, steps);
+    if (plain < best_us) {
+      best_us = plain;
+      best = Tile16Shape{tile, (int)items, 1, 0};
+    }
+    if (!may_split) continue;
+    for (const int round : {256, 512}) {  // whole rounds first, split what is left over
+      if (round == 512 && at_once == 1) continue;
+      const long long full = items / round * round, rest = items - full;
+      if (rest == 0) continue;
+      for (int splits = 2; splits <= 64; splits += splits < 8 ? 1 : splits < 16 ? 2 : 8) {
+        if (steps / splits < 2) break;
+        const double few = (double)((steps + splits - 1) / splits), bytes = 8.0 * (double)rest * splits * tile * tile;
+        const double us = rounds(full, steps) + rounds(rest * splits, few) + 4.0 + bytes / 4e6;
+        if (us < best_us) {
+          best_us = us;
+          best = Tile16Shape{tile, (int)full, splits, (size_t)rest * splits * tile * tile};
+        }
+      }
+    }
+  }
+  return best;
 }
 
 template <bool F16, int BM, int WM, int WN, int STAGES, class Epi>
-hipError_t launch_ring(const Tile16& p, const typename Epi::Args& e, dim3 grid, hipStream_t s) {
+hipError_t launch_ring(const Tile16& p, const typename Epi::Args& e, unsigned grid, hipStream_t s) {
   using K_ = TileKernel<BM, BM, WM, WN, STAGES>;
   auto kern = tile16_kernel<F16, BM, BM, WM, WN, STAGES, Epi>;
   static LdsOptIn opt_in;
   if (hipError_t err = opt_in.ensure(reinterpret_cast<const void*>(kern), K_::LDS); err != hipSuccess) return err;
-  launch_kernel(kern, grid, dim3(WM * WN * 64), K_::LDS, s, p, e);
+  launch_kernel(kern, dim3(grid), dim3(WM * WN * 64), K_::LDS, s, p, e);
   return hipGetLastError();
 }
 
-// p.tile: 64, 128 or 256.
+// p.M, N, K, operands, batch and symmetric set; `shape` from tile16_shape for the same sizes, `part` with room for
+// its part_floats.
 template <bool F16, class Epi>
-hipError_t launch_tile16(Tile16 p, const typename Epi::Args& e, int batch, hipStream_t s) {
+hipError_t launch_tile16(Tile16 p, const Tile16Shape& shape, float* part, const typename Epi::Args& e, hipStream_t s) {
+  p.tile = shape.tile;
+  p.splits = shape.splits < p.K / 64 ? shape.splits : p.K / 64;  // a K step at least for each (a shorter last piece)
+  p.part = part;
   p.tiles_m = (p.M + p.tile - 1) / p.tile;
   p.tiles_n = (p.N + p.tile - 1) / p.tile;
-  const long long tiles = p.symmetric ? (long long)p.tiles_m * (p.tiles_m + 1) / 2 : (long long)p.tiles_m * p.tiles_n;
-  const long long total = tiles * batch * p.splits;
-  if (total <= 0) return hipSuccess;
-  if (tiles > (1 << 27) || total > (1 << 27)) return hipErrorInvalidValue;
-  p.tiles = (int)tiles;
-  const dim3 grid((unsigned)total);
-  static int cfg128 = getenv("T128") ? atoi(getenv("T128")) : 0, cfg64 = getenv("T64") ? atoi(getenv("T64")) : 0;
+  const long long items = tile16_count(p.M, p.N, p.tile, p.symmetric, p.batch);
+  if (items <= 0) return hipSuccess;
+  p.tiles = (int)(items / p.batch);
+  // a smaller product than the one the shape was made for (the last piece of a vocabulary): no more split tiles than it has
+  p.full = p.splits <= 1 ? (int)items : (int)(items < shape.full ? items : shape.full);
+  const long long joined = items - p.full, total = p.full + joined * p.splits;
+  p.joined = (int)joined;
+  if (items > (1 << 27) || total > (1 << 27)) return hipErrorInvalidValue;
+  if ((size_t)joined * p.splits * p.tile * p.tile > shape.part_floats) return hipErrorInvalidValue;
+  const unsigned grid = (unsigned)total;
+  hipError_t err = hipSuccess;
   if (p.tile == 256) {
     auto kern = tile256_kernel<F16, Epi>;
     static LdsOptIn opt_in;
-    if (hipError_t err = opt_in.ensure(reinterpret_cast<const void*>(kern), x32::LDS_BYTES); err != hipSuccess) return err;
-    launch_kernel(kern, grid, dim3(x32::W4_NW * 64), x32::LDS_BYTES, s, p, e);
-    return hipGetLastError();
+    err = opt_in.ensure(reinterpret_cast<const void*>(kern), x32::LDS_BYTES);
+    if (err != hipSuccess) return err;
+    launch_kernel(kern, dim3(grid), dim3(x32::W4_NW * 64), x32::LDS_BYTES, s, p, e);
+    err = hipGetLastError();
+  } else if (p.tile == 128) {
+    // more than one workgroup per CU: two buffers (64 KB) let two share it; else four, requested three steps ahead
+    // (1000 x 4100, a triangle of 72 workgroups, 66 steps: 24 us instead of 37)
+    err = grid > 256 ? launch_ring<F16, 128, 2, 2, 2, Epi>(p, e, grid, s) : launch_ring<F16, 128, 2, 2, 4, Epi>(p, e, grid, s);
+  } else {
+    err = launch_ring<F16, 64, 4, 1, 4, Epi>(p, e, grid, s);
   }
-  if (p.tile == 128) {
-    if (cfg128 == 5) return launch_ring<F16, 128, 1, 2, 2, Epi>(p, e, grid, s);
-    if (cfg128 == 1) return launch_ring<F16, 128, 2, 2, 4, Epi>(p, e, grid, s);
-    if (cfg128 == 2) return launch_ring<F16, 128, 4, 2, 4, Epi>(p, e, grid, s);
-    if (cfg128 == 3) return launch_ring<F16, 128, 4, 2, 2, Epi>(p, e, grid, s);
-    if (cfg128 == 4) return launch_ring<F16, 128, 4, 2, 3, Epi>(p, e, grid, s);
-    return launch_ring<F16, 128, 2, 2, 2, Epi>(p, e, grid, s);
-  }
-  if (cfg64 == 2) return launch_ring<F16, 64, 2, 1, 4, Epi>(p, e, grid, s);
-  if (cfg64 == 3) return launch_ring<F16, 64, 2, 1, 8, Epi>(p, e, grid, s);
-  if (cfg64 == 4) return launch_ring<F16, 64, 1, 1, 4, Epi>(p, e, grid, s);
-  if (cfg64 == 1) return launch_ring<F16, 64, 4, 1, 4, Epi>(p, e, grid, s);
-  return launch_ring<F16, 64, 4, 1, 8, Epi>(p, e, grid, s);
+  if (err != hipSuccess || joined == 0) return err;
+  launch_kernel(tile16_join_kernel<Epi>, dim3((unsigned)(joined * (p.tile / 16) * (p.tile / 64) / 4)), dim3(256), 0, s, p, e);
+  return hipGetLastError();
 }
 
 }  // namespace mi

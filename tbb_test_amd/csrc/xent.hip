@@ -12,7 +12,6 @@
 // term) in both orders that the next two products read, g for dX += g W and g^T for dW = g^T X.
 // fp32 models: the same pieces through the framework's fp32 GEMMs, with the softmax between them.
 #include <hip/hip_runtime.h>
-#include <cstdlib>
 
 #include <algorithm>
 
@@ -53,7 +52,7 @@ __device__ __forceinline__ void finish_row(float m, float s, bool counts, float 
 
 // ---- bf16 tiles -------------------------------------------------------------------------------------
 
-struct EpiStats {
+struct EpiStats : NoPre {
   struct Args {
     const float* bias;    // of the first column, or null
     const int* target;
@@ -62,8 +61,8 @@ struct EpiStats {
     float2* part;         // [column block of 64][M], from this launch's first block on
   };
   template <int QB, class Get>
-  static __device__ __forceinline__ void run(const Args& e, const Tile16& p, Get get, int row0, int colw, int lane,
-                                             unsigned char*, int, int) {
+  static __device__ __forceinline__ void run(const Args& e, const Tile16& p, const Pre<QB>& pre, Get get, int row0, int colw, int lane,
+                                             unsigned char*, int) {
     const int l16 = lane & 15, q = lane >> 4, lane_col = colw + 8 * q;
     if (colw >= p.N) return;
     float bias[2][8];
@@ -122,7 +121,7 @@ struct EpiStats {
   }
 };
 
-struct EpiGrad {
+struct EpiGrad : NoPre {
   struct Args {
     const float* bias;
     const int* target;
@@ -136,8 +135,8 @@ struct EpiGrad {
     float* db_part;      // column sums per wavefront tile of 16 QB rows, [row0 / (16 QB)][ldg], or null
   };
   template <int QB, class Get>
-  static __device__ __forceinline__ void run(const Args& e, const Tile16& p, Get get, int row0, int colw, int lane,
-                                             unsigned char* stage, int, int) {
+  static __device__ __forceinline__ void run(const Args& e, const Tile16& p, const Pre<QB>& pre, Get get, int row0, int colw, int lane,
+                                             unsigned char* stage, int) {
     const int l16 = lane & 15, q = lane >> 4, lane_col = colw + 8 * q;
     float bias[2][8], sums[2][8];
 #pragma unroll
@@ -208,22 +207,43 @@ struct EpiGrad {
   }
 };
 
-// C (fp32 or bf16), one slab per K split; rows and columns behind the result are dropped.
+// C = factor * (base + A B^T), fp32 or bf16; rows and columns behind the result are dropped.
 template <bool OUT_BF16>
 struct EpiOut {
   struct Args {
     void* C;
-    long long slab;  // elements between the results of consecutive splits
     int ldc;
-    int vec;         // 16-byte stores allowed
-    int add;         // fp32: C += instead of C =
-    const float* factor;  // of the result, or null
+    int vec;              // 16-byte stores allowed
+    const float* base;    // [M][ld_base] or null; may be C
+    int ld_base;          // a multiple of 64
+    const float* factor;  // null: 1
   };
+  template <int QB>
+  struct Pre {
+    f32x4 base[QB][2][2];
+  };
+  template <int QB>
+  static __device__ __forceinline__ Pre<QB> before(const Args& e, const Tile16& p, int row0, int colw, int lane, int) {
+    Pre<QB> v;
+    if (!e.base) return v;
+#pragma unroll
+    for (int jq = 0; jq < QB; ++jq)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int row = row0 + 16 * jq + (lane & 15), col = colw + 8 * (lane >> 4) + 32 * h + 4 * k;
+          v.base[jq][h][k] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};  // rows of base have whole groups of 64 columns
+          if (row < p.M && col < p.N) v.base[jq][h][k] = *reinterpret_cast<const f32x4*>(e.base + (size_t)row * e.ld_base + col);
+        }
+    return v;
+  }
   template <int QB, class Get>
-  static __device__ __forceinline__ void run(const Args& e, const Tile16& p, Get get, int row0, int colw, int lane,
-                                             unsigned char*, int, int split) {
+  static __device__ __forceinline__ void run(const Args& e, const Tile16& p, const Pre<QB>& pre, Get get, int row0, int colw, int lane,
+                                             unsigned char*, int) {
     const int l16 = lane & 15, col0 = colw + 8 * (lane >> 4);
     const float factor = e.factor ? *e.factor : 1.0f;
+    asm volatile("" ::: "memory");  // (base was requested before the first store)
 #pragma unroll
     for (int jq = 0; jq < QB; ++jq) {
       const int row = row0 + 16 * jq + l16;
@@ -232,10 +252,16 @@ struct EpiOut {
       for (int h = 0; h < 2; ++h) {
         const int col = col0 + 32 * h;
         if (col >= p.N) continue;
-        const size_t at = (size_t)split * e.slab + (size_t)row * e.ldc + col;
+        const size_t at = (size_t)row * e.ldc + col;
         float v[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = factor * get(jq, h, i);
+        for (int i = 0; i < 8; ++i) v[i] = get(jq, h, i);
+        if (e.base) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) v[i] += pre.base[jq][h][i >> 2][i & 3];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] *= factor;
         const bool whole = e.vec && col + 8 <= p.N;
         if constexpr (OUT_BF16) {
           u16* c = reinterpret_cast<u16*>(e.C) + at;
@@ -250,18 +276,12 @@ struct EpiOut {
         } else {
           float* c = reinterpret_cast<float*>(e.C) + at;
           if (whole) {
-            f32x4* c4 = reinterpret_cast<f32x4*>(c);
-            f32x4 lo = {v[0], v[1], v[2], v[3]}, hi = {v[4], v[5], v[6], v[7]};
-            if (e.add) {
-              lo += c4[0];
-              hi += c4[1];
-            }
-            c4[0] = lo;
-            c4[1] = hi;
+            reinterpret_cast<f32x4*>(c)[0] = f32x4{v[0], v[1], v[2], v[3]};
+            reinterpret_cast<f32x4*>(c)[1] = f32x4{v[4], v[5], v[6], v[7]};
           } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-              if (col + i < p.N) c[i] = e.add ? c[i] + v[i] : v[i];
+              if (col + i < p.N) c[i] = v[i];
           }
         }
       }
@@ -269,38 +289,53 @@ struct EpiOut {
   }
 };
 
-// 256 x 256 tiles once there are enough of them for most of the 256 CUs, else 128 x 128.
-int tile_for(size_t rows, size_t cols) { return ((rows + 255) / 256) * ((cols + 255) / 256) >= 200 ? 256 : 128; }
-
 template <class Epi>
-hipError_t tiles(int tile, const u16* A, int lda, const u16* B, int ldb, int M, int N, int K, int splits, const typename Epi::Args& e,
-                 hipStream_t s) {
+hipError_t tiles(const Tile16Shape& shape, float* part, const u16* A, int lda, const u16* B, int ldb, int M, int N, int K,
+                 const typename Epi::Args& e, hipStream_t s) {
   Tile16 p{};
   p.A = A; p.B = B; p.lda = lda; p.ldb = ldb; p.M = M; p.N = N; p.K = K;
-  p.splits = splits;
-  p.tile = tile;
-  return launch_tile16<false, Epi>(p, e, 1, s);
+  p.batch = 1;
+  return launch_tile16<false, Epi>(p, shape, part, e, s);
 }
 
 // ---- joins and copies -------------------------------------------------------------------------------
 
-// Joins a row's column-block statistics.  16 rows x 16 lanes per workgroup: a lane takes every 16th block
-// of one row, the 16 lanes of a row are joined in a fixed order.
+// Joins a row's column-block statistics.  ROWS rows per workgroup, 256 / ROWS lanes on each: a lane takes every
+// so-manieth block, the lanes of a row are joined pairwise.  Few rows take many lanes each: one row over 500 blocks
+// takes 4 us with 256 lanes and 14 with 16.
+template <int ROWS>
 __global__ __launch_bounds__(256) void xent_fold_kernel(const float2* __restrict__ part, int blocks, int M, int vocab,
                                                         const int* __restrict__ target, const float* __restrict__ zt,
                                                         float* __restrict__ loss, float* __restrict__ lse) {
-  __shared__ float2 red[16][17];
-  const int r = threadIdx.x & 15, w = threadIdx.x >> 4, row = blockIdx.x * 16 + r;
+  constexpr int LANES = 256 / ROWS;
+  __shared__ float2 red[LANES][ROWS + 1];
+  const int r = threadIdx.x % ROWS, w = threadIdx.x / ROWS, row = blockIdx.x * ROWS + r;
   float m = -__builtin_inff(), s = 0.0f;
-  if (row < M)
-    for (int c = w; c < blocks; c += 16) {
+  if (row < M) {
+    int c = w;
+    for (; c + 3 * LANES < blocks; c += 4 * LANES) {
+      float2 v[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = part[(size_t)(c + k * LANES) * M + row];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) join(m, s, v[k].x, v[k].y);
+    }
+    for (; c < blocks; c += LANES) {
       const float2 v = part[(size_t)c * M + row];
       join(m, s, v.x, v.y);
     }
+  }
   red[w][r] = float2{m, s};
   __syncthreads();
+  for (int off = LANES / 2; off > 0; off >>= 1) {
+    if (w < off) {
+      const float2 v = red[w + off][r];
+      join(m, s, v.x, v.y);
+      red[w][r] = float2{m, s};
+    }
+    __syncthreads();
+  }
   if (w != 0 || row >= M) return;
-  for (int i = 1; i < 16; ++i) join(m, s, red[i][r].x, red[i][r].y);
   const int t = target[row];
   const bool counts = t >= 0 && t < vocab;
   finish_row(m, s, counts, counts ? zt[row] : 0.0f, loss + row, lse + row);
@@ -369,22 +404,17 @@ __global__ __launch_bounds__(256) void pack_transposed_kernel(u16* __restrict__ 
   }
 }
 
-// C[row][col] = factor * sum over slabs, in slab order, of part[slab][row][col] (fp32), to fp32 (add: on top of what C
-// holds) or bf16.
-template <bool OUT_BF16>
-__global__ __launch_bounds__(256) void fold_slabs_kernel(void* __restrict__ C, int ldc, const float* __restrict__ part, int ldp,
-                                                         long long slab, int slabs, int rows, int cols,
-                                                         const float* __restrict__ factor, int add) {
+// C[row][col] = sum over slabs, in slab order, of part[slab][row][col], on top of what C holds where `add`.
+__global__ __launch_bounds__(256) void fold_slabs_kernel(float* __restrict__ C, int ldc, const float* __restrict__ part, int ldp,
+                                                         long long slab, int slabs, int rows, int cols, int add) {
   const size_t n = (size_t)rows * cols, step = (size_t)gridDim.x * 256;
   for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += step) {
     const size_t r = i / cols;
     const int c = (int)(i - r * cols);
     const float* src = part + r * ldp + c;
-    float v = 0.0f;
+    float v = add ? C[r * ldc + c] : 0.0f;
     for (int k = 0; k < slabs; ++k) v += src[(size_t)k * slab];
-    if (factor) v *= *factor;
-    if constexpr (OUT_BF16) reinterpret_cast<u16*>(C)[r * ldc + c] = f2bf(v);
-    else reinterpret_cast<float*>(C)[r * ldc + c] = add ? reinterpret_cast<float*>(C)[r * ldc + c] + v : v;
+    C[r * ldc + c] = v;
   }
 }
 
@@ -515,10 +545,11 @@ struct ForwardPlan {
   int Kp;          // K rounded up to whole K steps
   int pack_cols;   // columns per launch where W has to be packed
   u16 *Xp, *Wp;
-  float* zt;
+  float *zt, *sums;
   float2* part;
   size_t bytes;
 };
+Tile16Shape stats_shape(int M, int cols, int Kp) { return cols ? tile16_shape(M, cols, Kp, false, 1, 64, 256, true) : Tile16Shape{}; }
 ForwardPlan plan_forward(char* base, int M, int V, int K) {
   ForwardPlan f{};
   Carver c{base};
@@ -528,28 +559,22 @@ ForwardPlan plan_forward(char* base, int M, int V, int K) {
   f.Wp = c.take<u16>((size_t)std::min(V, f.pack_cols) * f.Kp);
   f.zt = c.take<float>(M);
   f.part = c.take<float2>((size_t)M * (up(V, 64) / 64));
+  // (W read in place: one launch; packed: several, a workspace has to serve either)
+  f.sums = c.take<float>(std::max(stats_shape(M, V, f.Kp).part_floats,
+                                  std::max(stats_shape(M, std::min(V, f.pack_cols), f.Kp).part_floats,
+                                           stats_shape(M, V % f.pack_cols, f.Kp).part_floats)));
   f.bytes = c.used;
   return f;
 }
 
 struct BackwardPlan {
-  int Kp, Mp, piece, splits_x, splits_w;
-  int tile;        // of the launch that makes g; Mp and the pieces are multiples of it
-  int tile_x, tile_w;
-  bool sum_x;      // dX comes out of fp32 slabs
+  int Kp, Mp, piece;
+  Tile16Shape g, x, w;  // the launches that make g, dX and dW; Mp and the pieces are multiples of g's tile
+  int g_rows;           // rows of a wavefront in g's launch: one line of db_part
   u16 *Xp, *Xt, *Wp, *Wt, *G, *GT;
-  float *top, *db_part, *x_part, *w_part;
+  float *top, *db_part, *x_sum, *part;
   size_t bytes;
 };
-// Tile and K splits of a product whose result is rows x cols: 256 x 256 tiles where they fill the CUs by
-// themselves, else 128 x 128 with the K steps dealt out to reach the 256 CUs, at least eight to each.
-void shape_product(size_t rows, size_t cols, size_t steps, int* tile, int* splits) {
-  *tile = tile_for(rows, cols);
-  *splits = 1;
-  if (*tile == 256) return;
-  const size_t n = (rows + 127) / 128 * ((cols + 127) / 128);
-  *splits = (int)std::max<size_t>(1, std::min<size_t>({(256 + n - 1) / n, steps / 8, 64}));
-}
 BackwardPlan plan_backward(char* base, int M, int V, int K) {
   BackwardPlan b{};
   Carver c{base};
@@ -557,12 +582,12 @@ BackwardPlan plan_backward(char* base, int M, int V, int K) {
   // g and g^T of a piece take at most 2 x 512 MB, the copies of W's piece 256 MB each
   const size_t most = std::min(((size_t)1 << 28) / up(M, 256), ((size_t)1 << 27) / b.Kp) / 256 * 256;
   const size_t widest = std::max<size_t>(most, 256);
-  b.tile = tile_for(M, std::min<size_t>(V, widest));
-  b.Mp = (int)up(M, b.tile);
-  b.piece = (int)std::min<size_t>(up(V, b.tile), widest);
-  shape_product(M, K, b.piece / 64, &b.tile_x, &b.splits_x);
-  shape_product(b.piece, K, b.Mp / 64, &b.tile_w, &b.splits_w);
-  b.sum_x = b.splits_x > 1 || b.piece < V;
+  b.g = tile16_shape(M, (long long)std::min<size_t>(V, widest), b.Kp, false, 1, 64, 256, false);
+  b.g_rows = b.g.tile == 64 ? 16 : b.g.tile / 2;
+  b.Mp = (int)up(M, b.g.tile);
+  b.piece = (int)std::min<size_t>(up(V, b.g.tile), widest);
+  b.x = tile16_shape(M, K, b.piece, false, 1, 64, 256, true);
+  b.w = tile16_shape(b.piece, K, b.Mp, false, 1, 64, 256, true);
   b.top = c.take<float>(1);
   b.Xp = c.take<u16>((size_t)M * b.Kp);
   b.Xt = c.take<u16>((size_t)K * b.Mp);
@@ -570,9 +595,9 @@ BackwardPlan plan_backward(char* base, int M, int V, int K) {
   b.Wt = c.take<u16>((size_t)K * b.piece);
   b.G = c.take<u16>((size_t)b.Mp * b.piece);
   b.GT = c.take<u16>((size_t)b.Mp * b.piece);
-  b.db_part = c.take<float>((size_t)(b.Mp / 64) * b.piece);
-  if (b.sum_x) b.x_part = c.take<float>((size_t)b.splits_x * M * b.Kp);
-  if (b.splits_w > 1) b.w_part = c.take<float>((size_t)b.splits_w * b.piece * b.Kp);
+  b.db_part = c.take<float>((size_t)(b.Mp / b.g_rows) * b.piece);
+  b.x_sum = b.piece < V ? c.take<float>((size_t)M * b.Kp) : nullptr;
+  b.part = c.take<float>(std::max(b.x.part_floats, b.w.part_floats));
   b.bytes = c.used;
   return b;
 }
@@ -658,11 +683,16 @@ hipError_t xent_forward_bf16(int M, int V, int K, const u16* X, int ldx, const u
       w = f.Wp;
     }
     const EpiStats::Args e{bias ? bias + v0 : nullptr, target, v0, V, f.zt, f.part + (size_t)(v0 / 64) * M};
-    TRY(tiles<EpiStats>(tile_for(M, cols), X, ldx, w, w_direct ? ldw : f.Kp, M, cols, f.Kp, 1, e, s));
+    TRY(tiles<EpiStats>(stats_shape(M, cols, f.Kp), f.sums, X, ldx, w, w_direct ? ldw : f.Kp, M, cols, f.Kp, e, s));
   }
-  launch_kernel(xent_fold_kernel, dim3((M + 15) / 16), dim3(256), 0, s, (const float2*)f.part, (int)(up(V, 64) / 64), M, V,
-                target, (const float*)f.zt, loss, lse);
-  return hipGetLastError();
+  const int blocks = (int)(up(V, 64) / 64);
+  auto fold = [&](auto kern, int rows) {
+    launch_kernel(kern, dim3((M + rows - 1) / rows), dim3(256), 0, s, (const float2*)f.part, blocks, M, V, target, (const float*)f.zt,
+                  loss, lse);
+    return hipGetLastError();
+  };
+  // whole 128-byte lines of the statistics per workgroup once there are rows for every CU
+  return M <= 64 ? fold(xent_fold_kernel<1>, 1) : M <= 1024 ? fold(xent_fold_kernel<4>, 4) : fold(xent_fold_kernel<16>, 16);
 }
 
 hipError_t xent_backward_bf16(int M, int V, int K, const u16* X, int ldx, const u16* W, int ldw, const u16* Wt, int ldwt,
@@ -682,7 +712,7 @@ hipError_t xent_backward_bf16(int M, int V, int K, const u16* X, int ldx, const 
     ldx = b.Kp;
   }
   for (int v0 = 0; v0 < V; v0 += b.piece) {
-    const int cols = std::min(b.piece, V - v0), padded = (int)up(cols, b.tile), steps = (int)up(cols, 64) / 64;
+    const int cols = std::min(b.piece, V - v0), padded = (int)up(cols, b.g.tile), steps = (int)up(cols, 64) / 64;
     const u16* w = W + (size_t)v0 * ldw;
     int ld_w = ldw;
     if (!w_direct) {
@@ -691,10 +721,10 @@ hipError_t xent_backward_bf16(int M, int V, int K, const u16* X, int ldx, const 
       ld_w = b.Kp;
     }
     const EpiGrad::Args g{bias ? bias + v0 : nullptr, target, lse, dloss, top, v0, V, b.G, b.GT, padded, b.Mp, db ? b.db_part : nullptr};
-    TRY(tiles<EpiGrad>(b.tile, X, ldx, w, ld_w, M, cols, b.Kp, 1, g, s));
+    TRY(tiles<EpiGrad>(b.g, nullptr, X, ldx, w, ld_w, M, cols, b.Kp, g, s));
     if (db) {
       launch_kernel(fold_columns_kernel, dim3((cols + 255) / 256), dim3(256), 0, s, db + v0, (const float*)b.db_part, padded,
-                    b.Mp / (b.tile / 2), cols, top);
+                    b.Mp / b.g_rows, cols, top);
       TRY(hipGetLastError());
     }
     // dX (+)= g W: the caller's transposed copy where whole 16-byte chunks of it can be read
@@ -705,40 +735,24 @@ hipError_t xent_backward_bf16(int M, int V, int K, const u16* X, int ldx, const 
       wt = b.Wt;
       ld_t = padded;
     }
-    if (b.sum_x) {
-      const int splits = std::min(b.splits_x, steps);
-      const EpiOut<false>::Args e{b.x_part, (long long)M * b.Kp, b.Kp, 1, v0 > 0, nullptr};
-      TRY(tiles<EpiOut<false>>(b.tile_x, b.G, padded, wt, ld_t, M, K, steps * 64, splits, e, s));
+    const float* before = v0 > 0 ? b.x_sum : nullptr;
+    if (v0 + cols < V) {
+      const EpiOut<false>::Args e{b.x_sum, b.Kp, 1, before, b.Kp, nullptr};
+      TRY(tiles<EpiOut<false>>(b.x, b.part, b.G, padded, wt, ld_t, M, K, steps * 64, e, s));
     } else {
-      const EpiOut<true>::Args e{dX, 0, lddx, al16(dX) && lddx % 8 == 0, 0, top};
-      TRY(tiles<EpiOut<true>>(b.tile_x, b.G, padded, wt, ld_t, M, K, steps * 64, 1, e, s));
+      const EpiOut<true>::Args e{dX, lddx, al16(dX) && lddx % 8 == 0, before, b.Kp, top};
+      TRY(tiles<EpiOut<true>>(b.x, b.part, b.G, padded, wt, ld_t, M, K, steps * 64, e, s));
     }
     // dW = g^T X
-    void* dw = static_cast<char*>(dW) + (size_t)v0 * lddw * (dw_bf16 ? 2 : 4);
-    if (b.splits_w > 1) {
-      const EpiOut<false>::Args e{b.w_part, (long long)b.piece * b.Kp, b.Kp, 1, 0, nullptr};
-      TRY(tiles<EpiOut<false>>(b.tile_w, b.GT, b.Mp, b.Xt, b.Mp, cols, K, b.Mp, b.splits_w, e, s));
-      const dim3 grid(flat_grid((size_t)cols * K));
-      if (dw_bf16)
-        launch_kernel(fold_slabs_kernel<true>, grid, dim3(256), 0, s, dw, lddw, (const float*)b.w_part, b.Kp,
-                      (long long)b.piece * b.Kp, b.splits_w, cols, K, top, 0);
-      else
-        launch_kernel(fold_slabs_kernel<false>, grid, dim3(256), 0, s, dw, lddw, (const float*)b.w_part, b.Kp,
-                      (long long)b.piece * b.Kp, b.splits_w, cols, K, top, 0);
-      TRY(hipGetLastError());
-    } else if (dw_bf16) {
-      const EpiOut<true>::Args e{dw, 0, lddw, al16(dw) && lddw % 8 == 0, 0, top};
-      TRY(tiles<EpiOut<true>>(b.tile_w, b.GT, b.Mp, b.Xt, b.Mp, cols, K, b.Mp, 1, e, s));
+    if (dw_bf16) {
+      u16* dw = static_cast<u16*>(dW) + (size_t)v0 * lddw;
+      const EpiOut<true>::Args e{dw, lddw, al16(dw) && lddw % 8 == 0, nullptr, 0, top};
+      TRY(tiles<EpiOut<true>>(b.w, b.part, b.GT, b.Mp, b.Xt, b.Mp, cols, K, b.Mp, e, s));
     } else {
-      const EpiOut<false>::Args e{dw, 0, lddw, al16(dw) && lddw % 4 == 0, 0, top};
-      TRY(tiles<EpiOut<false>>(b.tile_w, b.GT, b.Mp, b.Xt, b.Mp, cols, K, b.Mp, 1, e, s));
+      float* dw = static_cast<float*>(dW) + (size_t)v0 * lddw;
+      const EpiOut<false>::Args e{dw, lddw, al16(dw) && lddw % 4 == 0, nullptr, 0, top};
+      TRY(tiles<EpiOut<false>>(b.w, b.part, b.GT, b.Mp, b.Xt, b.Mp, cols, K, b.Mp, e, s));
     }
-  }
-  if (b.sum_x) {
-    // the last piece may have had fewer splits than there are slabs; the first piece wrote them all
-    launch_kernel(fold_slabs_kernel<true>, dim3(flat_grid((size_t)M * K)), dim3(256), 0, s, (void*)dX, lddx,
-                  (const float*)b.x_part, b.Kp, (long long)M * b.Kp, std::min(b.splits_x, (int)up(std::min(b.piece, V), 64) / 64), M, K, top, 0);
-    TRY(hipGetLastError());
   }
   return hipSuccess;
 }
@@ -797,16 +811,16 @@ hipError_t xent_backward_f32(int M, int V, int K, const float* X, int ldx, const
     TRY(sgemm_tn(splits, f.Mp, f.Kp, cols_p / splits, f.Z, f.Mp, w, ld_w, dx, dx_direct ? lddx : f.Kp, (long long)f.Mp * f.Kp,
                  nullptr, 0, s, 0));
     if (!dx_direct) {
-      launch_kernel(fold_slabs_kernel<false>, dim3(flat_grid((size_t)M * K)), dim3(256), 0, s, (void*)dX, lddx,
-                    (const float*)f.x_part, f.Kp, (long long)f.Mp * f.Kp, splits, M, K, (const float*)nullptr, (int)(v0 > 0));
+      launch_kernel(fold_slabs_kernel, dim3(flat_grid((size_t)M * K)), dim3(256), 0, s, dX, lddx, (const float*)f.x_part, f.Kp,
+                    (long long)f.Mp * f.Kp, splits, M, K, (int)(v0 > 0));
       TRY(hipGetLastError());
     }
     float* dw = dW + (size_t)v0 * lddw;
     const bool dw_direct = whole(dw, lddw, cols, cols_p, K, f.Kp);
     TRY(sgemm_nn(cols_p, f.Kp, f.Mp, f.Z, f.Mp, X, ldx, dw_direct ? dw : f.w_part, dw_direct ? lddw : f.Kp, nullptr, 0, s, 0));
     if (!dw_direct) {
-      launch_kernel(fold_slabs_kernel<false>, dim3(flat_grid((size_t)cols * K)), dim3(256), 0, s, (void*)dw, lddw,
-                    (const float*)f.w_part, f.Kp, 0LL, 1, cols, K, (const float*)nullptr, 0);
+      launch_kernel(fold_slabs_kernel, dim3(flat_grid((size_t)cols * K)), dim3(256), 0, s, dw, lddw, (const float*)f.w_part, f.Kp,
+                    0LL, 1, cols, K, 0);
       TRY(hipGetLastError());
     }
   }
