@@ -131,8 +131,8 @@ struct EpiGrad : NoPre {
     int first, vocab;
     u16* G;              // [rows padded][ldg]
     u16* GT;             // [columns padded][ldgt]
-    int ldg, ldgt;
-    float* db_part;      // column sums per wavefront tile of 16 QB rows, [row0 / (16 QB)][ldg], or null
+    int ldg, ldgt, lddb;
+    float* db_part;      // column sums per wavefront tile of 16 QB rows, [row0 / (16 QB)][lddb], or null
   };
   template <int QB, class Get>
   static __device__ __forceinline__ void run(const Args& e, const Tile16& p, const Pre<QB>& pre, Get get, int row0, int colw, int lane,
@@ -190,7 +190,7 @@ struct EpiGrad : NoPre {
       }
     }
     if (e.db_part) {
-      float* dst = e.db_part + (size_t)(row0 / (16 * QB)) * e.ldg + lane_col;
+      float* dst = e.db_part + (size_t)(row0 / (16 * QB)) * e.lddb + lane_col;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
 #pragma unroll
@@ -341,28 +341,6 @@ __global__ __launch_bounds__(256) void xent_fold_kernel(const float2* __restrict
   finish_row(m, s, counts, counts ? zt[row] : 0.0f, loss + row, lse + row);
 }
 
-// *top = the largest |dloss| of the rows that count (1 if that is zero).  g is rounded to bf16 divided by it:
-// with the mean's weights, all the same, a rounding of 1 / count would shift every term the same way and
-// not average out in the sums over rows and classes.  One workgroup.
-__global__ __launch_bounds__(1024) void xent_top_kernel(const float* __restrict__ dloss, const int* __restrict__ target, int M,
-                                                        int vocab, float* __restrict__ top) {
-  __shared__ float red[1024];
-  float m = 0.0f;
-  for (int i = threadIdx.x; i < M; i += 1024) {
-    const int t = target[i];
-    const float d = fabsf(dloss[i]);
-    if (t >= 0 && t < vocab && d < __builtin_inff()) m = fmaxf(m, d);
-  }
-  red[threadIdx.x] = m;
-  __syncthreads();
-  for (int off = 512; off > 0; off >>= 1) {
-    if ((int)threadIdx.x < off) red[threadIdx.x] = fmaxf(red[threadIdx.x], red[threadIdx.x + off]);
-    __syncthreads();
-  }
-  // (below the smallest normal number the quotients could overflow)
-  if (threadIdx.x == 0) *top = red[0] >= 1.17549435e-38f ? red[0] : 1.0f;
-}
-
 // dst[rows][ldd] = src[rows][cols], zeros up to ldd.
 __global__ __launch_bounds__(256) void pack_rows_kernel(u16* __restrict__ dst, const u16* __restrict__ src, int rows, int cols,
                                                         int ld, int ldd) {
@@ -374,34 +352,81 @@ __global__ __launch_bounds__(256) void pack_rows_kernel(u16* __restrict__ dst, c
   }
 }
 
-// dst[c][r] = src[r][c] for c < cols, r < ldd; zeros from row `rows` on.  64 x 64 tiles through LDS.
-__global__ __launch_bounds__(256) void pack_transposed_kernel(u16* __restrict__ dst, const u16* __restrict__ src, int rows,
-                                                              int cols, int ld, int ldd, int vec) {
-  __shared__ __attribute__((aligned(16))) u16 tile[64][72];
-  const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;
+// dst[c][r] = src[r][c] for c < cols, r < ldd; zeros from row `rows` on.  ldd is a multiple of 64, dst 16-byte
+// aligned; vec: src is read in 16-byte pieces where a 64 x 64 tile is whole.
+struct Transposition {
+  u16* dst;
+  const u16* src;
+  int rows, cols, ld, ldd, vec;
+  int blocks_x, blocks;  // 64 x 64 tiles: across cols, and in all
+};
+__device__ __forceinline__ void transpose_tile(const Transposition& t, int block, u16 (*tile)[72]) {
+  const int by = block / t.blocks_x, r0 = by * 64, c0 = (block - by * t.blocks_x) * 64;
   const int part = threadIdx.x & 7, line = threadIdx.x >> 3;
-  if (vec && r0 + 64 <= rows && c0 + 64 <= cols) {
+  if (t.vec && r0 + 64 <= t.rows && c0 + 64 <= t.cols) {
 #pragma unroll
     for (int i = 0; i < 2; ++i)
       *reinterpret_cast<u32x4*>(&tile[line + 32 * i][part * 8]) =
-          *reinterpret_cast<const u32x4*>(src + (size_t)(r0 + line + 32 * i) * ld + c0 + part * 8);
+          *reinterpret_cast<const u32x4*>(t.src + (size_t)(r0 + line + 32 * i) * t.ld + c0 + part * 8);
   } else {
     const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
+#pragma unroll
     for (int i = ty; i < 64; i += 4)
-      tile[i][tx] = r0 + i < rows && c0 + tx < cols ? src[(size_t)(r0 + i) * ld + c0 + tx] : (u16)0;
+      tile[i][tx] = r0 + i < t.rows && c0 + tx < t.cols ? t.src[(size_t)(r0 + i) * t.ld + c0 + tx] : (u16)0;
   }
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {  // ldd is a multiple of 64 and dst 16-byte aligned
+  for (int i = 0; i < 2; ++i) {
     const int c = line + 32 * i;
-    if (c0 + c >= cols) continue;
+    if (c0 + c >= t.cols) continue;
     u16 v[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) v[k] = tile[part * 8 + k][c];
-    *reinterpret_cast<u32x4*>(dst + (size_t)(c0 + c) * ldd + r0 + part * 8) =
+    *reinterpret_cast<u32x4*>(t.dst + (size_t)(c0 + c) * t.ldd + r0 + part * 8) =
         u32x4{(unsigned)v[0] | ((unsigned)v[1] << 16), (unsigned)v[2] | ((unsigned)v[3] << 16),
               (unsigned)v[4] | ((unsigned)v[5] << 16), (unsigned)v[6] | ((unsigned)v[7] << 16)};
   }
+}
+
+// *top = the largest |dloss| of the rows that count (1 if that is zero).  g is rounded to bf16 divided by it:
+// with the mean's weights, all the same, a rounding of 1 / count would shift every term the same way and
+// not average out in the sums over rows and classes.  One workgroup.
+__device__ __forceinline__ void find_top(const float* __restrict__ dloss, const int* __restrict__ target, int M, int vocab,
+                                         float* __restrict__ top, float* red) {
+  float m = 0.0f;
+#pragma unroll 8
+  for (int i = threadIdx.x; i < M; i += 256) {
+    const int t = target[i];
+    const float d = fabsf(dloss[i]);
+    if (t >= 0 && t < vocab && d < __builtin_inff()) m = fmaxf(m, d);
+  }
+  red[threadIdx.x] = m;
+  __syncthreads();
+  for (int off = 128; off > 0; off >>= 1) {
+    if ((int)threadIdx.x < off) red[threadIdx.x] = fmaxf(red[threadIdx.x], red[threadIdx.x + off]);
+    __syncthreads();
+  }
+  // (below the smallest normal number the quotients could overflow)
+  if (threadIdx.x == 0) *top = red[0] >= 1.17549435e-38f ? red[0] : 1.0f;
+}
+
+// What the backward call needs before its products, in one launch: the first workgroup finds *top (dloss not null), the
+// others transpose X and, where it is needed (w.blocks > 0), the first piece of W.
+__global__ __launch_bounds__(256) void xent_prepare_kernel(Transposition x, Transposition w, const float* __restrict__ dloss,
+                                                           const int* __restrict__ target, int M, int vocab, float* __restrict__ top) {
+  __shared__ __attribute__((aligned(16))) u16 tile[64][72];
+  const int block = (int)blockIdx.x - 1;
+  if (block < 0) {
+    if (dloss) find_top(dloss, target, M, vocab, top, reinterpret_cast<float*>(tile));
+  } else if (block < x.blocks) {
+    transpose_tile(x, block, tile);
+  } else {
+    transpose_tile(w, block - x.blocks, tile);
+  }
+}
+__global__ __launch_bounds__(256) void xent_transpose_kernel(Transposition w) {
+  __shared__ __attribute__((aligned(16))) u16 tile[64][72];
+  transpose_tile(w, blockIdx.x, tile);
 }
 
 // C[row][col] = sum over slabs, in slab order, of part[slab][row][col], on top of what C holds where `add`.
@@ -424,6 +449,7 @@ __global__ __launch_bounds__(256) void fold_columns_kernel(float* __restrict__ o
   const int c = blockIdx.x * 256 + threadIdx.x;
   if (c >= cols) return;
   float v = 0.0f;
+#pragma unroll 8
   for (int b = 0; b < blocks; ++b) v += part[(size_t)b * ld + c];
   out[c] = factor ? v * *factor : v;
 }
@@ -445,7 +471,7 @@ __global__ __launch_bounds__(256) void pad_f32_kernel(float* __restrict__ dst, c
 __global__ __launch_bounds__(256) void xent_rows_f32_kernel(const float* __restrict__ Z, int ldz, int cols, int first, int vocab,
                                                             int last, const float* __restrict__ bias, const int* __restrict__ target,
                                                             float2* __restrict__ part, float* __restrict__ zt,
-                                                            float* __restrict__ loss, float* __restrict__ lse) {
+                                                            float* __restrict__ loss, float* __restrict__ lse, int vec) {
   __shared__ float2 red[256];
   const int row = blockIdx.x, tid = threadIdx.x;
   int t = target[row];
@@ -453,18 +479,35 @@ __global__ __launch_bounds__(256) void xent_rows_f32_kernel(const float* __restr
   t = counts ? t - first : -1;
   const float* z = Z + (size_t)row * ldz;
   float m = -__builtin_inff(), s = 0.0f;
-  for (int c = 4 * tid; c < cols; c += 1024) {
-    const f32x4 four = *reinterpret_cast<const f32x4*>(z + c);  // rows are padded to whole quadruples
-    float v[4], top = -__builtin_inff(), sum = 0.0f;
+  for (int c0 = 4 * tid; c0 < cols; c0 += 4096) {  // sixteen elements at a time, their loads in flight together
+    f32x4 four[4], add[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[i] = four[i] + (bias && c + i < cols ? bias[c + i] : 0.0f);
-      if (c + i >= cols || c + i == t) v[i] = -__builtin_inff();
-      top = fmaxf(top, v[i]);
+    for (int u = 0; u < 4; ++u) {
+      const int c = c0 + 1024 * u;
+      add[u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+      if (c >= cols) continue;
+      four[u] = *reinterpret_cast<const f32x4*>(z + c);  // rows are padded to whole quadruples
+      if (bias && vec && c + 4 <= cols) add[u] = *reinterpret_cast<const f32x4*>(bias + c);
+      else if (bias)
+        for (int i = 0; i < 4; ++i)
+          if (c + i < cols) add[u][i] = bias[c + i];
     }
+    float top = -__builtin_inff(), sum = 0.0f;
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int c = c0 + 1024 * u + i;
+        float v = -__builtin_inff();
+        if (c < cols && c != t) v = four[u][i] + add[u][i];
+        four[u][i] = v;
+        top = fmaxf(top, v);
+      }
     const float ref = finite_or_zero(top);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) sum += __builtin_amdgcn_exp2f((v[i] - ref) * LOG2E);
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum += __builtin_amdgcn_exp2f((four[u][i] - ref) * LOG2E);
     join(m, s, top, sum);
   }
   red[tid] = float2{m, s};
@@ -495,24 +538,36 @@ __global__ __launch_bounds__(256) void xent_rows_f32_kernel(const float* __restr
 __global__ __launch_bounds__(256) void xent_grad_f32_kernel(float* __restrict__ Zt, int Mp, int M, int rows, int rows_p, int first,
                                                             int vocab, const float* __restrict__ bias,
                                                             const int* __restrict__ target, const float* __restrict__ lse,
-                                                            const float* __restrict__ dloss, float* __restrict__ db) {
+                                                            const float* __restrict__ dloss, float* __restrict__ db, int vec) {
   const int j = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
   if (j >= rows_p) return;
   float* z = Zt + (size_t)j * Mp;
   const float add = bias && j < rows ? bias[j] : 0.0f;
   float sum = 0.0f;
+#pragma unroll 2
   for (int i = 4 * lane; i < Mp; i += 256) {
     f32x4 v = *reinterpret_cast<const f32x4*>(z + i);
+    int t[4];
+    float l[4], d[4];
+    if (vec && i + 4 <= M) {  // target, lse and dloss in 16-byte pieces
+      const u32x4 t4 = *reinterpret_cast<const u32x4*>(target + i);
+      const f32x4 l4 = *reinterpret_cast<const f32x4*>(lse + i), d4 = dloss ? *reinterpret_cast<const f32x4*>(dloss + i) : f32x4{1.0f, 1.0f, 1.0f, 1.0f};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) t[k] = (int)t4[k], l[k] = l4[k], d[k] = d4[k];
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        t[k] = i + k < M ? target[i + k] : -1;
+        l[k] = i + k < M ? lse[i + k] : 0.0f;
+        d[k] = i + k < M && dloss ? dloss[i + k] : 1.0f;
+      }
+    }
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      float g = 0.0f;
-      if (j < rows && i + k < M) {
-        const int t = target[i + k];
-        if (t >= 0 && t < vocab) {
-          const float x = v[k] + add - lse[i + k];
-          g = (dloss ? dloss[i + k] : 1.0f) * (t == first + j ? expm1f(x) : __builtin_amdgcn_exp2f(x * LOG2E));
-        }
-      }
+      const float x = v[k] + add - l[k];
+      float g = d[k] * __builtin_amdgcn_exp2f(x * LOG2E);
+      if (t[k] == first + j) g = d[k] * expm1f(x);
+      if (j >= rows || t[k] < 0 || t[k] >= vocab) g = 0.0f;
       v[k] = g;
       sum += g;
     }
@@ -570,6 +625,7 @@ ForwardPlan plan_forward(char* base, int M, int V, int K) {
 struct BackwardPlan {
   int Kp, Mp, piece;
   Tile16Shape g, x, w;  // the launches that make g, dX and dW; Mp and the pieces are multiples of g's tile
+  int ldg;              // of g: a line more than the piece, so that the rows of a tile do not all start in one memory channel
   int g_rows;           // rows of a wavefront in g's launch: one line of db_part
   u16 *Xp, *Xt, *Wp, *Wt, *G, *GT;
   float *top, *db_part, *x_sum, *part;
@@ -586,6 +642,7 @@ BackwardPlan plan_backward(char* base, int M, int V, int K) {
   b.g_rows = b.g.tile == 64 ? 16 : b.g.tile / 2;
   b.Mp = (int)up(M, b.g.tile);
   b.piece = (int)std::min<size_t>(up(V, b.g.tile), widest);
+  b.ldg = b.piece + 64;
   b.x = tile16_shape(M, K, b.piece, false, 1, 64, 256, true);
   b.w = tile16_shape(b.piece, K, b.Mp, false, 1, 64, 256, true);
   b.top = c.take<float>(1);
@@ -593,7 +650,7 @@ BackwardPlan plan_backward(char* base, int M, int V, int K) {
   b.Xt = c.take<u16>((size_t)K * b.Mp);
   b.Wp = c.take<u16>((size_t)std::min(V, b.piece) * b.Kp);
   b.Wt = c.take<u16>((size_t)K * b.piece);
-  b.G = c.take<u16>((size_t)b.Mp * b.piece);
+  b.G = c.take<u16>((size_t)b.Mp * b.ldg);
   b.GT = c.take<u16>((size_t)b.Mp * b.piece);
   b.db_part = c.take<float>((size_t)(b.Mp / b.g_rows) * b.piece);
   b.x_sum = b.piece < V ? c.take<float>((size_t)M * b.Kp) : nullptr;
@@ -624,6 +681,11 @@ F32Plan plan_f32(char* base, int M, int V, int K, bool backward) {
   f.Wp = c.take<float>((size_t)f.piece * f.Kp);
   f.Z = c.take<float>((size_t)f.Mp * f.piece);
   if (backward) {
+    // The products with a row per class run on 128 x 128 tiles, one per CU at a time: whole rounds of the 256 CUs
+    // first, the classes left over as a piece of their own (on smaller tiles, and only they are copied to
+    // whole tiles): 1024 x 10007 x 1024 in one piece 586 us, in pieces of 8192 and 1815 classes 5xx.
+    const int across = (int)up(f.Mp, 128) / 128, round = across >= 256 ? 128 : (256 / across) * 128;
+    if (V > round && f.piece >= V) f.piece = V / round * round;
     const size_t tiles = up(f.Mp, 128) / 128 * (up(f.Kp, 128) / 128);
     f.splits = tiles > 128 ? 1 : tiles > 64 ? 2 : 4;
     while (f.piece % (f.splits * 32) != 0) f.splits /= 2;
@@ -650,10 +712,9 @@ hipError_t pack_rows(u16* dst, const u16* src, int rows, int cols, int ld, int l
   launch_kernel(pack_rows_kernel, dim3(flat_grid((size_t)rows * ldd)), dim3(256), 0, s, dst, src, rows, cols, ld, ldd);
   return hipGetLastError();
 }
-hipError_t pack_transposed(u16* dst, const u16* src, int rows, int cols, int ld, int ldd, hipStream_t s) {
-  launch_kernel(pack_transposed_kernel, dim3((cols + 63) / 64, ldd / 64), dim3(256), 0, s, dst, src, rows, cols, ld, ldd,
-                (int)(al16(src) && ld % 8 == 0));
-  return hipGetLastError();
+Transposition transposition(u16* dst, const u16* src, int rows, int cols, int ld, int ldd) {
+  const int across = (cols + 63) / 64;
+  return Transposition{dst, src, rows, cols, ld, ldd, (int)(al16(src) && ld % 8 == 0), across, across * (ldd / 64)};
 }
 
 }  // namespace
@@ -701,11 +762,15 @@ hipError_t xent_backward_bf16(int M, int V, int K, const u16* X, int ldx, const 
   const BackwardPlan b = plan_backward(static_cast<char*>(ws), M, V, K);
   const bool x_direct = direct(X, ldx, K), w_direct = direct(W, ldw, K);
   const float* top = dloss ? b.top : nullptr;
-  if (dloss) {
-    launch_kernel(xent_top_kernel, dim3(1), dim3(1024), 0, s, dloss, target, M, V, b.top);
-    TRY(hipGetLastError());
-  }
-  TRY(pack_transposed(b.Xt, X, M, K, ldx, b.Mp, s));
+  // the caller's transposed copy serves a piece where whole 16-byte chunks of it can be read
+  auto wt_direct = [&](int v0, int cols) { return Wt && direct(Wt + v0, ldwt, cols); };
+  auto wt_copy = [&](int v0, int cols) {
+    return transposition(b.Wt, W + (size_t)v0 * ldw, cols, K, ldw, (int)up(cols, b.g.tile));
+  };
+  const int first = std::min(b.piece, V);
+  const Transposition xt = transposition(b.Xt, X, M, K, ldx, b.Mp), wt0 = wt_direct(0, first) ? Transposition{} : wt_copy(0, first);
+  launch_kernel(xent_prepare_kernel, dim3(1 + xt.blocks + wt0.blocks), dim3(256), 0, s, xt, wt0, dloss, target, M, V, b.top);
+  TRY(hipGetLastError());
   if (!x_direct) {
     TRY(pack_rows(b.Xp, X, M, K, ldx, b.Kp, s));
     X = b.Xp;
@@ -720,28 +785,32 @@ hipError_t xent_backward_bf16(int M, int V, int K, const u16* X, int ldx, const 
       w = b.Wp;
       ld_w = b.Kp;
     }
-    const EpiGrad::Args g{bias ? bias + v0 : nullptr, target, lse, dloss, top, v0, V, b.G, b.GT, padded, b.Mp, db ? b.db_part : nullptr};
+    const EpiGrad::Args g{bias ? bias + v0 : nullptr, target, lse, dloss, top, v0, V, b.G, b.GT, b.ldg, b.Mp, b.piece, db ? b.db_part : nullptr};
     TRY(tiles<EpiGrad>(b.g, nullptr, X, ldx, w, ld_w, M, cols, b.Kp, g, s));
     if (db) {
-      launch_kernel(fold_columns_kernel, dim3((cols + 255) / 256), dim3(256), 0, s, db + v0, (const float*)b.db_part, padded,
+      launch_kernel(fold_columns_kernel, dim3((cols + 255) / 256), dim3(256), 0, s, db + v0, (const float*)b.db_part, b.piece,
                     b.Mp / b.g_rows, cols, top);
       TRY(hipGetLastError());
     }
-    // dX (+)= g W: the caller's transposed copy where whole 16-byte chunks of it can be read
+    // dX (+)= g W
     const u16* wt = Wt ? Wt + v0 : nullptr;
     int ld_t = ldwt;
-    if (!wt || !direct(wt, ldwt, cols)) {
-      TRY(pack_transposed(b.Wt, W + (size_t)v0 * ldw, cols, K, ldw, padded, s));
+    if (!wt_direct(v0, cols)) {
+      if (v0 > 0) {
+        const Transposition t = wt_copy(v0, cols);
+        launch_kernel(xent_transpose_kernel, dim3(t.blocks), dim3(256), 0, s, t);
+        TRY(hipGetLastError());
+      }
       wt = b.Wt;
       ld_t = padded;
     }
     const float* before = v0 > 0 ? b.x_sum : nullptr;
     if (v0 + cols < V) {
       const EpiOut<false>::Args e{b.x_sum, b.Kp, 1, before, b.Kp, nullptr};
-      TRY(tiles<EpiOut<false>>(b.x, b.part, b.G, padded, wt, ld_t, M, K, steps * 64, e, s));
+      TRY(tiles<EpiOut<false>>(b.x, b.part, b.G, b.ldg, wt, ld_t, M, K, steps * 64, e, s));
     } else {
       const EpiOut<true>::Args e{dX, lddx, al16(dX) && lddx % 8 == 0, before, b.Kp, top};
-      TRY(tiles<EpiOut<true>>(b.x, b.part, b.G, padded, wt, ld_t, M, K, steps * 64, e, s));
+      TRY(tiles<EpiOut<true>>(b.x, b.part, b.G, b.ldg, wt, ld_t, M, K, steps * 64, e, s));
     }
     // dW = g^T X
     if (dw_bf16) {
@@ -782,7 +851,7 @@ hipError_t xent_forward_f32(int M, int V, int K, const float* X, int ldx, const 
     TRY(whole_operand(w, ld_w, f.Wp, cols, K, cols_p, f.Kp, s));
     TRY(sgemm_nt(f.Mp, cols_p, f.Kp, X, ldx, w, ld_w, f.Z, cols_p, nullptr, 0, s, 0));
     launch_kernel(xent_rows_f32_kernel, dim3(M), dim3(256), 0, s, (const float*)f.Z, cols_p, cols, v0, V, (int)(v0 + cols == V),
-                  bias ? bias + v0 : nullptr, target, f.part, f.zt, loss, lse);
+                  bias ? bias + v0 : nullptr, target, f.part, f.zt, loss, lse, (int)al16(bias));
     TRY(hipGetLastError());
   }
   return hipSuccess;
@@ -804,7 +873,8 @@ hipError_t xent_backward_f32(int M, int V, int K, const float* X, int ldx, const
     TRY(whole_operand(w, ld_w, f.Wp, cols, K, cols_p, f.Kp, s));
     TRY(sgemm_nt(cols_p, f.Mp, f.Kp, w, ld_w, X, ldx, f.Z, f.Mp, nullptr, 0, s, 0));
     launch_kernel(xent_grad_f32_kernel, dim3((cols_p + 3) / 4), dim3(256), 0, s, f.Z, f.Mp, M, cols, cols_p, v0, V,
-                  bias ? bias + v0 : nullptr, target, lse, dloss, db ? db + v0 : nullptr);
+                  bias ? bias + v0 : nullptr, target, lse, dloss, db ? db + v0 : nullptr,
+                  (int)(al16(target) && al16(lse) && al16(dloss)));
     TRY(hipGetLastError());
     const int splits = cols_p % (f.splits * 32) == 0 ? f.splits : 1;
     float* dx = dx_direct ? dX : f.x_part;
