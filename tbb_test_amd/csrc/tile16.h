@@ -393,6 +393,7 @@ struct NoPre {
 struct Tile16Shape {
   int tile = 128, full = 0, splits = 1;
   size_t part_floats = 0;
+  double us = 0.0;  // the estimate
 };
 inline long long tile16_count(long long rows, long long cols, int tile, bool symmetric, int batch) {
   const long long m = (rows + tile - 1) / tile, n = (cols + tile - 1) / tile;
@@ -425,7 +426,7 @@ inline Tile16Shape tile16_shape(long long rows, long long cols, int K, bool symm
     const double plain = rounds(items, steps);
     if (plain < best_us) {
       best_us = plain;
-      best = Tile16Shape{tile, (int)items, 1, 0};
+      best = Tile16Shape{tile, (int)items, 1, 0, plain};
     }
     if (!may_split) continue;
     for (const int round : {256, 512}) {  // whole rounds first, split what is left over
@@ -438,7 +439,7 @@ inline Tile16Shape tile16_shape(long long rows, long long cols, int K, bool symm
         const double us = rounds(full, steps) + rounds(rest * splits, few) + 4.0 + bytes / 4e6;
         if (us < best_us) {
           best_us = us;
-          best = Tile16Shape{tile, (int)full, splits, (size_t)rest * splits * tile * tile};
+          best = Tile16Shape{tile, (int)full, splits, (size_t)rest * splits * tile * tile, us};
         }
       }
     }

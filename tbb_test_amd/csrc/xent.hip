@@ -596,15 +596,30 @@ struct Carver {
   }
 };
 
+// The classes of one product in up to two launches: those that make whole rounds of 256 x 256 tiles on the 256
+// CUs, and what is left over on smaller tiles, where that is estimated to be faster than one launch (4096 x 50021
+// x 2048: 12 rounds and 869 classes on 128 x 128 tiles instead of 13 rounds).
+struct Cut {
+  int main;  // classes of the first launch; 0: only the second
+  Tile16Shape first, second;
+};
+Cut cut_classes(int M, int cols, int Kp) {
+  const Cut one{0, Tile16Shape{}, tile16_shape(M, cols, Kp, false, 1, 64, 256, false)};
+  const long long down = (M + 255) / 256, whole = down * (cols / 256) / 256 * 256;  // tiles of whole rounds
+  const int main = (int)(whole / down) * 256;
+  if (main == 0 || main == cols) return one;
+  const Cut two{main, tile16_shape(M, main, Kp, false, 1, 256, 256, false), tile16_shape(M, cols - main, Kp, false, 1, 64, 128, false)};
+  return two.first.us + two.second.us < one.second.us ? two : one;
+}
+
 struct ForwardPlan {
   int Kp;          // K rounded up to whole K steps
   int pack_cols;   // columns per launch where W has to be packed
   u16 *Xp, *Wp;
-  float *zt, *sums;
+  float* zt;
   float2* part;
   size_t bytes;
 };
-Tile16Shape stats_shape(int M, int cols, int Kp) { return cols ? tile16_shape(M, cols, Kp, false, 1, 64, 256, true) : Tile16Shape{}; }
 ForwardPlan plan_forward(char* base, int M, int V, int K) {
   ForwardPlan f{};
   Carver c{base};
@@ -614,19 +629,15 @@ ForwardPlan plan_forward(char* base, int M, int V, int K) {
   f.Wp = c.take<u16>((size_t)std::min(V, f.pack_cols) * f.Kp);
   f.zt = c.take<float>(M);
   f.part = c.take<float2>((size_t)M * (up(V, 64) / 64));
-  // (W read in place: one launch; packed: several, a workspace has to serve either)
-  f.sums = c.take<float>(std::max(stats_shape(M, V, f.Kp).part_floats,
-                                  std::max(stats_shape(M, std::min(V, f.pack_cols), f.Kp).part_floats,
-                                           stats_shape(M, V % f.pack_cols, f.Kp).part_floats)));
   f.bytes = c.used;
   return f;
 }
 
 struct BackwardPlan {
   int Kp, Mp, piece;
-  Tile16Shape g, x, w;  // the launches that make g, dX and dW; Mp and the pieces are multiples of g's tile
+  int tile;             // of g's (first) launch; Mp and the pieces are multiples of it
+  Tile16Shape x, w;     // the launches that make dX and dW
   int ldg;              // of g: a line more than the piece, so that the rows of a tile do not all start in one memory channel
-  int g_rows;           // rows of a wavefront in g's launch: one line of db_part
   u16 *Xp, *Xt, *Wp, *Wt, *G, *GT;
   float *top, *db_part, *x_sum, *part;
   size_t bytes;
@@ -638,10 +649,10 @@ BackwardPlan plan_backward(char* base, int M, int V, int K) {
   // g and g^T of a piece take at most 2 x 512 MB, the copies of W's piece 256 MB each
   const size_t most = std::min(((size_t)1 << 28) / up(M, 256), ((size_t)1 << 27) / b.Kp) / 256 * 256;
   const size_t widest = std::max<size_t>(most, 256);
-  b.g = tile16_shape(M, (long long)std::min<size_t>(V, widest), b.Kp, false, 1, 64, 256, false);
-  b.g_rows = b.g.tile == 64 ? 16 : b.g.tile / 2;
-  b.Mp = (int)up(M, b.g.tile);
-  b.piece = (int)std::min<size_t>(up(V, b.g.tile), widest);
+  const Cut cut = cut_classes(M, (int)std::min<size_t>(V, widest), b.Kp);
+  b.tile = cut.main ? cut.first.tile : cut.second.tile;
+  b.Mp = (int)up(M, b.tile);
+  b.piece = (int)std::min<size_t>(up(V, b.tile), widest);
   b.ldg = b.piece + 64;
   b.x = tile16_shape(M, K, b.piece, false, 1, 64, 256, true);
   b.w = tile16_shape(b.piece, K, b.Mp, false, 1, 64, 256, true);
@@ -652,7 +663,7 @@ BackwardPlan plan_backward(char* base, int M, int V, int K) {
   b.Wt = c.take<u16>((size_t)K * b.piece);
   b.G = c.take<u16>((size_t)b.Mp * b.ldg);
   b.GT = c.take<u16>((size_t)b.Mp * b.piece);
-  b.db_part = c.take<float>((size_t)(b.Mp / b.g_rows) * b.piece);
+  b.db_part = c.take<float>((size_t)(b.Mp / 16) * b.piece);  // (64 x 64 tiles: a line for every 16 rows)
   b.x_sum = b.piece < V ? c.take<float>((size_t)M * b.Kp) : nullptr;
   b.part = c.take<float>(std::max(b.x.part_floats, b.w.part_floats));
   b.bytes = c.used;
@@ -743,8 +754,14 @@ hipError_t xent_forward_bf16(int M, int V, int K, const u16* X, int ldx, const u
       TRY(pack_rows(f.Wp, w, cols, K, ldw, f.Kp, s));
       w = f.Wp;
     }
-    const EpiStats::Args e{bias ? bias + v0 : nullptr, target, v0, V, f.zt, f.part + (size_t)(v0 / 64) * M};
-    TRY(tiles<EpiStats>(stats_shape(M, cols, f.Kp), f.sums, X, ldx, w, w_direct ? ldw : f.Kp, M, cols, f.Kp, e, s));
+    const int ld_w = w_direct ? ldw : f.Kp;
+    const Cut cut = cut_classes(M, cols, f.Kp);
+    for (int c0 = 0; c0 < cols;) {
+      const int n = c0 < cut.main ? cut.main : cols - c0, at = v0 + c0;
+      const EpiStats::Args e{bias ? bias + at : nullptr, target, at, V, f.zt, f.part + (size_t)(at / 64) * M};
+      TRY(tiles<EpiStats>(c0 < cut.main ? cut.first : cut.second, nullptr, X, ldx, w + (size_t)c0 * ld_w, ld_w, M, n, f.Kp, e, s));
+      c0 += n;
+    }
   }
   const int blocks = (int)(up(V, 64) / 64);
   auto fold = [&](auto kern, int rows) {
@@ -765,7 +782,7 @@ hipError_t xent_backward_bf16(int M, int V, int K, const u16* X, int ldx, const 
   // the caller's transposed copy serves a piece where whole 16-byte chunks of it can be read
   auto wt_direct = [&](int v0, int cols) { return Wt && direct(Wt + v0, ldwt, cols); };
   auto wt_copy = [&](int v0, int cols) {
-    return transposition(b.Wt, W + (size_t)v0 * ldw, cols, K, ldw, (int)up(cols, b.g.tile));
+    return transposition(b.Wt, W + (size_t)v0 * ldw, cols, K, ldw, (int)up(cols, b.tile));
   };
   const int first = std::min(b.piece, V);
   const Transposition xt = transposition(b.Xt, X, M, K, ldx, b.Mp), wt0 = wt_direct(0, first) ? Transposition{} : wt_copy(0, first);
@@ -777,7 +794,7 @@ hipError_t xent_backward_bf16(int M, int V, int K, const u16* X, int ldx, const 
     ldx = b.Kp;
   }
   for (int v0 = 0; v0 < V; v0 += b.piece) {
-    const int cols = std::min(b.piece, V - v0), padded = (int)up(cols, b.g.tile), steps = (int)up(cols, 64) / 64;
+    const int cols = std::min(b.piece, V - v0), padded = (int)up(cols, b.tile), steps = (int)up(cols, 64) / 64;
     const u16* w = W + (size_t)v0 * ldw;
     int ld_w = ldw;
     if (!w_direct) {
@@ -785,12 +802,22 @@ hipError_t xent_backward_bf16(int M, int V, int K, const u16* X, int ldx, const 
       w = b.Wp;
       ld_w = b.Kp;
     }
-    const EpiGrad::Args g{bias ? bias + v0 : nullptr, target, lse, dloss, top, v0, V, b.G, b.GT, b.ldg, b.Mp, b.piece, db ? b.db_part : nullptr};
-    TRY(tiles<EpiGrad>(b.g, nullptr, X, ldx, w, ld_w, M, cols, b.Kp, g, s));
-    if (db) {
-      launch_kernel(fold_columns_kernel, dim3((cols + 255) / 256), dim3(256), 0, s, db + v0, (const float*)b.db_part, b.piece,
-                    b.Mp / b.g_rows, cols, top);
-      TRY(hipGetLastError());
+    // (the rows behind M up to Mp have to be written, as zeros, by either launch: dW sums over them)
+    Cut cut = cut_classes(M, cols, b.Kp);
+    if (cut.main == 0 || (int)up(M, cut.second.tile) != b.Mp || b.tile != 256) cut = Cut{0, {}, tile16_shape(M, cols, b.Kp, false, 1, b.tile, b.tile, false)};
+    for (int c0 = 0; c0 < cols;) {
+      const int n = c0 < cut.main ? cut.main : cols - c0, at = v0 + c0;
+      const Tile16Shape& shape = c0 < cut.main ? cut.first : cut.second;
+      const EpiGrad::Args g{bias ? bias + at : nullptr, target, lse, dloss, top, at, V, b.G + c0, b.GT + (size_t)c0 * b.Mp,
+                            b.ldg, b.Mp, b.piece, db ? b.db_part + c0 : nullptr};
+      TRY(tiles<EpiGrad>(shape, nullptr, X, ldx, w + (size_t)c0 * ld_w, ld_w, M, n, b.Kp, g, s));
+      if (db) {
+        const int lines = b.Mp / (shape.tile == 64 ? 16 : shape.tile / 2);  // a wavefront's rows each
+        launch_kernel(fold_columns_kernel, dim3((n + 255) / 256), dim3(256), 0, s, db + at, (const float*)b.db_part + c0, b.piece, lines,
+                      n, top);
+        TRY(hipGetLastError());
+      }
+      c0 += n;
     }
     // dX (+)= g W
     const u16* wt = Wt ? Wt + v0 : nullptr;

@@ -237,7 +237,9 @@ def test_fp32_logits_in_several_pieces():
 
 @pytest.mark.parametrize("M,V,K", [(4000, 3400, 64),    # the tiles of the logits fill the device
                                    (300, 4090, 3600),   # those of the weight gradient do
-                                   (4090, 200, 3400)])  # those of the input gradient do
+                                   (4090, 200, 3400),   # those of the input gradient do
+                                   (4090, 4300, 64),    # a whole round of tiles and some classes more: two launches
+                                   (3900, 4300, 64)])   # the same, but the rows are padded differently by the two
 def test_large_tiles(M, V, K):
     p = Problem(capi.MI_BF16, M, V, K)
     check_forward(p)
