@@ -11,9 +11,9 @@
 // the start and no singular value ever passes 1.21, hence |A_ij| < 1.5 and |b A + c A^2| < 2.9.
 // X is kept to 22 bits, because the a X term carries every direction from one iteration to the next and
 // grows small ones 3.4 times each: with the fp16 operand in that term its white rounding noise grows along
-// (4e-2 for a floor of 1e-2).  The diagonal of b A + c A^2, near b + c once
-// X is near its limit, stays in fp32 too and joins the a X term; its rounding would be most of what is
-// left.  Together: 2e-4 .. 8e-4 of |O|.
+// (4e-2 for a floor of 1e-2).  The diagonals of A, near 1, and of b A + c A^2, near b + c, stay in fp32 and out of
+// the products: their rounding would be most of what is left.  Together: 2e-4 .. 4e-4 of |O| on flat and
+// mixed spectra, 8e-4 on steep ones.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -192,36 +192,53 @@ __global__ __launch_bounds__(256) void ortho_scale_kernel(const float* __restric
 
 // ---- the products -----------------------------------------------------------------------------------
 
-// A = X X^T (times GRAM_SCALE, fp16): a tile of the lower triangle and its mirror image.
+// A = X X^T without its diagonal (times GRAM_SCALE, fp16): a tile of the lower triangle and its mirror image; the
+// diagonal in fp32.
 struct EpiGram : NoPre {
   struct Args {
     u16* A;
+    float* diag;
     int ld;
     long long batch;
-    float scale;
+    float scale;  // of the products, to GRAM_SCALE * A
   };
   template <int QB, class Get>
   static __device__ __forceinline__ void run(const Args& e, const Tile16& p, const Pre<QB>& pre, Get get, int row0, int colw, int lane,
                                              unsigned char* stage, int entry) {
     u16* A = e.A + (size_t)entry * e.batch;
     const int l16 = lane & 15, col = colw + 8 * (lane >> 4);
+    const bool on_diagonal = row0 / p.tile == colw / p.tile;
     u32x4 pk[QB][2];
 #pragma unroll
     for (int jq = 0; jq < QB; ++jq)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
+        const int row = row0 + 16 * jq + l16;
+        float v[8];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) pk[jq][h][k] = pack16<true>(e.scale * get(jq, h, 2 * k), e.scale * get(jq, h, 2 * k + 1));
-        *reinterpret_cast<u32x4*>(A + (size_t)(row0 + 16 * jq + l16) * e.ld + col + 32 * h) = pk[jq][h];
+        for (int i = 0; i < 8; ++i) v[i] = e.scale * get(jq, h, i);
+        if (on_diagonal) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (row == col + 32 * h + i) {
+              e.diag[(size_t)entry * e.ld + row] = v[i] * (1.0f / GRAM_SCALE);
+              v[i] = 0.0f;
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) pk[jq][h][k] = pack16<true>(v[2 * k], v[2 * k + 1]);
+        *reinterpret_cast<u32x4*>(A + (size_t)row * e.ld + col + 32 * h) = pk[jq][h];
       }
-    if (row0 / p.tile != colw / p.tile) store_transposed<QB>(A + (size_t)colw * e.ld + row0, e.ld, pk, lane, stage);
+    if (!on_diagonal) store_transposed<QB>(A + (size_t)colw * e.ld + row0, e.ld, pk, lane, stage);
   }
 };
 
-// P = b A + c A A without its diagonal (times GRAM_SCALE, fp16), the diagonal in fp32.
+// P = b A + c A A without its diagonal (times GRAM_SCALE, fp16), the diagonal in fp32.  With A = A' + D, D its
+// diagonal: P = c A' A' + b A' + c (D A' + A' D) off the diagonal, and b D + c (A' A' + D D) on it.
 struct EpiPoly {
   struct Args {
     const u16* A;
+    const float* diag_a;
     u16* P;
     float* diag;
     int ld;
@@ -230,6 +247,8 @@ struct EpiPoly {
   template <int QB>
   struct Pre {
     u32x4 a[QB][2];
+    float d_row[QB];
+    f32x4 d_col[2][2];
   };
   template <int QB>
   static __device__ __forceinline__ Pre<QB> before(const Args& e, const Tile16&, int row0, int colw, int lane, int entry) {
@@ -239,6 +258,13 @@ struct EpiPoly {
     for (int jq = 0; jq < QB; ++jq)
 #pragma unroll
       for (int h = 0; h < 2; ++h) v.a[jq][h] = *reinterpret_cast<const u32x4*>(A + (size_t)(16 * jq) * e.ld + 32 * h);
+    const float* d = e.diag_a + (size_t)entry * e.ld;
+#pragma unroll
+    for (int jq = 0; jq < QB; ++jq) v.d_row[jq] = d[row0 + (lane & 15) + 16 * jq];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) v.d_col[h][k] = *reinterpret_cast<const f32x4*>(d + colw + 8 * (lane >> 4) + 32 * h + 4 * k);
     return v;
   }
   template <int QB, class Get>
@@ -257,13 +283,16 @@ struct EpiPoly {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const unsigned w = pre.a[jq][h][i >> 1];
-          v[i] = fmaf(NS_C / GRAM_SCALE, get(jq, h, i), NS_B * ((i & 1) ? f16_hi(w) : f16_lo(w)));
+          const float factor = fmaf(NS_C, pre.d_row[jq] + pre.d_col[h][i >> 2][i & 3], NS_B);
+          v[i] = fmaf(NS_C / GRAM_SCALE, get(jq, h, i), factor * ((i & 1) ? f16_hi(w) : f16_lo(w)));
         }
         if (on_diagonal) {
 #pragma unroll
           for (int i = 0; i < 8; ++i)
             if (row == col + 32 * h + i) {
-              e.diag[(size_t)entry * e.ld + row] = v[i] * (1.0f / GRAM_SCALE);
+              // here A' is zero and v = GRAM_SCALE c (A' A')
+              const float d = pre.d_row[jq];
+              e.diag[(size_t)entry * e.ld + row] = fmaf(v[i], 1.0f / GRAM_SCALE, d * fmaf(NS_C, d, NS_B));
               v[i] = 0.0f;
             }
         }
@@ -428,7 +457,7 @@ struct Plan {
   Tile16Shape gram, poly, step;
   float* U;
   u16 *Xh, *Xl, *XhT[2], *A, *P;
-  float *diag, *part;
+  float *diag_a, *diag, *part;
   double *sumsq, *inv;
   size_t bytes;
 };
@@ -465,6 +494,7 @@ Plan plan_ortho(char* base, int batch, int rows, int cols) {
   q.XhT[1] = (u16*)take(x * 2);
   q.A = (u16*)take(a * 2);
   q.P = (u16*)take(a * 2);
+  q.diag_a = (float*)take((size_t)batch * q.mp * 4);
   q.diag = (float*)take((size_t)batch * q.mp * 4);
   q.part = (float*)take(std::max({q.gram.part_floats, q.poly.part_floats, q.step.part_floats}) * 4);
   q.sumsq = (double*)take((size_t)batch * (q.mp / 64) * (q.np / 64) * 8);
@@ -513,9 +543,9 @@ hipError_t newton_schulz(const Plan& q, GatherArgs g, bool bf16, int batch, int 
   TRY(hipGetLastError());
   const long long a = (long long)q.mp * q.mp;
   for (int k = 0; k < steps; ++k) {
-    const EpiGram::Args gram{q.A, q.mp, a, GRAM_SCALE / (q.scale * q.scale)};
+    const EpiGram::Args gram{q.A, q.diag_a, q.mp, a, GRAM_SCALE / (q.scale * q.scale)};
     TRY(tiles<EpiGram>(q, q.gram, q.Xh, q.Xh, q.mp, q.mp, q.np, batch, true, gram, s));
-    const EpiPoly::Args poly{q.A, q.P, q.diag, q.mp, a};
+    const EpiPoly::Args poly{q.A, q.diag_a, q.P, q.diag, q.mp, a};
     TRY(tiles<EpiPoly>(q, q.poly, q.A, q.A, q.mp, q.mp, q.mp, batch, true, poly, s));
     const EpiStep::Args step{q.diag, q.Xh, q.Xl, k + 1 == steps ? nullptr : q.XhT[(k + 1) & 1], q.mp, q.np, 1.0f / GRAM_SCALE};
     TRY(tiles<EpiStep>(q, q.step, q.P, q.XhT[k & 1], q.mp, q.np, q.mp, batch, false, step, s));
