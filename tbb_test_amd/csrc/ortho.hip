@@ -128,25 +128,30 @@ __global__ __launch_bounds__(256) void ortho_gather_kernel(GatherArgs p) {
   if (threadIdx.x == 0) p.sumsq[((size_t)blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x] = red[0];
 }
 
-// inv[entry] = 1 / |U|_F; 0 for U = 0, NaN where |U|_F is not finite.
-__global__ __launch_bounds__(256) void ortho_norm_kernel(const double* __restrict__ sumsq, int blocks, double* __restrict__ inv) {
-  __shared__ double red[256];
+// 1 / |U|_F from the workgroups' sums of squares; 0 for U = 0, NaN where |U|_F is not finite.  For a whole workgroup.
+__device__ __forceinline__ double inverse_norm(const double* __restrict__ sumsq, int blocks, double* red) {
   double part[8] = {};
   int i = threadIdx.x;
   for (; i + 7 * 256 < blocks; i += 8 * 256)
 #pragma unroll
-    for (int k = 0; k < 8; ++k) part[k] += sumsq[(size_t)blockIdx.x * blocks + i + 256 * k];
-  for (; i < blocks; i += 256) part[0] += sumsq[(size_t)blockIdx.x * blocks + i];
+    for (int k = 0; k < 8; ++k) part[k] += sumsq[i + 256 * k];
+  for (; i < blocks; i += 256) part[0] += sumsq[i];
   red[threadIdx.x] = ((part[0] + part[1]) + (part[2] + part[3])) + ((part[4] + part[5]) + (part[6] + part[7]));
   __syncthreads();
   for (int off = 128; off > 0; off >>= 1) {
     if ((int)threadIdx.x < off) red[threadIdx.x] += red[threadIdx.x + off];
     __syncthreads();
   }
-  if (threadIdx.x == 0) {
-    const double q = red[0];
-    inv[blockIdx.x] = q == 0.0 ? 0.0 : __builtin_isfinite(q) ? 1.0 / sqrt(q) : __builtin_nan("");
-  }
+  const double q = red[0];
+  return q == 0.0 ? 0.0 : __builtin_isfinite(q) ? 1.0 / sqrt(q) : __builtin_nan("");
+}
+
+// One launch more, for matrices with so many sums that every workgroup of the next kernel should not add them up.
+constexpr int FEW_SUMS = 1024;
+__global__ __launch_bounds__(256) void ortho_norm_kernel(const double* __restrict__ sumsq, int blocks, double* __restrict__ inv) {
+  __shared__ double red[256];
+  const double f = inverse_norm(sumsq + (size_t)blockIdx.x * blocks, blocks, red);
+  if (threadIdx.x == 0) inv[blockIdx.x] = f;
 }
 
 // X = scale * x is kept as two fp16 numbers, x rounded and 2^11 times what the rounding left: 22 bits, as much
@@ -156,12 +161,13 @@ __device__ __forceinline__ float joined(float high, float low) { return fmaf(low
 
 // X_0 = scale * U / |U|_F as two halves, and the first half transposed.  64 x 64 tiles.
 __global__ __launch_bounds__(256) void ortho_scale_kernel(const float* __restrict__ U, u16* __restrict__ Xh, u16* __restrict__ Xl,
-                                                          u16* __restrict__ XhT, int mp, int np, const double* __restrict__ inv,
-                                                          float scale) {
+                                                          u16* __restrict__ XhT, int mp, int np, const double* __restrict__ sumsq,
+                                                          int blocks, const double* __restrict__ inv, float scale) {
   __shared__ u16 tile[64][66];
+  __shared__ double red[256];
   const size_t base = (size_t)blockIdx.z * mp * np;
   const int tx = (threadIdx.x & 15) * 4, ty = threadIdx.x >> 4, r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;
-  const double f = inv[blockIdx.z] * (double)scale;
+  const double f = (double)scale * (blocks > FEW_SUMS ? inv[blockIdx.z] : inverse_norm(sumsq + (size_t)blockIdx.z * blocks, blocks, red));
 #pragma unroll
   for (int pass = 0; pass < 4; ++pass) {
     const int i = pass * 16 + ty;
@@ -536,10 +542,13 @@ hipError_t newton_schulz(const Plan& q, GatherArgs g, bool bf16, int batch, int 
     else launch_kernel((ortho_gather_kernel<false, false>), source, dim3(256), 0, s, g);
   }
   TRY(hipGetLastError());
-  launch_kernel(ortho_norm_kernel, dim3(batch), dim3(256), 0, s, (const double*)q.sumsq, (q.mp / 64) * (q.np / 64), q.inv);
-  TRY(hipGetLastError());
+  const int blocks = (q.mp / 64) * (q.np / 64);
+  if (blocks > FEW_SUMS) {
+    launch_kernel(ortho_norm_kernel, dim3(batch), dim3(256), 0, s, (const double*)q.sumsq, blocks, q.inv);
+    TRY(hipGetLastError());
+  }
   launch_kernel(ortho_scale_kernel, tiles64, dim3(256), 0, s, (const float*)q.U, q.Xh, q.Xl, q.XhT[0], q.mp, q.np,
-                (const double*)q.inv, q.scale);
+                (const double*)q.sumsq, blocks, (const double*)q.inv, q.scale);
   TRY(hipGetLastError());
   const long long a = (long long)q.mp * q.mp;
   for (int k = 0; k < steps; ++k) {

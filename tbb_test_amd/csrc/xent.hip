@@ -341,14 +341,24 @@ __global__ __launch_bounds__(256) void xent_fold_kernel(const float2* __restrict
   finish_row(m, s, counts, counts ? zt[row] : 0.0f, loss + row, lse + row);
 }
 
-// dst[rows][ldd] = src[rows][cols], zeros up to ldd.
+// dst[rows][ldd] = src[rows][cols], zeros up to ldd (a multiple of 64).  A wavefront copies 512 elements of a row, eight
+// per lane; pairs: rows of src start at multiples of 4 bytes.
 __global__ __launch_bounds__(256) void pack_rows_kernel(u16* __restrict__ dst, const u16* __restrict__ src, int rows, int cols,
-                                                        int ld, int ldd) {
-  const size_t n = (size_t)rows * ldd, step = (size_t)gridDim.x * 256;
-  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += step) {
-    const size_t r = i / ldd;
-    const int c = (int)(i - r * ldd);
-    dst[i] = c < cols ? src[r * ld + c] : (u16)0;
+                                                        int ld, int ldd, int pairs) {
+  const int c = blockIdx.x * 512 + (threadIdx.x & 63) * 8;
+  if (c >= ldd) return;
+  for (int r = blockIdx.y * 4 + (threadIdx.x >> 6); r < rows; r += gridDim.y * 4) {
+    const u16* from = src + (size_t)r * ld + c;
+    u32x4 v = {0u, 0u, 0u, 0u};
+    if (pairs && c + 8 <= cols) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) v[k] = reinterpret_cast<const unsigned*>(from)[k];
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (c + k < cols) v[k >> 1] |= (unsigned)from[k] << (16 * (k & 1));
+    }
+    *reinterpret_cast<u32x4*>(dst + (size_t)r * ldd + c) = v;
   }
 }
 
@@ -429,18 +439,25 @@ __global__ __launch_bounds__(256) void xent_transpose_kernel(Transposition w) {
   transpose_tile(w, blockIdx.x, tile);
 }
 
-// C[row][col] = sum over slabs, in slab order, of part[slab][row][col], on top of what C holds where `add`.
+// C[row][col] = sum over slabs, in slab order, of part[slab][row][col], on top of what C holds where `add`.  One
+// element per thread, 256 of a row per workgroup.
 __global__ __launch_bounds__(256) void fold_slabs_kernel(float* __restrict__ C, int ldc, const float* __restrict__ part, int ldp,
                                                          long long slab, int slabs, int rows, int cols, int add) {
-  const size_t n = (size_t)rows * cols, step = (size_t)gridDim.x * 256;
-  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += step) {
-    const size_t r = i / cols;
-    const int c = (int)(i - r * cols);
-    const float* src = part + r * ldp + c;
-    float v = add ? C[r * ldc + c] : 0.0f;
-    for (int k = 0; k < slabs; ++k) v += src[(size_t)k * slab];
-    C[r * ldc + c] = v;
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c >= cols) return;
+  for (int r = blockIdx.y; r < rows; r += gridDim.y) {
+    const float* src = part + (size_t)r * ldp + c;
+    float v = add ? C[(size_t)r * ldc + c] : 0.0f;
+#pragma unroll 4
+    for (int n = 0; n < slabs; ++n) v += src[(size_t)n * slab];
+    C[(size_t)r * ldc + c] = v;
   }
+}
+hipError_t fold_slabs(float* C, int ldc, const float* part, int ldp, long long slab, int slabs, int rows, int cols, bool add,
+                      hipStream_t s) {
+  launch_kernel(fold_slabs_kernel, dim3((cols + 255) / 256, std::min(rows, 65535)), dim3(256), 0, s, C, ldc, part, ldp, slab, slabs,
+                rows, cols, (int)add);
+  return hipGetLastError();
 }
 
 // out[c] = factor * sum over blocks of part[block][c]
@@ -459,11 +476,13 @@ __global__ __launch_bounds__(256) void fold_columns_kernel(float* __restrict__ o
 // dst[rows_p][cols_p] = src[rows][cols], zeros around it.
 __global__ __launch_bounds__(256) void pad_f32_kernel(float* __restrict__ dst, const float* __restrict__ src, int rows, int cols,
                                                       int ld, int rows_p, int cols_p) {
-  const size_t n = (size_t)rows_p * cols_p, step = (size_t)gridDim.x * 256;
-  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += step) {
-    const int r = (int)(i / cols_p), c = (int)(i - (size_t)r * cols_p);
-    dst[i] = r < rows && c < cols ? src[(size_t)r * ld + c] : 0.0f;
-  }
+  for (int r = blockIdx.y * 4 + (threadIdx.x >> 6); r < rows_p; r += gridDim.y * 4)
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int c = blockIdx.x * 512 + 64 * k + (threadIdx.x & 63);
+      if (c >= cols_p) break;
+      dst[(size_t)r * cols_p + c] = r < rows && c < cols ? src[(size_t)r * ld + c] : 0.0f;
+    }
 }
 
 // Statistics of one piece of products Z [M x cols] (the bias is added here), joined to those of the pieces
@@ -582,7 +601,8 @@ __global__ __launch_bounds__(256) void xent_grad_f32_kernel(float* __restrict__ 
 
 inline size_t up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 inline bool al16(const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0; }
-inline unsigned flat_grid(size_t n) { return (unsigned)std::min<size_t>((n + 255) / 256, 8192); }
+// Workgroups of four wavefronts, 512 columns of a row each.
+inline dim3 row_grid(int rows, int cols) { return dim3((cols + 511) / 512, std::min((rows + 3) / 4, 16384)); }
 
 // Hands out 256-byte aligned parts of a workspace (or only adds them up, base = null).
 struct Carver {
@@ -720,7 +740,8 @@ F32Plan plan_f32(char* base, int M, int V, int K, bool backward) {
 bool direct(const u16* q, int ld, int K) { return al16(q) && ld % 8 == 0 && ld <= TILE16_MAX_LD && K % 64 == 0; }
 
 hipError_t pack_rows(u16* dst, const u16* src, int rows, int cols, int ld, int ldd, hipStream_t s) {
-  launch_kernel(pack_rows_kernel, dim3(flat_grid((size_t)rows * ldd)), dim3(256), 0, s, dst, src, rows, cols, ld, ldd);
+  launch_kernel(pack_rows_kernel, row_grid(rows, ldd), dim3(256), 0, s, dst, src, rows, cols, ld, ldd,
+                (int)(reinterpret_cast<uintptr_t>(src) % 4 == 0 && ld % 2 == 0));
   return hipGetLastError();
 }
 Transposition transposition(u16* dst, const u16* src, int rows, int cols, int ld, int ldd) {
@@ -860,7 +881,7 @@ bool whole(const float* q, int ld, int rows, int rows_p, int cols, int cols_p) {
 // An operand in whole tiles: where it stands, or copied to `room`.
 hipError_t whole_operand(const float*& q, int& ld, float* room, int rows, int cols, int rows_p, int cols_p, hipStream_t s) {
   if (whole(q, ld, rows, rows_p, cols, cols_p)) return hipSuccess;
-  launch_kernel(pad_f32_kernel, dim3(flat_grid((size_t)rows_p * cols_p)), dim3(256), 0, s, room, q, rows, cols, ld, rows_p, cols_p);
+  launch_kernel(pad_f32_kernel, row_grid(rows_p, cols_p), dim3(256), 0, s, room, q, rows, cols, ld, rows_p, cols_p);
   q = room;
   ld = cols_p;
   return hipGetLastError();
@@ -908,17 +929,13 @@ hipError_t xent_backward_f32(int M, int V, int K, const float* X, int ldx, const
     TRY(sgemm_tn(splits, f.Mp, f.Kp, cols_p / splits, f.Z, f.Mp, w, ld_w, dx, dx_direct ? lddx : f.Kp, (long long)f.Mp * f.Kp,
                  nullptr, 0, s, 0));
     if (!dx_direct) {
-      launch_kernel(fold_slabs_kernel, dim3(flat_grid((size_t)M * K)), dim3(256), 0, s, dX, lddx, (const float*)f.x_part, f.Kp,
-                    (long long)f.Mp * f.Kp, splits, M, K, (int)(v0 > 0));
-      TRY(hipGetLastError());
+      TRY(fold_slabs(dX, lddx, f.x_part, f.Kp, (long long)f.Mp * f.Kp, splits, M, K, v0 > 0, s));
     }
     float* dw = dW + (size_t)v0 * lddw;
     const bool dw_direct = whole(dw, lddw, cols, cols_p, K, f.Kp);
     TRY(sgemm_nn(cols_p, f.Kp, f.Mp, f.Z, f.Mp, X, ldx, dw_direct ? dw : f.w_part, dw_direct ? lddw : f.Kp, nullptr, 0, s, 0));
     if (!dw_direct) {
-      launch_kernel(fold_slabs_kernel, dim3(flat_grid((size_t)cols * K)), dim3(256), 0, s, dw, lddw, (const float*)f.w_part, f.Kp,
-                    0LL, 1, cols, K, 0);
-      TRY(hipGetLastError());
+      TRY(fold_slabs(dw, lddw, f.w_part, f.Kp, 0, 1, cols, K, false, s));
     }
   }
   return hipSuccess;
