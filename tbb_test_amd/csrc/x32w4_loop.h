@@ -197,6 +197,11 @@ __device__ __forceinline__ void w4_loop(const W4Operands& op, int nk, unsigned l
   });
   // the compiler does not know that MFMAs have just written the accumulators it is about to read
   asm volatile("s_nop 15\n\ts_nop 15" ::: "memory");
+  // what the last step read ahead is used by nothing: kept until it has arrived, lest its registers are given away before
+#pragma unroll
+  for (int r = 0; r < 4; ++r) asm volatile("" : : "v"(fq[0][r]));
+#pragma unroll
+  for (int r = 0; r < W4_PB; ++r) asm volatile("" : : "v"(fp[0][r]));
 }
 
 }  // namespace x32

@@ -148,7 +148,7 @@ struct EpiGrad : NoPre {
         sums[h][i] = 0.0f;
       }
     const bool edge = colw + 64 > p.N;
-    const float inv_top = e.dloss ? 1.0f / *e.top : 1.0f;
+    const float top = e.dloss ? *e.top : 1.0f;
     u32x4 pk[QB][2];
 #pragma unroll
     for (int jq = 0; jq < QB; ++jq) {
@@ -157,7 +157,7 @@ struct EpiGrad : NoPre {
       const bool live = t >= 0 && t < e.vocab;
       t = t - e.first - lane_col;
       const float lse = live ? e.lse[row] : 0.0f;
-      const float d = live ? (e.dloss ? e.dloss[row] * inv_top : 1.0f) : 0.0f;
+      const float d = live ? (e.dloss ? e.dloss[row] / top : 1.0f) : 0.0f;
       float g[2][8];
 #pragma unroll
       for (int h = 0; h < 2; ++h)
@@ -635,6 +635,7 @@ Cut cut_classes(int M, int cols, int Kp) {
 struct ForwardPlan {
   int Kp;          // K rounded up to whole K steps
   int pack_cols;   // columns per launch where W has to be packed
+  int rows;        // rows at a time: the statistics of more would not fit 256 MB
   u16 *Xp, *Wp;
   float* zt;
   float2* part;
@@ -645,10 +646,11 @@ ForwardPlan plan_forward(char* base, int M, int V, int K) {
   Carver c{base};
   f.Kp = (int)up(K, 64);
   f.pack_cols = (int)std::min<size_t>(up(V, 64), std::max<size_t>(((size_t)1 << 24) / f.Kp / 256 * 256, 256));
-  f.Xp = c.take<u16>((size_t)M * f.Kp);
+  f.rows = (int)std::min<size_t>(M, std::max<size_t>(((size_t)1 << 25) / (up(V, 64) / 64) / 256 * 256, 256));
+  f.Xp = c.take<u16>((size_t)f.rows * f.Kp);
   f.Wp = c.take<u16>((size_t)std::min(V, f.pack_cols) * f.Kp);
-  f.zt = c.take<float>(M);
-  f.part = c.take<float2>((size_t)M * (up(V, 64) / 64));
+  f.zt = c.take<float>(f.rows);
+  f.part = c.take<float2>((size_t)f.rows * (up(V, 64) / 64));
   f.bytes = c.used;
   return f;
 }
@@ -758,24 +760,22 @@ size_t xent_backward_bytes(bool bf16, int M, int V, int K) {
   return bf16 ? plan_backward(nullptr, M, V, K).bytes : plan_f32(nullptr, M, V, K, true).bytes;
 }
 
-hipError_t xent_forward_bf16(int M, int V, int K, const u16* X, int ldx, const u16* W, int ldw, const float* bias,
-                             const int* target, float* loss, float* lse, void* ws, hipStream_t s) {
-  const ForwardPlan f = plan_forward(static_cast<char*>(ws), M, V, K);
-  const bool x_direct = direct(X, ldx, K), w_direct = direct(W, ldw, K);
-  if (!x_direct) {
+static hipError_t forward_rows(const ForwardPlan& f, int M, int V, int K, const u16* X, int ldx, const u16* W, int ldw,
+                               const float* bias, const int* target, float* loss, float* lse, hipStream_t s) {
+  const bool w_direct = direct(W, ldw, K);
+  if (!direct(X, ldx, K)) {
     TRY(pack_rows(f.Xp, X, M, K, ldx, f.Kp, s));
     X = f.Xp;
     ldx = f.Kp;
   }
   const int per = w_direct ? V : f.pack_cols;
   for (int v0 = 0; v0 < V; v0 += per) {
-    const int cols = std::min(per, V - v0);
+    const int cols = std::min(per, V - v0), ld_w = w_direct ? ldw : f.Kp;
     const u16* w = W + (size_t)v0 * ldw;
     if (!w_direct) {
       TRY(pack_rows(f.Wp, w, cols, K, ldw, f.Kp, s));
       w = f.Wp;
     }
-    const int ld_w = w_direct ? ldw : f.Kp;
     const Cut cut = cut_classes(M, cols, f.Kp);
     for (int c0 = 0; c0 < cols;) {
       const int n = c0 < cut.main ? cut.main : cols - c0, at = v0 + c0;
@@ -792,6 +792,14 @@ hipError_t xent_forward_bf16(int M, int V, int K, const u16* X, int ldx, const u
   };
   // whole 128-byte lines of the statistics per workgroup once there are rows for every CU
   return M <= 64 ? fold(xent_fold_kernel<1>, 1) : M <= 1024 ? fold(xent_fold_kernel<4>, 4) : fold(xent_fold_kernel<16>, 16);
+}
+
+hipError_t xent_forward_bf16(int M, int V, int K, const u16* X, int ldx, const u16* W, int ldw, const float* bias,
+                             const int* target, float* loss, float* lse, void* ws, hipStream_t s) {
+  const ForwardPlan f = plan_forward(static_cast<char*>(ws), M, V, K);
+  for (int r0 = 0; r0 < M; r0 += f.rows)
+    TRY(forward_rows(f, std::min(f.rows, M - r0), V, K, X + (size_t)r0 * ldx, ldx, W, ldw, bias, target + r0, loss + r0, lse + r0, s));
+  return hipSuccess;
 }
 
 hipError_t xent_backward_bf16(int M, int V, int K, const u16* X, int ldx, const u16* W, int ldw, const u16* Wt, int ldwt,

@@ -220,6 +220,33 @@ def test_packed_weights_in_several_launches():
     check_forward(p)
 
 
+def test_more_rows_than_fit_at_once():
+    # statistics of 2^25 / 1563 = 21248 rows at a time; the formula for the rows around the cut and at the ends
+    M, V, K = 21800, 100000, 64
+    rng = np.random.default_rng(11)
+    X, W = widen(bf16_bits(rng.standard_normal((M, K)))), widen(bf16_bits(0.25 * rng.standard_normal((V, K))))
+    t = rng.integers(-1, V, M).astype(np.int32)
+    lib, dev = capi.lib(), capi.DeviceBuffer.from_numpy
+    dX, dW, dt = dev(bf16_bits(X)), dev(bf16_bits(W)), dev(t)
+    loss, lse = Strided(1, M, M, 0, np.float32), Strided(1, M, M, 0, np.float32)
+    n = ctypes.c_size_t()
+    capi.check(lib.mi_xent_workspace(capi.MI_BF16, M, V, K, ctypes.byref(n), None))
+    assert n.value < 300 << 20
+    ws = capi.DeviceBuffer(n.value)
+    capi.check(lib.mi_xent_forward(capi.MI_BF16, M, V, K, dX.ptr, K, dW.ptr, K, None, dt.ptr, loss.ptr, lse.ptr, ws.ptr, n.value, None))
+    capi.check(lib.mi_stream_sync(None))
+    rows = np.r_[0:100, 21200:21300, M - 100:M]
+    z = X[rows].astype(np.float64) @ W.T.astype(np.float64)
+    top = z.max(1)
+    want = np.log(np.exp(z - top[:, None]).sum(1)) + top
+    counts = t[rows] >= 0
+    ez = (K + 8) * U * (np.abs(X[rows]) @ np.abs(W).T).max(1)
+    bound = ez + (2 * 40.0 + 400) * U + 2 * U * np.abs(want)
+    assert np.all(np.abs(lse.get()[0][rows] - want) <= bound)
+    picked = z[np.arange(len(rows)), np.where(counts, t[rows], 0)]
+    assert np.all(np.abs(loss.get()[0][rows] - np.where(counts, want - picked, 0.0)) <= 2 * bound)
+
+
 @pytest.mark.parametrize("M,V,K", [(2000, 64, 64), (4096, 130, 128)])
 def test_long_batch_against_few_classes(M, V, K):
     p = Problem(capi.MI_BF16, M, V, K)
