@@ -75,10 +75,9 @@ __device__ __forceinline__ void tile16_of_item(const Tile16& p, int item, int& e
 struct Tile16Job {
   int item, split, entry, tm, tn, k0, nk;
 };
-__device__ __forceinline__ Tile16Job tile16_job(const Tile16& p) {
+__device__ __forceinline__ Tile16Job tile16_job(const Tile16& p, int id) {
   Tile16Job j;
   const int steps = p.K / 64;
-  int id = blockIdx.x;
   if (id < p.full) {
     const int xcd = id & 7, rest = p.full & 7;
     j.item = xcd * (p.full >> 3) + (xcd < rest ? xcd : rest) + (id >> 3);
@@ -155,7 +154,7 @@ struct TileKernel {
 };
 
 template <bool F16, int BM, int BN, int WM, int WN, int STAGES, class Epi>
-__global__ __launch_bounds__(WM* WN * 64) void tile16_kernel(Tile16 p, typename Epi::Args e) {
+__device__ __forceinline__ void tile16_run(const Tile16& p, const typename Epi::Args& e, int workgroup) {
   using K_ = TileKernel<BM, BN, WM, WN, STAGES>;
   constexpr int NW = K_::NW, QB = K_::QB, BK = K_::BK;
   using frag = std::conditional_t<F16, f16x8, bf16x8>;
@@ -165,7 +164,7 @@ __global__ __launch_bounds__(WM* WN * 64) void tile16_kernel(Tile16 p, typename 
   const int l16 = lane & 15, q = lane >> 4;
   const int wm0 = (wave / WN) * (BM / WM), wn0 = (wave % WN) * 64;
 
-  const Tile16Job job = tile16_job(p);
+  const Tile16Job job = tile16_job(p, workgroup);
   const int m0 = job.tm * BM, n0 = job.tn * BN, nk = job.nk;
 
   unsigned offa[K_::NIA], offb[K_::NIB];
@@ -304,13 +303,18 @@ __global__ __launch_bounds__(WM* WN * 64) void tile16_kernel(Tile16 p, typename 
   Epi::template run<QB>(e, p, pre, get, m0 + wm0, n0 + wn0, lane, stage, job.entry);
 }
 
+template <bool F16, int BM, int BN, int WM, int WN, int STAGES, class Epi>
+__global__ __launch_bounds__(WM* WN * 64) void tile16_kernel(Tile16 p, typename Epi::Args e) {
+  tile16_run<F16, BM, BN, WM, WN, STAGES, Epi>(p, e, blockIdx.x);
+}
+
 // The same on tiles of 256 x 256 with four wavefronts of 128 x 128 and the hand-ordered K loop.
 template <bool F16, class Epi>
 __global__ __launch_bounds__(x32::W4_NW * 64) void tile256_kernel(Tile16 p, typename Epi::Args e) {
   extern __shared__ __attribute__((aligned(16))) u16 smem_t[];
   const unsigned lds_base = __builtin_amdgcn_readfirstlane((unsigned)(size_t)((__attribute__((address_space(3))) const void*)smem_t));
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const Tile16Job job = tile16_job(p);
+  const Tile16Job job = tile16_job(p, blockIdx.x);
   const int m0 = job.tm * x32::BM, n0 = job.tn * x32::BN;
   f32x4 acc[2][x32::QB][4];
   const x32::W4Operands op{p.A + (size_t)job.entry * p.batchA + (size_t)m0 * p.lda + (size_t)job.k0 * x32::BK,
@@ -458,23 +462,30 @@ hipError_t launch_ring(const Tile16& p, const typename Epi::Args& e, unsigned gr
 }
 
 // p.M, N, K, operands, batch and symmetric set; `shape` from tile16_shape for the same sizes, `part` with room for
-// its part_floats.
-template <bool F16, class Epi>
-hipError_t launch_tile16(Tile16 p, const Tile16Shape& shape, float* part, const typename Epi::Args& e, hipStream_t s) {
+// its part_floats.  Completes p; the number of workgroups, or -1 where they are too many.
+inline long long tile16_complete(Tile16& p, const Tile16Shape& shape, float* part) {
   p.tile = shape.tile;
   p.splits = shape.splits < p.K / 64 ? shape.splits : p.K / 64;  // a K step at least for each (a shorter last piece)
   p.part = part;
   p.tiles_m = (p.M + p.tile - 1) / p.tile;
   p.tiles_n = (p.N + p.tile - 1) / p.tile;
   const long long items = tile16_count(p.M, p.N, p.tile, p.symmetric, p.batch);
-  if (items <= 0) return hipSuccess;
+  if (items <= 0) return 0;
   p.tiles = (int)(items / p.batch);
   // a smaller product than the one the shape was made for (the last piece of a vocabulary): no more split tiles than it has
   p.full = p.splits <= 1 ? (int)items : (int)(items < shape.full ? items : shape.full);
   const long long joined = items - p.full, total = p.full + joined * p.splits;
   p.joined = (int)joined;
-  if (items > (1 << 27) || total > (1 << 27)) return hipErrorInvalidValue;
-  if ((size_t)joined * p.splits * p.tile * p.tile > shape.part_floats) return hipErrorInvalidValue;
+  if (items > (1 << 27) || total > (1 << 27)) return -1;
+  if ((size_t)joined * p.splits * p.tile * p.tile > shape.part_floats) return -1;
+  return total;
+}
+
+template <bool F16, class Epi>
+hipError_t launch_tile16(Tile16 p, const Tile16Shape& shape, float* part, const typename Epi::Args& e, hipStream_t s) {
+  const long long total = tile16_complete(p, shape, part);
+  if (total <= 0) return total == 0 ? hipSuccess : hipErrorInvalidValue;
+  const int joined = p.joined;
   const unsigned grid = (unsigned)total;
   hipError_t err = hipSuccess;
   if (p.tile == 256) {

@@ -289,13 +289,16 @@ struct EpiOut {
   }
 };
 
-template <class Epi>
-hipError_t tiles(const Tile16Shape& shape, float* part, const u16* A, int lda, const u16* B, int ldb, int M, int N, int K,
-                 const typename Epi::Args& e, hipStream_t s) {
+Tile16 product(const u16* A, int lda, const u16* B, int ldb, int M, int N, int K) {
   Tile16 p{};
   p.A = A; p.B = B; p.lda = lda; p.ldb = ldb; p.M = M; p.N = N; p.K = K;
   p.batch = 1;
-  return launch_tile16<false, Epi>(p, shape, part, e, s);
+  return p;
+}
+template <class Epi>
+hipError_t tiles(const Tile16Shape& shape, float* part, const u16* A, int lda, const u16* B, int ldb, int M, int N, int K,
+                 const typename Epi::Args& e, hipStream_t s) {
+  return launch_tile16<false, Epi>(product(A, lda, B, ldb, M, N, K), shape, part, e, s);
 }
 
 // ---- joins and copies -------------------------------------------------------------------------------
@@ -460,15 +463,43 @@ hipError_t fold_slabs(float* C, int ldc, const float* part, int ldp, long long s
   return hipGetLastError();
 }
 
-// out[c] = factor * sum over blocks of part[block][c]
-__global__ __launch_bounds__(256) void fold_columns_kernel(float* __restrict__ out, const float* __restrict__ part, int ld,
-                                                           int blocks, int cols, const float* __restrict__ factor) {
-  const int c = blockIdx.x * 256 + threadIdx.x;
-  if (c >= cols) return;
+// out[c] = factor * sum over lines of part[line][c].  64 columns per workgroup, four groups of lines added up in order.
+struct ColumnFold {
+  float* out;
+  const float* part;
+  int ld, lines, cols;
+  const float* factor;
+  int workgroups;
+};
+__device__ __forceinline__ void fold_columns(const ColumnFold& f, int workgroup, float (*red)[64]) {
+  const int l = threadIdx.x & 63, g = threadIdx.x >> 6, c = workgroup * 64 + l;
+  const int each = (f.lines + 3) / 4, from = g * each, to = min(from + each, f.lines);
   float v = 0.0f;
+  if (c < f.cols) {
 #pragma unroll 8
-  for (int b = 0; b < blocks; ++b) v += part[(size_t)b * ld + c];
-  out[c] = factor ? v * *factor : v;
+    for (int b = from; b < to; ++b) v += f.part[(size_t)b * f.ld + c];
+  }
+  red[g][l] = v;
+  __syncthreads();
+  if (g != 0 || c >= f.cols) return;
+  v = ((red[0][l] + red[1][l]) + red[2][l]) + red[3][l];
+  f.out[c] = f.factor ? v * *f.factor : v;
+}
+__global__ __launch_bounds__(256) void fold_columns_kernel(ColumnFold f) {
+  __shared__ float red[4][64];
+  fold_columns(f, blockIdx.x, red);
+}
+
+// What follows g in a backward call too small to fill the device, in one launch: dX, dW and db do not depend on each
+// other.  64 x 64 tiles; workgroups [0, nx) make dX, the next ones dW, the last ones db.
+template <class EpiX, class EpiW>
+__global__ __launch_bounds__(256) void xent_products_kernel(Tile16 px, typename EpiX::Args ex, int nx, Tile16 pw, typename EpiW::Args ew,
+                                                            int nw, ColumnFold db) {
+  extern __shared__ __attribute__((aligned(16))) u16 smem_t[];  // the tiles' ring
+  const int id = blockIdx.x;
+  if (id < nx) tile16_run<false, 64, 64, 4, 1, 4, EpiX>(px, ex, id);
+  else if (id < nx + nw) tile16_run<false, 64, 64, 4, 1, 4, EpiW>(pw, ew, id - nx);
+  else fold_columns(db, id - nx - nw, reinterpret_cast<float(*)[64]>(smem_t));
 }
 
 // ---- fp32 models ------------------------------------------------------------------------------------
@@ -716,7 +747,7 @@ F32Plan plan_f32(char* base, int M, int V, int K, bool backward) {
   if (backward) {
     // The products with a row per class run on 128 x 128 tiles, one per CU at a time: whole rounds of the 256 CUs
     // first, the classes left over as a piece of their own (on smaller tiles, and only they are copied to
-    // whole tiles): 1024 x 10007 x 1024 in one piece 586 us, in pieces of 8192 and 1815 classes 5xx.
+    // whole tiles): 1024 x 10007 x 1024 in one piece 586 us, in pieces of 8192 and 1815 classes 521.
     const int across = (int)up(f.Mp, 128) / 128, round = across >= 256 ? 128 : (256 / across) * 128;
     if (V > round && f.piece >= V) f.piece = V / round * round;
     const size_t tiles = up(f.Mp, 128) / 128 * (up(f.Kp, 128) / 128);
@@ -749,6 +780,17 @@ hipError_t pack_rows(u16* dst, const u16* src, int rows, int cols, int ld, int l
 Transposition transposition(u16* dst, const u16* src, int rows, int cols, int ld, int ldd) {
   const int across = (cols + 63) / 64;
   return Transposition{dst, src, rows, cols, ld, ldd, (int)(al16(src) && ld % 8 == 0), across, across * (ldd / 64)};
+}
+
+template <class EpiW>
+hipError_t launch_products(const Tile16& px, const EpiOut<true>::Args& ex, int nx, const Tile16& pw, const typename EpiW::Args& ew, int nw,
+                           const ColumnFold& db, hipStream_t s) {
+  using Ring = TileKernel<64, 64, 4, 1, 4>;
+  auto kern = xent_products_kernel<EpiOut<true>, EpiW>;
+  static LdsOptIn opt_in;
+  TRY(opt_in.ensure(reinterpret_cast<const void*>(kern), Ring::LDS));
+  launch_kernel(kern, dim3(nx + nw + db.workgroups), dim3(256), Ring::LDS, s, px, ex, nx, pw, ew, nw, db);
+  return hipGetLastError();
 }
 
 }  // namespace
@@ -814,6 +856,10 @@ hipError_t xent_backward_bf16(int M, int V, int K, const u16* X, int ldx, const 
     return transposition(b.Wt, W + (size_t)v0 * ldw, cols, K, ldw, (int)up(cols, b.tile));
   };
   const int first = std::min(b.piece, V);
+  // One piece and few tiles of 64 x 64: dX, dW and db share a launch (256 x 1000 x 512: 176
+  // workgroups in one launch instead of three, the call 24 -> 18.5 us).
+  const bool together = b.piece >= V && b.x.tile == 64 && b.w.tile == 64 && b.x.splits == 1 && b.w.splits == 1 &&
+                        b.x.full + b.w.full <= 512;
   const Transposition xt = transposition(b.Xt, X, M, K, ldx, b.Mp), wt0 = wt_direct(0, first) ? Transposition{} : wt_copy(0, first);
   launch_kernel(xent_prepare_kernel, dim3(1 + xt.blocks + wt0.blocks), dim3(256), 0, s, xt, wt0, dloss, target, M, V, b.top);
   TRY(hipGetLastError());
@@ -834,6 +880,7 @@ hipError_t xent_backward_bf16(int M, int V, int K, const u16* X, int ldx, const 
     // (the rows behind M up to Mp have to be written, as zeros, by either launch: dW sums over them)
     Cut cut = cut_classes(M, cols, b.Kp);
     if (cut.main == 0 || (int)up(M, cut.second.tile) != b.Mp || b.tile != 256) cut = Cut{0, {}, tile16_shape(M, cols, b.Kp, false, 1, b.tile, b.tile, false)};
+    ColumnFold fold{};
     for (int c0 = 0; c0 < cols;) {
       const int n = c0 < cut.main ? cut.main : cols - c0, at = v0 + c0;
       const Tile16Shape& shape = c0 < cut.main ? cut.first : cut.second;
@@ -842,9 +889,11 @@ hipError_t xent_backward_bf16(int M, int V, int K, const u16* X, int ldx, const 
       TRY(tiles<EpiGrad>(shape, nullptr, X, ldx, w + (size_t)c0 * ld_w, ld_w, M, n, b.Kp, g, s));
       if (db) {
         const int lines = b.Mp / (shape.tile == 64 ? 16 : shape.tile / 2);  // a wavefront's rows each
-        launch_kernel(fold_columns_kernel, dim3((n + 255) / 256), dim3(256), 0, s, db + at, (const float*)b.db_part + c0, b.piece, lines,
-                      n, top);
-        TRY(hipGetLastError());
+        fold = ColumnFold{db + at, b.db_part + c0, b.piece, lines, n, top, (n + 63) / 64};
+        if (!together) {
+          launch_kernel(fold_columns_kernel, dim3(fold.workgroups), dim3(256), 0, s, fold);
+          TRY(hipGetLastError());
+        }
       }
       c0 += n;
     }
@@ -861,23 +910,27 @@ hipError_t xent_backward_bf16(int M, int V, int K, const u16* X, int ldx, const 
       ld_t = padded;
     }
     const float* before = v0 > 0 ? b.x_sum : nullptr;
+    const EpiOut<true>::Args dx{dX, lddx, al16(dX) && lddx % 8 == 0, before, b.Kp, top};
+    void* dw = static_cast<char*>(dW) + (size_t)v0 * lddw * (dw_bf16 ? 2 : 4);
+    const EpiOut<true>::Args dw16{dw, lddw, al16(dw) && lddw % 8 == 0, nullptr, 0, top};
+    const EpiOut<false>::Args dw32{dw, lddw, al16(dw) && lddw % 4 == 0, nullptr, 0, top};
+    if (together) {
+      Tile16 px = product(b.G, b.ldg, wt, ld_t, M, K, steps * 64), pw = product(b.GT, b.Mp, b.Xt, b.Mp, cols, K, b.Mp);
+      const int nx = (int)tile16_complete(px, b.x, nullptr), nw = (int)tile16_complete(pw, b.w, nullptr);
+      if (nx < 0 || nw < 0) return hipErrorInvalidValue;
+      if (dw_bf16) TRY((launch_products<EpiOut<true>>(px, dx, nx, pw, dw16, nw, fold, s)));
+      else TRY((launch_products<EpiOut<false>>(px, dx, nx, pw, dw32, nw, fold, s)));
+      continue;
+    }
     if (v0 + cols < V) {
-      const EpiOut<false>::Args e{b.x_sum, b.Kp, 1, before, b.Kp, nullptr};
-      TRY(tiles<EpiOut<false>>(b.x, b.part, b.G, b.ldg, wt, ld_t, M, K, steps * 64, e, s));
+      const EpiOut<false>::Args sum{b.x_sum, b.Kp, 1, before, b.Kp, nullptr};
+      TRY(tiles<EpiOut<false>>(b.x, b.part, b.G, b.ldg, wt, ld_t, M, K, steps * 64, sum, s));
     } else {
-      const EpiOut<true>::Args e{dX, lddx, al16(dX) && lddx % 8 == 0, before, b.Kp, top};
-      TRY(tiles<EpiOut<true>>(b.x, b.part, b.G, b.ldg, wt, ld_t, M, K, steps * 64, e, s));
+      TRY(tiles<EpiOut<true>>(b.x, b.part, b.G, b.ldg, wt, ld_t, M, K, steps * 64, dx, s));
     }
     // dW = g^T X
-    if (dw_bf16) {
-      u16* dw = static_cast<u16*>(dW) + (size_t)v0 * lddw;
-      const EpiOut<true>::Args e{dw, lddw, al16(dw) && lddw % 8 == 0, nullptr, 0, top};
-      TRY(tiles<EpiOut<true>>(b.w, b.part, b.GT, b.Mp, b.Xt, b.Mp, cols, K, b.Mp, e, s));
-    } else {
-      float* dw = static_cast<float*>(dW) + (size_t)v0 * lddw;
-      const EpiOut<false>::Args e{dw, lddw, al16(dw) && lddw % 4 == 0, nullptr, 0, top};
-      TRY(tiles<EpiOut<false>>(b.w, b.part, b.GT, b.Mp, b.Xt, b.Mp, cols, K, b.Mp, e, s));
-    }
+    if (dw_bf16) TRY(tiles<EpiOut<true>>(b.w, b.part, b.GT, b.Mp, b.Xt, b.Mp, cols, K, b.Mp, dw16, s));
+    else TRY(tiles<EpiOut<false>>(b.w, b.part, b.GT, b.Mp, b.Xt, b.Mp, cols, K, b.Mp, dw32, s));
   }
   return hipSuccess;
 }
