@@ -222,9 +222,9 @@ int mi_convert_bf16_to_f32(float* dst, const void* src_bf16, size_t n, void* str
  *   K a multiple of 64 are read in place, others are copied into the workspace first.
  * workspace: device memory, 256-byte aligned, at least what mi_xent_workspace says for the same dtype,
  * M, V and K.  Its contents do not matter before a call and mean nothing after it; calls that may run
- * at the same time need one each.  Nothing is allocated and nothing synchronises, so the calls can be
- * captured into a graph once each has run outside a capture on that device.  Results do not depend on
- * timing: the same inputs give the same bits.
+ * at the same time need one each.  Nothing is allocated and nothing synchronises, so a call can be
+ * captured into a graph once a call of the same sizes has run outside a capture on that device.  Results
+ * do not depend on timing: the same inputs give the same bits.
  */
 int mi_xent_workspace(int dtype, int M, int V, int K, size_t* forward_bytes, size_t* backward_bytes);
 int mi_xent_forward(int dtype, int M, int V, int K, const void* X, int ldx, const void* W, int ldw,
@@ -258,7 +258,7 @@ int mi_xent_backward(int dtype, int M, int V, int K, const void* X, int ldx, con
  * (on the transposed matrix where rows > cols), which leaves singular values of G that are not tiny
  * against |G|_F between about 0.7 and 1.2.  `batch` matrices of one shape, strideG / strideO elements
  * apart; G is fp32 (in_dtype = MI_F32) or bf16, O is bf16.  The products run in fp16 with fp32
- * accumulation and the iterate is kept in fp32: O is off by about 1e-3 of |O|_F before its rounding.
+ * accumulation and the iterate is kept to 22 bits: O is off by 2e-4 .. 8e-4 of |O|_F before its rounding.
  * G = 0 gives O = 0; a G with an infinity or NaN gives NaN throughout.  O may be G itself (bf16, same
  * strides).  rows, cols: 1 .. 65536, batch: 1 .. 4096.
  * workspace as for mi_xent_forward, sized by mi_ortho_workspace for the same batch, rows and cols.

@@ -278,6 +278,31 @@ def test_same_bits_every_time_and_captured():
     rt.hipStreamDestroy(stream)
 
 
+def test_two_streams_at_once():
+    rt = ctypes.CDLL("libamdhip64.so")
+    args = (0.01, 1.0, 0.1, 0.95, 1)
+    want = []
+    for seed in (1, 2):
+        p = Update(2, 200, 300, 2, seed=seed)
+        for _ in range(4):
+            p.call(*args)
+        capi.check(capi.lib().mi_stream_sync(None))
+        want.append([x.get() for x in (p.w, p.m, p.w16, p.wt16)])
+    pair = [Update(2, 200, 300, 2, seed=seed) for seed in (1, 2)]
+    streams = [ctypes.c_void_p(), ctypes.c_void_p()]
+    for s in streams:
+        assert rt.hipStreamCreateWithFlags(ctypes.byref(s), ctypes.c_uint(1)) == 0
+    for _ in range(4):
+        for p, s in zip(pair, streams):
+            p.call(*args, stream=s)
+    for s in streams:
+        capi.check(capi.lib().mi_stream_sync(s))
+        rt.hipStreamDestroy(s)
+    for p, w in zip(pair, want):
+        for x, y in zip((p.w, p.m, p.w16, p.wt16), w):
+            assert np.array_equal(x.get().view(np.uint8), y.view(np.uint8))
+
+
 def test_one_training_step_of_a_classifier_head():
     """The operators as they are used together, on one stream with nothing waited for in between: loss and
     gradients of a linear head per replica, then the update from both replicas' weight gradients, then the loss with the

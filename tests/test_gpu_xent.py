@@ -60,7 +60,7 @@ class Strided:
 
 
 class Problem:
-    def __init__(self, dtype, M, V, K, bias=True, seed=0, pad=0, offset=0, ignored=0.2, tweak=None):
+    def __init__(self, dtype, M, V, K, bias=True, seed=0, pad=0, offset=0, ignored=0.2, tweak=None, shift=0):
         rng = np.random.default_rng(seed + 7 * M + 11 * V + 13 * K)
         self.dtype, self.M, self.V, self.K = dtype, M, V, K
         self.bf16 = dtype == capi.MI_BF16
@@ -83,9 +83,9 @@ class Problem:
         enc = bf16_bits if self.bf16 else (lambda a: a)
         self.dX_, self.dW_ = Strided(M, K, K + pad, offset, el, enc(X)), Strided(V, K, K + pad, offset, el, enc(W))
         self.dWt = Strided(K, V, V + pad, offset, el, enc(W.T)) if self.bf16 else None
-        dev = capi.DeviceBuffer.from_numpy
-        self.db_, self.dt_, self.dd_ = dev(b) if bias else None, dev(t), dev(d)
-        self.loss, self.lse = Strided(1, M, M, 0, np.float32), Strided(1, M, M, 0, np.float32)
+        vec = lambda a: Strided(1, a.size, a.size, shift, a.dtype, a)  # noqa: E731
+        self.db_, self.dt_, self.dd_ = vec(b) if bias else None, vec(t), vec(d)
+        self.loss, self.lse = Strided(1, M, M, shift, np.float32), Strided(1, M, M, shift, np.float32)
         self.pad, self.offset = pad, offset
         f, w = ctypes.c_size_t(), ctypes.c_size_t()
         capi.check(capi.lib().mi_xent_workspace(dtype, M, V, K, ctypes.byref(f), ctypes.byref(w)))
@@ -194,6 +194,13 @@ def test_loss_and_gradients(M, V, K, dtype, bias):
 @pytest.mark.parametrize("dtype", [capi.MI_BF16, capi.MI_F32], ids=["bf16", "f32"])
 def test_strides_and_alignment(dtype, pad, offset):
     p = Problem(dtype, 150, 384, 128, pad=pad, offset=offset)
+    check_forward(p)
+    check_backward(p, dtype)
+
+
+@pytest.mark.parametrize("dtype", [capi.MI_BF16, capi.MI_F32], ids=["bf16", "f32"])
+def test_vectors_that_start_anywhere(dtype):
+    p = Problem(dtype, 150, 384, 128, shift=1)  # bias, target, dloss, loss and lse at odd multiples of 4 bytes
     check_forward(p)
     check_backward(p, dtype)
 
