@@ -202,6 +202,7 @@ __global__ __launch_bounds__(256) void ortho_scale_kernel(const float* __restric
 // diagonal in fp32.  Bound by the MFMAs: 8192 x 8192 433 us for half of the product, 1270 TFLOP/s; 8 x 1024 x 1024 20 us,
 // 36 tiles of 128 x 128 on the 32 CUs of an XCD.
 struct EpiGram : NoPre {
+  static constexpr bool MAY_SPLIT = true;
   struct Args {
     u16* A;
     float* diag;
@@ -244,6 +245,7 @@ struct EpiGram : NoPre {
 // diagonal: P = c A' A' + b A' + c (D A' + A' D) off the diagonal, and b D + c (A' A' + D D) on it.  As fast as the
 // one above (449 and 23 us).
 struct EpiPoly {
+  static constexpr bool MAY_SPLIT = true;
   struct Args {
     const u16* A;
     const float* diag_a;
@@ -316,6 +318,7 @@ struct EpiPoly {
 // 902 us, 1220 TFLOP/s, of which the ten bytes an element take 0.1 ms; 8 x 1024 x 1024: 30 us, half of them those bytes
 // (17 MB in 3 us, and no K loop left to hide them behind).
 struct EpiStep {
+  static constexpr bool MAY_SPLIT = true;
   struct Args {
     const float* diag;
     u16 *Xh, *Xl, *XhT;

@@ -291,13 +291,14 @@ __device__ __forceinline__ void tile16_run(const Tile16& p, const typename Epi::
   for (int jq = 0; jq < QB; ++jq)
 #pragma unroll
     for (int ip = 0; ip < 4; ++ip) asm volatile("" : "+v"(acc[jq][ip]));
-  if (job.split >= 0) {
+  if constexpr (Epi::MAY_SPLIT)
+    if (job.split >= 0) {
 #pragma unroll
-    for (int jq = 0; jq < QB; ++jq)
+      for (int jq = 0; jq < QB; ++jq)
 #pragma unroll
-      for (int ip = 0; ip < 4; ++ip) tile16_part(p, job.item, job.split, wm0 + 16 * jq, wn0, lane)[64 * ip] = acc[jq][ip];
-    return;
-  }
+        for (int ip = 0; ip < 4; ++ip) tile16_part(p, job.item, job.split, wm0 + 16 * jq, wn0, lane)[64 * ip] = acc[jq][ip];
+      return;
+    }
   __syncthreads();  // every wavefront is done with the operand tiles: the epilogue may use the LDS
   unsigned char* stage = reinterpret_cast<unsigned char*>(smem_t) + (size_t)wave * K_::STAGE_REGION;
   auto get = [&](int jq, int h, int i) __attribute__((always_inline)) { return acc[jq][2 * h + (i >> 2)][i & 3]; };
@@ -333,19 +334,20 @@ __global__ __launch_bounds__(x32::W4_NW * 64) void tile256_kernel(Tile16 p, type
   };
   using H0 = std::integral_constant<int, 0>;
   using H1 = std::integral_constant<int, 1>;
-  if (job.split >= 0) {
-    auto half = [&](auto h_c) __attribute__((always_inline)) {
+  if constexpr (Epi::MAY_SPLIT)
+    if (job.split >= 0) {
+      auto half = [&](auto h_c) __attribute__((always_inline)) {
 #pragma unroll
-      for (int jq = 0; jq < x32::QB; ++jq)
+        for (int jq = 0; jq < x32::QB; ++jq)
 #pragma unroll
-        for (int ip = 0; ip < 4; ++ip)
-          tile16_part(p, job.item, job.split, row_e + 16 * jq, col_e + 64 * decltype(h_c)::value, lane_e)[64 * ip] =
-              f32x4{value(h_c, jq, ip, 0), value(h_c, jq, ip, 1), value(h_c, jq, ip, 2), value(h_c, jq, ip, 3)};
-    };
-    half(H0{});
-    half(H1{});
-    return;
-  }
+          for (int ip = 0; ip < 4; ++ip)
+            tile16_part(p, job.item, job.split, row_e + 16 * jq, col_e + 64 * decltype(h_c)::value, lane_e)[64 * ip] =
+                f32x4{value(h_c, jq, ip, 0), value(h_c, jq, ip, 1), value(h_c, jq, ip, 2), value(h_c, jq, ip, 3)};
+      };
+      half(H0{});
+      half(H1{});
+      return;
+    }
   __syncthreads();  // every wavefront is done with the operand tiles: the epilogue may use the LDS
   unsigned char* stage = reinterpret_cast<unsigned char*>(smem_t) + (size_t)wave * x32::STAGE_REGION;
   auto half = [&](auto h_c) __attribute__((always_inline)) {
@@ -477,11 +479,13 @@ inline long long tile16_complete(Tile16& p, const Tile16Shape& shape, float* par
   p.full = p.splits <= 1 ? (int)items : (int)(items < shape.full ? items : shape.full);
   const long long joined = items - p.full, total = p.full + joined * p.splits;
   p.joined = (int)joined;
-  if (items > (1 << 27) || total > (1 << 27)) return -1;
+  if (items > (1 << 23) || total > (1 << 23)) return -1;  // (a launch holds less than 2^32 threads)
   if ((size_t)joined * p.splits * p.tile * p.tile > shape.part_floats) return -1;
   return total;
 }
 
+// Epi::MAY_SPLIT: the epilogue can run on blocks of 16 rows in a second launch; shapes for others come from tile16_shape
+// without splits.
 template <bool F16, class Epi>
 hipError_t launch_tile16(Tile16 p, const Tile16Shape& shape, float* part, const typename Epi::Args& e, hipStream_t s) {
   const long long total = tile16_complete(p, shape, part);
@@ -504,7 +508,8 @@ hipError_t launch_tile16(Tile16 p, const Tile16Shape& shape, float* part, const 
     err = launch_ring<F16, 64, 4, 1, 4, Epi>(p, e, grid, s);
   }
   if (err != hipSuccess || joined == 0) return err;
-  launch_kernel(tile16_join_kernel<Epi>, dim3((unsigned)(joined * (p.tile / 16) * (p.tile / 64) / 4)), dim3(256), 0, s, p, e);
+  if constexpr (Epi::MAY_SPLIT)
+    launch_kernel(tile16_join_kernel<Epi>, dim3((unsigned)(joined * (p.tile / 16) * (p.tile / 64) / 4)), dim3(256), 0, s, p, e);
   return hipGetLastError();
 }
 

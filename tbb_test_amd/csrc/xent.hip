@@ -56,6 +56,7 @@ __device__ __forceinline__ void finish_row(float m, float s, bool counts, float 
 // exchanges, one pair of floats is stored.  Bound by the MFMAs: 16384 x 131072 x 4096 in 12.4 ms, 1415 TFLOP/s, what a
 // large library product reaches; with K = 2048 (32 steps a tile) the exponentials cost a tenth (1180).
 struct EpiStats : NoPre {
+  static constexpr bool MAY_SPLIT = false;
   struct Args {
     const float* bias;    // of the first column, or null
     const int* target;
@@ -127,6 +128,7 @@ struct EpiStats : NoPre {
 // g from z and lse, in both orders, and its column sums.  8192 x 32768 x 4096: 1.79 ms, 1230 TFLOP/s; the 1.07 GB of g
 // and g^T take what is missing to the products that store one result (1.58 ms).
 struct EpiGrad : NoPre {
+  static constexpr bool MAY_SPLIT = false;
   struct Args {
     const float* bias;
     const int* target;
@@ -217,6 +219,7 @@ struct EpiGrad : NoPre {
 // a power of two apart share memory channels).
 template <bool OUT_BF16>
 struct EpiOut {
+  static constexpr bool MAY_SPLIT = true;
   struct Args {
     void* C;
     int ldc;
