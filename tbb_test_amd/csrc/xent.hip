@@ -311,6 +311,127 @@ hipError_t tiles(const Tile16Shape& shape, float* part, const u16* A, int lda, c
   return launch_tile16<false, Epi>(product(A, lda, B, ldb, M, N, K), shape, part, e, s);
 }
 
+// ---- few rows against classes that the tiles cannot read in place ----------------------------------------
+
+// Statistics as EpiStats leaves them, for at most 16 QB rows: W is read once, straight into registers in 16-byte pieces
+// that may start at any element (the direct loads into LDS cannot), 16 NB classes per wavefront, AHEAD K chunks of 32
+// requested ahead of those being multiplied; X (packed, zeros behind K) comes out of the caches.  Wavefronts join to
+// blocks of 64 classes.  4 x 30592 x 2956: 52 us, 3.5 TB/s of W, where copying W for the tiles, two more passes over it,
+// makes 164; 64 x 49165 x 3501, rows at any 2 bytes: 235 us instead of 422.  More rows want more classes per wavefront
+// (X is read once for each): 16 rows 52 us with 16 classes and 53 with 32, 32 rows of 50000 x 1002 55 and 46, 64 rows
+// 245 us with 32 and 235 with 64.
+constexpr int FEW_ROWS = 64;
+struct FewRows {
+  const u16* X;  // [M][Kp]
+  const u16* W;  // [V][ldw]
+  int M, V, K, Kp, ldw;
+  const float* bias;
+  const int* target;
+  float* zt;
+  float2* part;
+};
+template <int QB, int NB, int AHEAD>
+__global__ __launch_bounds__(256) void xent_few_rows_kernel(FewRows p) {
+  struct __attribute__((packed, aligned(2))) Piece {
+    u32x4 v;
+  };
+  __shared__ float2 red[4][16 * QB];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, q = lane >> 4;
+  const int c0 = ((int)blockIdx.x * 4 + wave) * 16 * NB;
+  const u16* w[NB];
+  const u16* x[QB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b) w[b] = p.W + (size_t)min(c0 + 16 * b + l16, p.V - 1) * p.ldw + 8 * q;
+#pragma unroll
+  for (int j = 0; j < QB; ++j) x[j] = p.X + (size_t)min(16 * j + l16, p.M - 1) * p.Kp + 8 * q;
+  f32x4 acc[QB][NB];
+#pragma unroll
+  for (int j = 0; j < QB; ++j)
+#pragma unroll
+    for (int b = 0; b < NB; ++b) acc[j][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  auto multiply = [&](const u32x4(&fw)[NB], int t) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < QB; ++j) {
+      const u32x4 fx = *reinterpret_cast<const u32x4*>(x[j] + 32 * t);
+#pragma unroll
+      for (int b = 0; b < NB; ++b)
+        acc[j][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, fw[b]), __builtin_bit_cast(bf16x8, fx), acc[j][b], 0, 0, 0);
+    }
+  };
+  const int whole = p.K / 32;
+  u32x4 now[AHEAD][NB], next[AHEAD][NB];
+  auto request = [&](u32x4(&f)[AHEAD][NB], int t) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+      for (int b = 0; b < NB; ++b) f[u][b] = reinterpret_cast<const Piece*>(w[b] + 32 * (t + u))->v;
+  };
+  int t = 0;
+  if (t + AHEAD <= whole) request(now, t);
+  for (; t + AHEAD <= whole; t += AHEAD) {
+    if (t + 2 * AHEAD <= whole) request(next, t + AHEAD);
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) multiply(now[u], t + u);
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+      for (int b = 0; b < NB; ++b) now[u][b] = next[u][b];
+  }
+  for (; 32 * t < p.K; ++t) {  // the chunks left over, the last of them element by element where it is cut
+    u32x4 fw[NB];
+    const int there = p.K - 32 * t - 8 * q;  // elements of the lane's eight that are there
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      fw[b] = u32x4{0u, 0u, 0u, 0u};
+      if (there >= 8) fw[b] = reinterpret_cast<const Piece*>(w[b] + 32 * t)->v;
+      else
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (i < there) fw[b][i >> 1] |= (unsigned)w[b][32 * t + i] << (16 * (i & 1));
+    }
+    multiply(fw, t);
+  }
+  // a lane holds classes c0 + 16 b + 4 q + r of row 16 j + l16
+#pragma unroll
+  for (int j = 0; j < QB; ++j) {
+    const int row = 16 * j + l16;
+    int target = row < p.M ? p.target[row] : -1;
+    if (target >= p.V) target = -1;
+    float top = -__builtin_inff(), sum = 0.0f;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int c = c0 + 16 * b + 4 * q + r;
+        float v = acc[j][b][r] + (p.bias && c < p.V ? p.bias[c] : 0.0f);
+        if (c == target) p.zt[row] = v;
+        if (c == target || c >= p.V) v = -__builtin_inff();
+        acc[j][b][r] = v;
+        top = fmaxf(top, v);
+      }
+    top = fmaxf(top, __shfl_xor(top, 16, 64));
+    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    const float ref = finite_or_zero(top);
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) sum += __builtin_amdgcn_exp2f((acc[j][b][r] - ref) * LOG2E);
+    sum += __shfl_xor(sum, 16, 64);
+    sum += __shfl_xor(sum, 32, 64);
+    if (q == 0) red[wave][row] = float2{top, sum};
+  }
+  __syncthreads();
+  // NB blocks of 64 classes per workgroup, 4 / NB wavefronts each
+  for (int i = threadIdx.x; i < NB * 16 * QB; i += 256) {
+    const int b = i / (16 * QB), row = i % (16 * QB), block = blockIdx.x * NB + b;
+    if (row >= p.M || 64 * block >= p.V) continue;
+    float2 all = red[b * (4 / NB)][row];
+#pragma unroll
+    for (int k = 1; k < 4 / NB; ++k) join(all.x, all.y, red[b * (4 / NB) + k][row].x, red[b * (4 / NB) + k][row].y);
+    p.part[(size_t)block * p.M + row] = all;
+  }
+}
+
 // ---- joins and copies -------------------------------------------------------------------------------
 
 // Joins a row's column-block statistics.  ROWS rows per workgroup, 256 / ROWS lanes on each: a lane takes every
@@ -743,14 +864,19 @@ struct F32Plan {
   size_t bytes;
 };
 int whole_tiles(int n) { return (int)(n >= 128 ? up(n, 128) : up(n, 32)); }
+// K: a dimension of dX and dW too, whose tiles are 64 wide at least; the forward products only need whole K steps.
+int whole_k(int K, bool backward) { return !backward ? (int)up(K, 32) : K % 64 == 0 ? K : whole_tiles(K); }
 F32Plan plan_f32(char* base, int M, int V, int K, bool backward) {
   F32Plan f{};
   Carver c{base};
   f.Mp = whole_tiles(M);
-  f.Kp = whole_tiles(K);
+  f.Kp = whole_k(K, backward);
   // a piece of products and a piece of W take at most 1 GB each
   const size_t most = std::max<size_t>(((size_t)1 << 28) / std::max(f.Mp, f.Kp) / 128 * 128, 128);
   f.piece = (int)std::min<size_t>(whole_tiles(V), most);
+  // Where W is large (8 M elements: two more passes over it take 13 us, a piece more about as long), the classes that make
+  // whole tiles are read in place and those left over are a piece of their own, copied to whole tiles.
+  if (f.piece >= V && V % 128 != 0 && V > 128 && (size_t)V * K >= ((size_t)1 << 23)) f.piece = V / 128 * 128;
   f.Xp = c.take<float>((size_t)f.Mp * f.Kp);
   f.Wp = c.take<float>((size_t)f.piece * f.Kp);
   f.Z = c.take<float>((size_t)f.Mp * f.piece);
@@ -759,7 +885,7 @@ F32Plan plan_f32(char* base, int M, int V, int K, bool backward) {
     // first, the classes left over as a piece of their own (on smaller tiles, and only they are copied to
     // whole tiles): 1024 x 10007 x 1024 in one piece 586 us, in pieces of 8192 and 1815 classes 521.
     const int across = (int)up(f.Mp, 128) / 128, round = across >= 256 ? 128 : (256 / across) * 128;
-    if (V > round && f.piece >= V) f.piece = V / round * round;
+    if (V > round && f.piece >= V / 128 * 128) f.piece = V / round * round;
     const size_t tiles = up(f.Mp, 128) / 128 * (up(f.Kp, 128) / 128);
     f.splits = tiles > 128 ? 1 : tiles > 64 ? 2 : 4;
     while (f.piece % (f.splits * 32) != 0) f.splits /= 2;
@@ -814,14 +940,22 @@ size_t xent_backward_bytes(bool bf16, int M, int V, int K) {
 
 static hipError_t forward_rows(const ForwardPlan& f, int M, int V, int K, const u16* X, int ldx, const u16* W, int ldw,
                                const float* bias, const int* target, float* loss, float* lse, hipStream_t s) {
-  const bool w_direct = direct(W, ldw, K);
-  if (!direct(X, ldx, K)) {
+  const bool w_direct = direct(W, ldw, K), few = !w_direct && M <= FEW_ROWS;
+  if (few || !direct(X, ldx, K)) {
     TRY(pack_rows(f.Xp, X, M, K, ldx, f.Kp, s));
     X = f.Xp;
     ldx = f.Kp;
   }
+  if (few) {
+    const FewRows p{X, W, M, V, K, f.Kp, ldw, bias, target, f.zt, f.part};
+    auto go = [&](auto kern, int nb) { launch_kernel(kern, dim3((V + 64 * nb - 1) / (64 * nb)), dim3(256), 0, s, p); };
+    if (M <= 16) go(xent_few_rows_kernel<1, 1, 8>, 1);
+    else if (M <= 32) go(xent_few_rows_kernel<2, 2, 4>, 2);
+    else go(xent_few_rows_kernel<4, 4, 2>, 4);
+    TRY(hipGetLastError());
+  }
   const int per = w_direct ? V : f.pack_cols;
-  for (int v0 = 0; v0 < V; v0 += per) {
+  for (int v0 = few ? V : 0; v0 < V; v0 += per) {
     const int cols = std::min(per, V - v0), ld_w = w_direct ? ldw : f.Kp;
     const u16* w = W + (size_t)v0 * ldw;
     if (!w_direct) {

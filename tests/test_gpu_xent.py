@@ -190,6 +190,19 @@ def test_loss_and_gradients(M, V, K, dtype, bias):
     check_backward(p, dtype)
 
 
+@pytest.mark.parametrize("M,V,K", [(1, 300, 37), (9, 1000, 300), (16, 333, 31), (17, 700, 515), (33, 129, 1001), (64, 2000, 260)])
+@pytest.mark.parametrize("pad,offset", [(0, 0), (1, 1)])
+def test_few_rows_against_unaligned_classes(M, V, K, pad, offset):
+    p = Problem(capi.MI_BF16, M, V, K, pad=pad, offset=offset)
+    check_forward(p)
+
+
+def test_fp32_classes_that_are_no_whole_tiles():
+    p = Problem(capi.MI_F32, 40, 66000, 128)  # most read in place, 80 left over
+    check_forward(p)
+    check_backward(p, capi.MI_F32)
+
+
 @pytest.mark.parametrize("pad,offset", [(8, 0), (8, 8), (0, 1), (3, 0), (5, 3)])
 @pytest.mark.parametrize("dtype", [capi.MI_BF16, capi.MI_F32], ids=["bf16", "f32"])
 def test_strides_and_alignment(dtype, pad, offset):
