@@ -213,8 +213,9 @@ int mi_convert_bf16_to_f32(float* dst, const void* src_bf16, size_t n, void* str
  *   lse[i]  = log sum_j exp z_ij
  *   loss[i] = lse[i] - z_i,target[i]
  * A target outside [0, V) marks a row that does not count (padding): its loss is 0 and its gradient
- * zero; its lse is still written.  Infinite logits mean what they mean in the formula: -inf (a bias of
- * -inf, say) is a class of probability zero, +inf or NaN makes the row's lse +inf or NaN.
+ * zero, and it adds nothing to dW and dbias, whatever X and dloss hold there; its lse is still written.
+ * Infinite logits mean what they mean in the formula: -inf (a bias of -inf, say) is a class of
+ * probability zero, +inf or NaN makes the row's lse +inf or NaN.
  * Stands beside mi_l2_loss_static; no counterpart in the reference, whose harness has the L2 loss only.
  *   dtype MI_BF16: X and W bf16, MFMA products with fp32 accumulation; MI_F32: X and W fp32.
  *   bias, loss, lse, dloss, dbias: fp32.  target: 32-bit integers.  bias may be NULL.

@@ -496,27 +496,40 @@ __global__ __launch_bounds__(256) void pack_rows_kernel(u16* __restrict__ dst, c
   }
 }
 
-// dst[c][r] = src[r][c] for c < cols, r < ldd; zeros from row `rows` on.  ldd is a multiple of 64, dst 16-byte
+// Whether row r counts; target = null: every row does.
+__device__ __forceinline__ bool row_counts(const int* __restrict__ target, int vocab, int r) {
+  if (!target) return true;
+  const int t = target[r];
+  return t >= 0 && t < vocab;
+}
+
+// dst[c][r] = src[r][c] for c < cols, r < ldd; zeros from row `rows` on, and for rows that do not count (their g is
+// zero, but zero times an infinity or NaN would reach every dW).  ldd is a multiple of 64, dst 16-byte
 // aligned; vec: src is read in 16-byte pieces where a 64 x 64 tile is whole.
 struct Transposition {
   u16* dst;
   const u16* src;
   int rows, cols, ld, ldd, vec;
   int blocks_x, blocks;  // 64 x 64 tiles: across cols, and in all
+  const int* target;     // of the rows, or null
+  int vocab;
 };
 __device__ __forceinline__ void transpose_tile(const Transposition& t, int block, u16 (*tile)[72]) {
   const int by = block / t.blocks_x, r0 = by * 64, c0 = (block - by * t.blocks_x) * 64;
   const int part = threadIdx.x & 7, line = threadIdx.x >> 3;
   if (t.vec && r0 + 64 <= t.rows && c0 + 64 <= t.cols) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-      *reinterpret_cast<u32x4*>(&tile[line + 32 * i][part * 8]) =
-          *reinterpret_cast<const u32x4*>(t.src + (size_t)(r0 + line + 32 * i) * t.ld + c0 + part * 8);
+    for (int i = 0; i < 2; ++i) {
+      const int r = line + 32 * i;
+      const u32x4 v = *reinterpret_cast<const u32x4*>(t.src + (size_t)(r0 + r) * t.ld + c0 + part * 8);
+      *reinterpret_cast<u32x4*>(&tile[r][part * 8]) = row_counts(t.target, t.vocab, r0 + r) ? v : u32x4{0u, 0u, 0u, 0u};
+    }
   } else {
     const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
 #pragma unroll
     for (int i = ty; i < 64; i += 4)
-      tile[i][tx] = r0 + i < t.rows && c0 + tx < t.cols ? t.src[(size_t)(r0 + i) * t.ld + c0 + tx] : (u16)0;
+      tile[i][tx] = r0 + i < t.rows && c0 + tx < t.cols && row_counts(t.target, t.vocab, r0 + i)
+                        ? t.src[(size_t)(r0 + i) * t.ld + c0 + tx] : (u16)0;
   }
   __syncthreads();
 #pragma unroll
@@ -635,16 +648,26 @@ __global__ __launch_bounds__(256) void xent_products_kernel(Tile16 px, typename 
 
 // ---- fp32 models ------------------------------------------------------------------------------------
 
-// dst[rows_p][cols_p] = src[rows][cols], zeros around it.
+// dst[rows_p][cols_p] = src[rows][cols], zeros around it and for rows that do not count.  Whole 16-byte pieces
+// where src has them (vec); cols_p is a multiple of 32.
 __global__ __launch_bounds__(256) void pad_f32_kernel(float* __restrict__ dst, const float* __restrict__ src, int rows, int cols,
-                                                      int ld, int rows_p, int cols_p) {
-  for (int r = blockIdx.y * 4 + (threadIdx.x >> 6); r < rows_p; r += gridDim.y * 4)
+                                                      int ld, int rows_p, int cols_p, const int* __restrict__ target, int vocab, int vec) {
+  for (int r = blockIdx.y * 4 + (threadIdx.x >> 6); r < rows_p; r += gridDim.y * 4) {
+    const bool there = r < rows && row_counts(target, vocab, r);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const int c = blockIdx.x * 512 + 64 * k + (threadIdx.x & 63);
+    for (int k = 0; k < 2; ++k) {
+      const int c = blockIdx.x * 512 + 256 * k + 4 * (threadIdx.x & 63);
       if (c >= cols_p) break;
-      dst[(size_t)r * cols_p + c] = r < rows && c < cols ? src[(size_t)r * ld + c] : 0.0f;
+      const float* from = src + (size_t)r * ld + c;
+      f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+      if (there && vec && c + 4 <= cols) v = *reinterpret_cast<const f32x4*>(from);
+      else if (there)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (c + i < cols) v[i] = from[i];
+      *reinterpret_cast<f32x4*>(dst + (size_t)r * cols_p + c) = v;
     }
+  }
 }
 
 // (1024 x 32000: 24 us, 5.4 TB/s.)  Statistics of one piece of products Z [M x cols] (the bias is added here), joined to those of the pieces
@@ -915,7 +938,7 @@ hipError_t pack_rows(u16* dst, const u16* src, int rows, int cols, int ld, int l
 }
 Transposition transposition(u16* dst, const u16* src, int rows, int cols, int ld, int ldd) {
   const int across = (cols + 63) / 64;
-  return Transposition{dst, src, rows, cols, ld, ldd, (int)(al16(src) && ld % 8 == 0), across, across * (ldd / 64)};
+  return Transposition{dst, src, rows, cols, ld, ldd, (int)(al16(src) && ld % 8 == 0), across, across * (ldd / 64), nullptr, 0};
 }
 
 template <class EpiW>
@@ -1004,7 +1027,10 @@ hipError_t xent_backward_bf16(int M, int V, int K, const u16* X, int ldx, const 
   // workgroups in one launch instead of three, the call 24 -> 18.5 us).
   const bool together = b.piece >= V && b.x.tile == 64 && b.w.tile == 64 && b.x.splits == 1 && b.w.splits == 1 &&
                         b.x.full + b.w.full <= 512;
-  const Transposition xt = transposition(b.Xt, X, M, K, ldx, b.Mp), wt0 = wt_direct(0, first) ? Transposition{} : wt_copy(0, first);
+  Transposition xt = transposition(b.Xt, X, M, K, ldx, b.Mp);
+  xt.target = target;
+  xt.vocab = V;
+  const Transposition wt0 = wt_direct(0, first) ? Transposition{} : wt_copy(0, first);
   launch_kernel(xent_prepare_kernel, dim3(1 + xt.blocks + wt0.blocks), dim3(256), 0, s, xt, wt0, dloss, target, M, V, b.top);
   TRY(hipGetLastError());
   if (!x_direct) {
@@ -1083,13 +1109,18 @@ namespace {
 bool whole(const float* q, int ld, int rows, int rows_p, int cols, int cols_p) {
   return rows == rows_p && cols == cols_p && al16(q) && ld % 4 == 0;
 }
-// An operand in whole tiles: where it stands, or copied to `room`.
-hipError_t whole_operand(const float*& q, int& ld, float* room, int rows, int cols, int rows_p, int cols_p, hipStream_t s) {
-  if (whole(q, ld, rows, rows_p, cols, cols_p)) return hipSuccess;
-  launch_kernel(pad_f32_kernel, row_grid(rows_p, cols_p), dim3(256), 0, s, room, q, rows, cols, ld, rows_p, cols_p);
+hipError_t padded_copy(const float*& q, int& ld, float* room, int rows, int cols, int rows_p, int cols_p, const int* target, int vocab,
+                       hipStream_t s) {
+  launch_kernel(pad_f32_kernel, row_grid(rows_p, cols_p), dim3(256), 0, s, room, q, rows, cols, ld, rows_p, cols_p, target, vocab,
+                (int)(al16(q) && ld % 4 == 0));
   q = room;
   ld = cols_p;
   return hipGetLastError();
+}
+// An operand in whole tiles: where it stands, or copied to `room`.
+hipError_t whole_operand(const float*& q, int& ld, float* room, int rows, int cols, int rows_p, int cols_p, hipStream_t s) {
+  if (whole(q, ld, rows, rows_p, cols, cols_p)) return hipSuccess;
+  return padded_copy(q, ld, room, rows, cols, rows_p, cols_p, nullptr, 0, s);
 }
 }  // namespace
 
@@ -1117,7 +1148,8 @@ hipError_t xent_backward_f32(int M, int V, int K, const float* X, int ldx, const
                              const int* target, const float* lse, const float* dloss, float* dX, int lddx, float* dW, int lddw,
                              float* db, void* ws, hipStream_t s) {
   const F32Plan f = plan_f32(static_cast<char*>(ws), M, V, K, true);
-  TRY(whole_operand(X, ldx, f.Xp, M, K, f.Mp, f.Kp, s));
+  // always copied: rows that do not count become zeros, as dW = g^T X needs them (zero times an infinity or NaN is NaN)
+  TRY(padded_copy(X, ldx, f.Xp, M, K, f.Mp, f.Kp, target, V, s));
   const bool dx_direct = f.splits == 1 && f.piece >= V && whole(dX, lddx, M, f.Mp, K, f.Kp);
   for (int v0 = 0; v0 < V; v0 += f.piece) {
     const int cols = std::min(f.piece, V - v0), cols_p = whole_tiles(cols);

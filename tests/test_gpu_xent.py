@@ -346,6 +346,33 @@ def test_infinite_and_nan_logits_stay_in_their_row(dtype):
     assert np.all(np.isfinite(loss[fine])) and np.all(np.isfinite(gX[fine]))
 
 
+@pytest.mark.parametrize("M,V,K", [(20, 300, 64), (33, 77, 50), (300, 700, 256), (256, 128, 128), (70, 1000, 1000)])
+@pytest.mark.parametrize("dtype", [capi.MI_BF16, capi.MI_F32], ids=["bf16", "f32"])
+def test_rows_that_do_not_count_may_hold_anything(dtype, M, V, K):
+    """What stands in padding rows leaves no trace in dW, db and the other rows of dX: bit for bit as with zeros there."""
+    dead = [0, 5, M // 2, M - 1]
+
+    def run(values):
+        def tweak(X, W, b, t, d):
+            t[dead] = [-100, V, -1, 2 ** 31 - 1]
+            X[dead] = values
+            d[dead] = values[:, 0]
+        with np.errstate(all="ignore"):
+            p = Problem(dtype, M, V, K, tweak=tweak, ignored=0.0)
+        p.forward()
+        p.make_outputs(dtype)
+        p.backward(use_wt=False)
+        capi.check(capi.lib().mi_stream_sync(None))
+        assert np.all(p.loss.get()[0][dead] == 0.0)
+        return p.gX.get(), p.gW.get(), p.gb.get(), np.delete(p.lse.get()[0], dead)
+    zero = run(np.zeros((4, K), np.float32))
+    rest = np.full((4, K), np.nan, np.float32)
+    rest[1] = np.inf
+    rest[2, ::2] = -np.inf
+    for a, b in zip(zero, run(rest)):
+        assert np.array_equal(a, b)
+
+
 @pytest.mark.parametrize("dtype", [capi.MI_BF16, capi.MI_F32], ids=["bf16", "f32"])
 def test_no_class_possible(dtype):
     def tweak(X, W, b, t, d):
