@@ -1106,8 +1106,9 @@ hipError_t xent_backward_bf16(int M, int V, int K, const u16* X, int ldx, const 
 }
 
 namespace {
+// Whether the fp32 GEMMs can read or write a matrix as whole tiles where it is (their byte offsets in a tile have 32 bits).
 bool whole(const float* q, int ld, int rows, int rows_p, int cols, int cols_p) {
-  return rows == rows_p && cols == cols_p && al16(q) && ld % 4 == 0;
+  return rows == rows_p && cols == cols_p && al16(q) && ld % 4 == 0 && ld <= TILE16_MAX_LD;
 }
 hipError_t padded_copy(const float*& q, int& ld, float* room, int rows, int cols, int rows_p, int cols_p, const int* target, int vocab,
                        hipStream_t s) {

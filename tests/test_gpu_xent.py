@@ -374,6 +374,43 @@ def test_rows_that_do_not_count_may_hold_anything(dtype, M, V, K):
 
 
 @pytest.mark.parametrize("dtype", [capi.MI_BF16, capi.MI_F32], ids=["bf16", "f32"])
+def test_rows_so_far_apart_that_a_tile_passes_32_bits(dtype):
+    """W and dW with rows of 9 M elements (128 of them span more than 2^32 bytes): the same bits as dense ones."""
+    M, V, K, ld = 128, 256, 64, 9 << 20
+    p = Problem(dtype, M, V, K)
+    p.forward()
+    p.make_outputs(dtype)
+    p.backward(use_wt=False)
+    capi.check(capi.lib().mi_stream_sync(None))
+    dense = [p.loss.get(), p.lse.get(), p.gX.get(), p.gW.get()]
+    size = np.dtype(p.dX_.dtype).itemsize
+    rows = p.dW_.get()
+
+    class Far:
+        def __init__(self):
+            self.buf, self.ld = capi.DeviceBuffer(((V - 1) * ld + K) * size), ld
+            self.ptr = self.buf.ptr
+
+        def get(self):
+            out = np.empty((V, K), rows.dtype)
+            for i in range(V):
+                capi.check(capi.lib().mi_memcpy_d2h(out[i].ctypes.data_as(ctypes.c_void_p), self.ptr + i * ld * size, K * size))
+            return out
+
+    p.dW_, p.gW = Far(), Far()
+    for i in range(V):
+        row = np.ascontiguousarray(rows[i])
+        capi.check(capi.lib().mi_memcpy_h2d(p.dW_.ptr + i * ld * size, row.ctypes.data_as(ctypes.c_void_p), K * size))
+    p.loss, p.lse = Strided(1, M, M, 0, np.float32), Strided(1, M, M, 0, np.float32)
+    p.gX = Strided(M, K, K, 0, p.dX_.dtype)
+    p.forward()
+    p.backward(use_wt=False)
+    capi.check(capi.lib().mi_stream_sync(None))
+    for a, b in zip(dense, [p.loss.get(), p.lse.get(), p.gX.get(), p.gW.get()]):
+        assert np.array_equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [capi.MI_BF16, capi.MI_F32], ids=["bf16", "f32"])
 def test_no_class_possible(dtype):
     def tweak(X, W, b, t, d):
         b[:] = -np.inf
