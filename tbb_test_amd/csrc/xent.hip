@@ -311,85 +311,106 @@ hipError_t tiles(const Tile16Shape& shape, float* part, const u16* A, int lda, c
   return launch_tile16<false, Epi>(product(A, lda, B, ldb, M, N, K), shape, part, e, s);
 }
 
-// ---- few rows against classes that the tiles cannot read in place ----------------------------------------
+// ---- few rows ----------------------------------------------------------------------------------------
 
 // Statistics as EpiStats leaves them, for at most 16 QB rows: W is read once, straight into registers in 16-byte pieces
-// that may start at any element (the direct loads into LDS cannot), 16 NB classes per wavefront, AHEAD K chunks of 32
-// requested ahead of those being multiplied; X (packed, zeros behind K) comes out of the caches.  Wavefronts join to
-// blocks of 64 classes.  4 x 30592 x 2956: 52 us, 3.5 TB/s of W, where copying W for the tiles, two more passes over it,
-// makes 164; 64 x 49165 x 3501, rows at any 2 bytes: 235 us instead of 422.  More rows want more classes per wavefront
-// (X is read once for each): 16 rows 52 us with 16 classes and 53 with 32, 32 rows of 50000 x 1002 55 and 46, 64 rows
-// 245 us with 32 and 235 with 64.
-constexpr int FEW_ROWS = 64;
+// that may start at any element (the direct loads into LDS cannot), 16 NB classes per wavefront, AHEAD K chunks (of 32
+// elements bf16, 16 fp32) of W and X requested ahead of those being multiplied; X (rows of whole pieces, zeros behind K)
+// comes out of the caches.  Wavefronts join to blocks of 64 classes.
+// For bf16 classes that the tiles cannot read in place, and for fp32, where tiles of 16 or 32 rows wait for memory:
+//   bf16  4 x 30592 x 2956: 47 us, 3.9 TB/s of W, where copying W for the tiles, two more passes over it, makes 164;
+//         64 x 49165 x 3501, rows at any 2 bytes: 192 us instead of 422
+//   fp32  1 x 32000 x 1024: 32 us, 4.1 TB/s of W, instead of 50; 1 x 44992 x 1944: 82 us, with its copy 337
+// More rows want more classes per wavefront (X is read once for each) where that leaves enough wavefronts: 32 rows of
+// 50000 x 1002 bf16 52 us with 16 classes and 42 with 32, of 6464 x 1501 30 and 44 us; 64 rows of 49165 x 3501 221 us
+// with 32 and 192 with 64.  Few classes leave each wavefront alone with its whole K: 32 rows of 1500 x 1501 bf16 take 32 us
+// and through copies and tiles 21 us, of 6464 x 1501 30 and 34 us.
+template <class T>
+constexpr int FEW_ROWS = sizeof(T) == 2 ? 64 : 32;
+template <class T>
 struct FewRows {
-  const u16* X;  // [M][Kp]
-  const u16* W;  // [V][ldw]
-  int M, V, K, Kp, ldw;
+  const T* X;  // [M][ldx], rows of whole 16-byte pieces, zeros behind K up to whole chunks
+  const T* W;  // [V][ldw]
+  int M, V, K, ldx, ldw;
   const float* bias;
   const int* target;
   float* zt;
   float2* part;
 };
-template <int QB, int NB, int AHEAD>
-__global__ __launch_bounds__(256) void xent_few_rows_kernel(FewRows p) {
-  struct __attribute__((packed, aligned(2))) Piece {
+template <class T, int QB, int NB, int AHEAD>
+__global__ __launch_bounds__(256) void xent_few_rows_kernel(FewRows<T> p) {
+  constexpr int EACH = 16 / sizeof(T), CHUNK = 4 * EACH;  // elements of a piece, and of the four lanes of a class
+  struct __attribute__((packed, aligned(sizeof(T)))) Piece {
     u32x4 v;
   };
   __shared__ float2 red[4][16 * QB];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, q = lane >> 4;
   const int c0 = ((int)blockIdx.x * 4 + wave) * 16 * NB;
-  const u16* w[NB];
-  const u16* x[QB];
+  const T* w[NB];
+  const T* x[QB];
 #pragma unroll
-  for (int b = 0; b < NB; ++b) w[b] = p.W + (size_t)min(c0 + 16 * b + l16, p.V - 1) * p.ldw + 8 * q;
+  for (int b = 0; b < NB; ++b) w[b] = p.W + (size_t)min(c0 + 16 * b + l16, p.V - 1) * p.ldw + EACH * q;
 #pragma unroll
-  for (int j = 0; j < QB; ++j) x[j] = p.X + (size_t)min(16 * j + l16, p.M - 1) * p.Kp + 8 * q;
+  for (int j = 0; j < QB; ++j) x[j] = p.X + (size_t)min(16 * j + l16, p.M - 1) * p.ldx + EACH * q;
   f32x4 acc[QB][NB];
 #pragma unroll
   for (int j = 0; j < QB; ++j)
 #pragma unroll
     for (int b = 0; b < NB; ++b) acc[j][b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  auto multiply = [&](const u32x4(&fw)[NB], int t) __attribute__((always_inline)) {
+  struct Chunk {
+    u32x4 x[QB], w[NB];
+  };
+  auto multiply = [&](const Chunk& f) __attribute__((always_inline)) {
 #pragma unroll
-    for (int j = 0; j < QB; ++j) {
-      const u32x4 fx = *reinterpret_cast<const u32x4*>(x[j] + 32 * t);
+    for (int j = 0; j < QB; ++j)
 #pragma unroll
       for (int b = 0; b < NB; ++b)
-        acc[j][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, fw[b]), __builtin_bit_cast(bf16x8, fx), acc[j][b], 0, 0, 0);
-    }
+        if constexpr (sizeof(T) == 2)
+          acc[j][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, f.w[b]), __builtin_bit_cast(bf16x8, f.x[j]), acc[j][b], 0, 0, 0);
+        else  // one element of each lane's four at a time: which four K elements share a product is the same on both sides
+#pragma unroll
+          for (int u = 0; u < 4; ++u)
+            acc[j][b] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(f.w[b][u]), __uint_as_float(f.x[j][u]), acc[j][b], 0, 0, 0);
   };
-  const int whole = p.K / 32;
-  u32x4 now[AHEAD][NB], next[AHEAD][NB];
-  auto request = [&](u32x4(&f)[AHEAD][NB], int t) __attribute__((always_inline)) {
+  // X is requested as far ahead as W: loads return in order, so one for now would wait for the W of later
+  const int whole = p.K / CHUNK;
+  Chunk now[AHEAD], next[AHEAD];
+  auto request = [&](Chunk(&f)[AHEAD], int t) __attribute__((always_inline)) {
 #pragma unroll
-    for (int u = 0; u < AHEAD; ++u)
+    for (int u = 0; u < AHEAD; ++u) {
 #pragma unroll
-      for (int b = 0; b < NB; ++b) f[u][b] = reinterpret_cast<const Piece*>(w[b] + 32 * (t + u))->v;
+      for (int j = 0; j < QB; ++j) f[u].x[j] = *reinterpret_cast<const u32x4*>(x[j] + CHUNK * (t + u));
+#pragma unroll
+      for (int b = 0; b < NB; ++b) f[u].w[b] = reinterpret_cast<const Piece*>(w[b] + CHUNK * (t + u))->v;
+    }
   };
   int t = 0;
   if (t + AHEAD <= whole) request(now, t);
   for (; t + AHEAD <= whole; t += AHEAD) {
     if (t + 2 * AHEAD <= whole) request(next, t + AHEAD);
 #pragma unroll
-    for (int u = 0; u < AHEAD; ++u) multiply(now[u], t + u);
+    for (int u = 0; u < AHEAD; ++u) multiply(now[u]);
 #pragma unroll
-    for (int u = 0; u < AHEAD; ++u)
-#pragma unroll
-      for (int b = 0; b < NB; ++b) now[u][b] = next[u][b];
+    for (int u = 0; u < AHEAD; ++u) now[u] = next[u];
   }
-  for (; 32 * t < p.K; ++t) {  // the chunks left over, the last of them element by element where it is cut
-    u32x4 fw[NB];
-    const int there = p.K - 32 * t - 8 * q;  // elements of the lane's eight that are there
+  for (; CHUNK * t < p.K; ++t) {  // the chunks left over, the last of them element by element where it is cut
+    Chunk f;
+#pragma unroll
+    for (int j = 0; j < QB; ++j) f.x[j] = *reinterpret_cast<const u32x4*>(x[j] + CHUNK * t);
+    const int there = p.K - CHUNK * t - EACH * q;  // elements of the lane's piece that are there
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-      fw[b] = u32x4{0u, 0u, 0u, 0u};
-      if (there >= 8) fw[b] = reinterpret_cast<const Piece*>(w[b] + 32 * t)->v;
+      f.w[b] = u32x4{0u, 0u, 0u, 0u};
+      if (there >= EACH) f.w[b] = reinterpret_cast<const Piece*>(w[b] + CHUNK * t)->v;
       else
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (i < there) fw[b][i >> 1] |= (unsigned)w[b][32 * t + i] << (16 * (i & 1));
+        for (int i = 0; i < EACH; ++i)
+          if (i < there) {
+            if constexpr (sizeof(T) == 2) f.w[b][i >> 1] |= (unsigned)w[b][CHUNK * t + i] << (16 * (i & 1));
+            else f.w[b][i] = __float_as_uint(w[b][CHUNK * t + i]);
+          }
     }
-    multiply(fw, t);
+    multiply(f);
   }
   // a lane holds classes c0 + 16 b + 4 q + r of row 16 j + l16
 #pragma unroll
@@ -880,8 +901,10 @@ BackwardPlan plan_backward(char* base, int M, int V, int K) {
 // fp32: the framework's fp32 GEMMs are fast on whole tiles of aligned operands only, so everything is padded to
 // them; what already is whole is used where it stands.
 struct F32Plan {
-  int Mp, Kp, piece;
-  int splits;       // of the classes, for dX
+  int Mp, Kp;
+  int most, piece;  // classes at a time: at most, and the largest piece in whole tiles
+  bool backward;
+  int splits;       // of the classes, for dX: at most
   float *Xp, *Wp, *Z, *zt, *x_part, *w_part;
   float2* part;
   size_t bytes;
@@ -889,34 +912,54 @@ struct F32Plan {
 int whole_tiles(int n) { return (int)(n >= 128 ? up(n, 128) : up(n, 32)); }
 // K: a dimension of dX and dW too, whose tiles are 64 wide at least; the forward products only need whole K steps.
 int whole_k(int K, bool backward) { return !backward ? (int)up(K, 32) : K % 64 == 0 ? K : whole_tiles(K); }
+// Which fp32 forward calls take the kernel for few rows: with rows of whole 256 elements the tiles of 32 rows go through the
+// LDS and are faster (32 x 50048 x 1536: 98 us, few rows 110), and so are those of few classes that need no copy (16 x 1500
+// x 1536: 23 us, few rows 28).
+bool few_rows_f32(int M, int V, int K) {
+  return M <= FEW_ROWS<float> && (V >= 4096 ? M <= 16 || K % 256 != 0 : M <= 16 && K % 32 != 0);
+}
+// How many of the `left` classes the next piece takes.  Backward, the products with a row per class run on 128 x 128 tiles,
+// one per CU at a time (from 128 rows on): whole rounds of the 256 CUs first, the classes left over as a piece of their own
+// on smaller tiles (1024 x 10007 x 1024 in one piece 586 us, in pieces of 8192 and 1815 classes 521).  Where what
+// does not make whole tiles would mean copying much, the classes that do are read in place and the others are a piece
+// of their own: forward from 8 M elements on (two more passes over them take 13 us, a piece more about as long), backward
+// from 32 M (four passes, 110 us; a piece more is six launches, 90 us); thousands of them, so that dX's sum can be
+// dealt out.
+int next_piece(const F32Plan& f, int left, int K) {
+  const int n = std::min(left, f.most), across = f.Mp / 128, round = across >= 256 ? 128 : across > 0 ? 256 / across * 128 : 0;
+  if (f.backward && f.Mp % 128 == 0 && n > round) return n / round * round;
+  const int unit = f.backward && n > 16384 ? 1024 : 128;
+  const bool large = (size_t)n * K >= (f.backward ? (size_t)1 << 25 : (size_t)1 << 23);
+  return n % 128 != 0 && n > 128 && large && K == f.Kp ? n / unit * unit : n;
+}
 F32Plan plan_f32(char* base, int M, int V, int K, bool backward) {
   F32Plan f{};
   Carver c{base};
   f.Mp = whole_tiles(M);
   f.Kp = whole_k(K, backward);
   // a piece of products and a piece of W take at most 1 GB each
-  const size_t most = std::max<size_t>(((size_t)1 << 28) / std::max(f.Mp, f.Kp) / 128 * 128, 128);
-  f.piece = (int)std::min<size_t>(whole_tiles(V), most);
-  // Where W is large (8 M elements: two more passes over it take 13 us, a piece more about as long), the classes that make
-  // whole tiles are read in place and those left over are a piece of their own, copied to whole tiles.
-  if (f.piece >= V && V % 128 != 0 && V > 128 && (size_t)V * K >= ((size_t)1 << 23)) f.piece = V / 128 * 128;
+  f.most = (int)std::max<size_t>(((size_t)1 << 28) / std::max(f.Mp, f.Kp) / 128 * 128, 128);
+  f.backward = backward;
+  for (int v0 = 0, n; v0 < V; v0 += n) {
+    n = next_piece(f, V - v0, K);
+    f.piece = std::max(f.piece, whole_tiles(n));
+  }
   f.Xp = c.take<float>((size_t)f.Mp * f.Kp);
-  f.Wp = c.take<float>((size_t)f.piece * f.Kp);
-  f.Z = c.take<float>((size_t)f.Mp * f.piece);
+  const bool few = !backward && few_rows_f32(M, V, K);
+  if (!few) {
+    f.Wp = c.take<float>((size_t)f.piece * f.Kp);
+    f.Z = c.take<float>((size_t)f.Mp * f.piece);
+  }
   if (backward) {
-    // The products with a row per class run on 128 x 128 tiles, one per CU at a time: whole rounds of the 256 CUs
-    // first, the classes left over as a piece of their own (on smaller tiles, and only they are copied to
-    // whole tiles): 1024 x 10007 x 1024 in one piece 586 us, in pieces of 8192 and 1815 classes 521.
-    const int across = (int)up(f.Mp, 128) / 128, round = across >= 256 ? 128 : (256 / across) * 128;
-    if (V > round && f.piece >= V / 128 * 128) f.piece = V / round * round;
+    // as many parts of dX's sum as make a round of its 128 x 128 tiles
     const size_t tiles = up(f.Mp, 128) / 128 * (up(f.Kp, 128) / 128);
-    f.splits = tiles > 128 ? 1 : tiles > 64 ? 2 : 4;
-    while (f.piece % (f.splits * 32) != 0) f.splits /= 2;
+    f.splits = 1;
+    while (f.splits < 32 && 2 * f.splits * tiles <= 256) f.splits *= 2;
     f.x_part = c.take<float>((size_t)f.splits * f.Mp * f.Kp);
     f.w_part = c.take<float>((size_t)f.piece * f.Kp);
   } else {
     f.zt = c.take<float>(M);
-    f.part = c.take<float2>(M);
+    f.part = c.take<float2>((size_t)M * (few ? up(V, 64) / 64 : 1));
   }
   f.bytes = c.used;
   return f;
@@ -961,21 +1004,39 @@ size_t xent_backward_bytes(bool bf16, int M, int V, int K) {
   return bf16 ? plan_backward(nullptr, M, V, K).bytes : plan_f32(nullptr, M, V, K, true).bytes;
 }
 
+template <class T>
+static hipError_t launch_few_rows(const FewRows<T>& p, hipStream_t s) {
+  auto go = [&](auto kern, int nb) { launch_kernel(kern, dim3((p.V + 64 * nb - 1) / (64 * nb)), dim3(256), 0, s, p); };
+  const bool many = p.V >= 1 << 15;
+  if (p.M <= 16) go(xent_few_rows_kernel<T, 1, 1, 4>, 1);
+  else if (p.M <= 32 && many) go(xent_few_rows_kernel<T, 2, 2, 2>, 2);
+  else if (p.M <= 32) go(xent_few_rows_kernel<T, 2, 1, 4>, 1);
+  else if constexpr (FEW_ROWS<T> > 32) {
+    if (many) go(xent_few_rows_kernel<T, 4, 4, 2>, 4);
+    else go(xent_few_rows_kernel<T, 4, 1, 2>, 1);
+  }
+  return hipGetLastError();
+}
+static hipError_t launch_fold(const float2* part, int blocks, int M, int V, const int* target, const float* zt, float* loss, float* lse,
+                              hipStream_t s) {
+  auto fold = [&](auto kern, int rows) {
+    launch_kernel(kern, dim3((M + rows - 1) / rows), dim3(256), 0, s, part, blocks, M, V, target, zt, loss, lse);
+    return hipGetLastError();
+  };
+  // whole 128-byte lines of the statistics per workgroup once there are rows for every CU
+  return M <= 64 ? fold(xent_fold_kernel<1>, 1) : M <= 1024 ? fold(xent_fold_kernel<4>, 4) : fold(xent_fold_kernel<16>, 16);
+}
+
 static hipError_t forward_rows(const ForwardPlan& f, int M, int V, int K, const u16* X, int ldx, const u16* W, int ldw,
                                const float* bias, const int* target, float* loss, float* lse, hipStream_t s) {
-  const bool w_direct = direct(W, ldw, K), few = !w_direct && M <= FEW_ROWS;
+  const bool w_direct = direct(W, ldw, K), few = !w_direct && M <= FEW_ROWS<u16> && V >= (M <= 32 ? 4096 : 8192);
   if (few || !direct(X, ldx, K)) {
     TRY(pack_rows(f.Xp, X, M, K, ldx, f.Kp, s));
     X = f.Xp;
     ldx = f.Kp;
   }
   if (few) {
-    const FewRows p{X, W, M, V, K, f.Kp, ldw, bias, target, f.zt, f.part};
-    auto go = [&](auto kern, int nb) { launch_kernel(kern, dim3((V + 64 * nb - 1) / (64 * nb)), dim3(256), 0, s, p); };
-    if (M <= 16) go(xent_few_rows_kernel<1, 1, 8>, 1);
-    else if (M <= 32) go(xent_few_rows_kernel<2, 2, 4>, 2);
-    else go(xent_few_rows_kernel<4, 4, 2>, 4);
-    TRY(hipGetLastError());
+    TRY(launch_few_rows<u16>(FewRows<u16>{X, W, M, V, K, f.Kp, ldw, bias, target, f.zt, f.part}, s));
   }
   const int per = w_direct ? V : f.pack_cols;
   for (int v0 = few ? V : 0; v0 < V; v0 += per) {
@@ -993,14 +1054,7 @@ static hipError_t forward_rows(const ForwardPlan& f, int M, int V, int K, const 
       c0 += n;
     }
   }
-  const int blocks = (int)(up(V, 64) / 64);
-  auto fold = [&](auto kern, int rows) {
-    launch_kernel(kern, dim3((M + rows - 1) / rows), dim3(256), 0, s, (const float2*)f.part, blocks, M, V, target, (const float*)f.zt,
-                  loss, lse);
-    return hipGetLastError();
-  };
-  // whole 128-byte lines of the statistics per workgroup once there are rows for every CU
-  return M <= 64 ? fold(xent_fold_kernel<1>, 1) : M <= 1024 ? fold(xent_fold_kernel<4>, 4) : fold(xent_fold_kernel<16>, 16);
+  return launch_fold(f.part, (int)(up(V, 64) / 64), M, V, target, f.zt, loss, lse, s);
 }
 
 hipError_t xent_forward_bf16(int M, int V, int K, const u16* X, int ldx, const u16* W, int ldw, const float* bias,
@@ -1128,9 +1182,15 @@ hipError_t whole_operand(const float*& q, int& ld, float* room, int rows, int co
 hipError_t xent_forward_f32(int M, int V, int K, const float* X, int ldx, const float* W, int ldw, const float* bias,
                             const int* target, float* loss, float* lse, void* ws, hipStream_t s) {
   const F32Plan f = plan_f32(static_cast<char*>(ws), M, V, K, false);
+  if (few_rows_f32(M, V, K)) {
+    if (!whole(X, ldx, M, M, K, f.Kp)) TRY(padded_copy(X, ldx, f.Xp, M, K, M, f.Kp, nullptr, 0, s));
+    TRY(launch_few_rows<float>(FewRows<float>{X, W, M, V, K, ldx, ldw, bias, target, f.zt, f.part}, s));
+    return launch_fold(f.part, (int)(up(V, 64) / 64), M, V, target, f.zt, loss, lse, s);
+  }
   TRY(whole_operand(X, ldx, f.Xp, M, K, f.Mp, f.Kp, s));
-  for (int v0 = 0; v0 < V; v0 += f.piece) {
-    const int cols = std::min(f.piece, V - v0), cols_p = whole_tiles(cols);
+  for (int v0 = 0, cols; v0 < V; v0 += cols) {
+    cols = next_piece(f, V - v0, K);
+    const int cols_p = whole_tiles(cols);
     const float* w = W + (size_t)v0 * ldw;
     int ld_w = ldw;
     TRY(whole_operand(w, ld_w, f.Wp, cols, K, cols_p, f.Kp, s));
@@ -1151,9 +1211,10 @@ hipError_t xent_backward_f32(int M, int V, int K, const float* X, int ldx, const
   const F32Plan f = plan_f32(static_cast<char*>(ws), M, V, K, true);
   // always copied: rows that do not count become zeros, as dW = g^T X needs them (zero times an infinity or NaN is NaN)
   TRY(padded_copy(X, ldx, f.Xp, M, K, f.Mp, f.Kp, target, V, s));
-  const bool dx_direct = f.splits == 1 && f.piece >= V && whole(dX, lddx, M, f.Mp, K, f.Kp);
-  for (int v0 = 0; v0 < V; v0 += f.piece) {
-    const int cols = std::min(f.piece, V - v0), cols_p = whole_tiles(cols);
+  const bool dx_direct = f.splits == 1 && next_piece(f, V, K) == V && whole(dX, lddx, M, f.Mp, K, f.Kp);
+  for (int v0 = 0, cols; v0 < V; v0 += cols) {
+    cols = next_piece(f, V - v0, K);
+    const int cols_p = whole_tiles(cols);
     const float* w = W + (size_t)v0 * ldw;
     int ld_w = ldw;
     TRY(whole_operand(w, ld_w, f.Wp, cols, K, cols_p, f.Kp, s));
@@ -1162,7 +1223,8 @@ hipError_t xent_backward_f32(int M, int V, int K, const float* X, int ldx, const
                   bias ? bias + v0 : nullptr, target, lse, dloss, db ? db + v0 : nullptr,
                   (int)(al16(target) && al16(lse) && al16(dloss)));
     TRY(hipGetLastError());
-    const int splits = cols_p % (f.splits * 32) == 0 ? f.splits : 1;
+    int splits = f.splits;
+    while (cols_p % (splits * 32) != 0 || (splits > 1 && cols_p / splits < 256)) splits /= 2;
     float* dx = dx_direct ? dX : f.x_part;
     TRY(sgemm_tn(splits, f.Mp, f.Kp, cols_p / splits, f.Z, f.Mp, w, ld_w, dx, dx_direct ? lddx : f.Kp, (long long)f.Mp * f.Kp,
                  nullptr, 0, s, 0));

@@ -197,6 +197,23 @@ def test_few_rows_against_unaligned_classes(M, V, K, pad, offset):
     check_forward(p)
 
 
+@pytest.mark.parametrize("M,V,K", [(1, 4100, 37), (9, 5000, 300), (16, 4333, 31), (17, 4700, 515), (32, 33000, 70), (33, 8200, 1001),
+                                   (64, 9000, 260), (64, 33000, 90)])
+@pytest.mark.parametrize("pad,offset", [(0, 0), (1, 1)])
+@pytest.mark.parametrize("dtype", [capi.MI_BF16, capi.MI_F32], ids=["bf16", "f32"])
+def test_few_rows_against_many_classes(dtype, M, V, K, pad, offset):
+    p = Problem(dtype, M, V, K, pad=pad, offset=offset)
+    check_forward(p)
+
+
+# pieces of whole rounds, of whole tiles and what is left over; parts of dX's sum in each
+@pytest.mark.parametrize("M,V,K", [(50, 20500, 1664), (200, 20100, 512), (130, 33000, 64), (256, 17000, 1999), (5, 9000, 3776)])
+def test_fp32_gradients_in_pieces(M, V, K):
+    p = Problem(capi.MI_F32, M, V, K)
+    check_forward(p)
+    check_backward(p, capi.MI_F32)
+
+
 def test_fp32_classes_that_are_no_whole_tiles():
     p = Problem(capi.MI_F32, 40, 66000, 128)  # most read in place, 80 left over
     check_forward(p)
