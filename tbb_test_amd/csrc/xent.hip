@@ -607,27 +607,34 @@ __global__ __launch_bounds__(256) void xent_transpose_kernel(Transposition w) {
   transpose_tile(w, blockIdx.x, tile);
 }
 
-// C[row][col] = sum over slabs, in slab order, of part[slab][row][col], on top of what C holds where `add`.  One
-// element per thread, 256 of a row per workgroup.
+// C[row][col] = sum over slabs, in slab order, of part[slab][row][col], on top of what C holds where `add`.  A
+// wavefront takes 512 elements of a row, in 16-byte pieces (part's rows are whole ones, C's may start at any element).
 __global__ __launch_bounds__(256) void fold_slabs_kernel(float* __restrict__ C, int ldc, const float* __restrict__ part, int ldp,
                                                          long long slab, int slabs, int rows, int cols, int add) {
-  const int c = blockIdx.x * 256 + threadIdx.x;
-  if (c >= cols) return;
-  for (int r = blockIdx.y; r < rows; r += gridDim.y) {
-    const float* src = part + (size_t)r * ldp + c;
-    float v = add ? C[(size_t)r * ldc + c] : 0.0f;
+  struct __attribute__((packed, aligned(4))) Piece {
+    f32x4 v;
+  };
+  for (int r = blockIdx.y * 4 + (threadIdx.x >> 6); r < rows; r += gridDim.y * 4)
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int c = blockIdx.x * 512 + 256 * k + 4 * (threadIdx.x & 63);
+      if (c >= cols) break;
+      const float* src = part + (size_t)r * ldp + c;
+      float* dst = C + (size_t)r * ldc + c;
+      const bool whole = c + 4 <= cols;
+      f32x4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+      if (add && whole) v = reinterpret_cast<const Piece*>(dst)->v;
+      else if (add)
+        for (int i = 0; i < 4; ++i)
+          if (c + i < cols) v[i] = dst[i];
 #pragma unroll 4
-    for (int n = 0; n < slabs; ++n) v += src[(size_t)n * slab];
-    C[(size_t)r * ldc + c] = v;
-  }
+      for (int n = 0; n < slabs; ++n) v += *reinterpret_cast<const f32x4*>(src + (size_t)n * slab);
+      if (whole) reinterpret_cast<Piece*>(dst)->v = v;
+      else
+        for (int i = 0; i < 4; ++i)
+          if (c + i < cols) dst[i] = v[i];
+    }
 }
-hipError_t fold_slabs(float* C, int ldc, const float* part, int ldp, long long slab, int slabs, int rows, int cols, bool add,
-                      hipStream_t s) {
-  launch_kernel(fold_slabs_kernel, dim3((cols + 255) / 256, std::min(rows, 65535)), dim3(256), 0, s, C, ldc, part, ldp, slab, slabs,
-                rows, cols, (int)add);
-  return hipGetLastError();
-}
-
 // out[c] = factor * sum over lines of part[line][c].  64 columns per workgroup, four groups of lines added up in order.
 struct ColumnFold {
   float* out;
@@ -809,6 +816,11 @@ inline size_t up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 inline bool al16(const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15) == 0; }
 // Workgroups of four wavefronts, 512 columns of a row each.
 inline dim3 row_grid(int rows, int cols) { return dim3((cols + 511) / 512, std::min((rows + 3) / 4, 16384)); }
+hipError_t fold_slabs(float* C, int ldc, const float* part, int ldp, long long slab, int slabs, int rows, int cols, bool add,
+                      hipStream_t s) {
+  launch_kernel(fold_slabs_kernel, row_grid(rows, cols), dim3(256), 0, s, C, ldc, part, ldp, slab, slabs, rows, cols, (int)add);
+  return hipGetLastError();
+}
 
 // Hands out 256-byte aligned parts of a workspace (or only adds them up, base = null).
 struct Carver {
