@@ -968,7 +968,9 @@ F32Plan plan_f32(char* base, int M, int V, int K, bool backward) {
     f.splits = 1;
     while (f.splits < 32 && 2 * f.splits * tiles <= 256) f.splits *= 2;
     f.x_part = c.take<float>((size_t)f.splits * f.Mp * f.Kp);
-    f.w_part = c.take<float>((size_t)f.piece * f.Kp);
+    // Where dW has no whole tiles: in whole tiles here first, or, with a sum over few rows, straight on the slower ragged
+    // tiles (64 x 44992 x 1944 700 and 595 us, 300 x 20000 x 1001 538 and 549).
+    f.w_part = f.Mp > 128 ? c.take<float>((size_t)f.piece * f.Kp) : nullptr;
   } else {
     f.zt = c.take<float>(M);
     f.part = c.take<float2>((size_t)M * (few ? up(V, 64) / 64 : 1));
@@ -1244,9 +1246,12 @@ hipError_t xent_backward_f32(int M, int V, int K, const float* X, int ldx, const
       TRY(fold_slabs(dX, lddx, f.x_part, f.Kp, (long long)f.Mp * f.Kp, splits, M, K, v0 > 0, s));
     }
     float* dw = dW + (size_t)v0 * lddw;
-    const bool dw_direct = whole(dw, lddw, cols, cols_p, K, f.Kp);
-    TRY(sgemm_nn(cols_p, f.Kp, f.Mp, f.Z, f.Mp, X, ldx, dw_direct ? dw : f.w_part, dw_direct ? lddw : f.Kp, nullptr, 0, s, 0));
-    if (!dw_direct) {
+    if (whole(dw, lddw, cols, cols_p, K, f.Kp)) {
+      TRY(sgemm_nn(cols_p, f.Kp, f.Mp, f.Z, f.Mp, X, ldx, dw, lddw, nullptr, 0, s, 0));
+    } else if (f.w_part == nullptr) {
+      TRY(sgemm_nn(cols, K, f.Mp, f.Z, f.Mp, X, ldx, dw, lddw, nullptr, 0, s, 0));
+    } else {
+      TRY(sgemm_nn(cols_p, f.Kp, f.Mp, f.Z, f.Mp, X, ldx, f.w_part, f.Kp, nullptr, 0, s, 0));
       TRY(fold_slabs(dw, lddw, f.w_part, f.Kp, 0, 1, cols, K, false, s));
     }
   }
