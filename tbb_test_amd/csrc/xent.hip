@@ -497,17 +497,19 @@ __global__ __launch_bounds__(256) void xent_fold_kernel(const float2* __restrict
 }
 
 // dst[rows][ldd] = src[rows][cols], zeros up to ldd (a multiple of 64).  A wavefront copies 512 elements of a row, eight
-// per lane; pairs: rows of src start at multiples of 4 bytes.
+// per lane, in one load that may start at any element.
 __global__ __launch_bounds__(256) void pack_rows_kernel(u16* __restrict__ dst, const u16* __restrict__ src, int rows, int cols,
-                                                        int ld, int ldd, int pairs) {
+                                                        int ld, int ldd) {
+  struct __attribute__((packed, aligned(2))) Piece {
+    u32x4 v;
+  };
   const int c = blockIdx.x * 512 + (threadIdx.x & 63) * 8;
   if (c >= ldd) return;
   for (int r = blockIdx.y * 4 + (threadIdx.x >> 6); r < rows; r += gridDim.y * 4) {
     const u16* from = src + (size_t)r * ld + c;
     u32x4 v = {0u, 0u, 0u, 0u};
-    if (pairs && c + 8 <= cols) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] = reinterpret_cast<const unsigned*>(from)[k];
+    if (c + 8 <= cols) {
+      v = reinterpret_cast<const Piece*>(from)->v;
     } else {
 #pragma unroll
       for (int k = 0; k < 8; ++k)
@@ -912,6 +914,8 @@ BackwardPlan plan_backward(char* base, int M, int V, int K) {
 
 // fp32: the framework's fp32 GEMMs are fast on whole tiles of aligned operands only, so everything is padded to
 // them; what already is whole is used where it stands.
+// Backward, 129 to 192 and 257 to 320 rows are padded to whole tiles of 64 only: those are a fifth slower but a quarter or
+// a sixth fewer (162 x 80192 x 768 890 and 733 us, 300 x 5000 x 700 126 and 111 us; 400 x 20000 x 1024 528 and 582).
 struct F32Plan {
   int Mp, Kp;
   int most, piece;  // classes at a time: at most, and the largest piece in whole tiles
@@ -935,12 +939,15 @@ bool few_rows_f32(int M, int V, int K) {
 // on smaller tiles (1024 x 10007 x 1024 in one piece 586 us, in pieces of 8192 and 1815 classes 521).  Where what
 // does not make whole tiles would mean copying much, the classes that do are read in place and the others are a piece
 // of their own: forward from 8 M elements on (two more passes over them take 13 us, a piece more about as long), backward
-// from 32 M (four passes, 110 us; a piece more is six launches, 90 us); thousands of them, so that dX's sum can be
-// dealt out.
+// from 32 M (four passes, 110 us; a piece more is six launches, 90 us).  Pieces are multiples of what dX's sum is dealt
+// to where they can be.
 int next_piece(const F32Plan& f, int left, int K) {
-  const int n = std::min(left, f.most), across = f.Mp / 128, round = across >= 256 ? 128 : across > 0 ? 256 / across * 128 : 0;
-  if (f.backward && f.Mp % 128 == 0 && n > round) return n / round * round;
-  const int unit = f.backward && n > 16384 ? 1024 : 128;
+  const int n = std::min(left, f.most), across = f.Mp / 128, deal = 128 * f.splits;  // (f.splits: 0 forward)
+  if (f.backward && f.Mp % 128 == 0) {
+    const int most = across >= 256 ? 128 : 256 / across * 128, round = most >= deal ? most / deal * deal : most;
+    if (n > round) return n / round * round;
+  }
+  const int unit = f.backward && n > 16384 ? std::min(deal, 1024) : 128;
   const bool large = (size_t)n * K >= (f.backward ? (size_t)1 << 25 : (size_t)1 << 23);
   return n % 128 != 0 && n > 128 && large && K == f.Kp ? n / unit * unit : n;
 }
@@ -952,6 +959,12 @@ F32Plan plan_f32(char* base, int M, int V, int K, bool backward) {
   // a piece of products and a piece of W take at most 1 GB each
   f.most = (int)std::max<size_t>(((size_t)1 << 28) / std::max(f.Mp, f.Kp) / 128 * 128, 128);
   f.backward = backward;
+  if (backward) {
+    if (M > 128 && M <= 320) f.Mp = (int)up(M, 64);
+    // as many parts of dX's sum as make a round of its 128 x 128 tiles, or four of 64 x 64
+    const size_t tiles = up(f.Mp, 128) / 128 * (up(f.Kp, 128) / 128), places = f.Mp % 128 == 0 ? 256 : 512;
+    f.splits = (int)std::min<size_t>(std::max<size_t>(places / tiles, 1), 32);
+  }
   for (int v0 = 0, n; v0 < V; v0 += n) {
     n = next_piece(f, V - v0, K);
     f.piece = std::max(f.piece, whole_tiles(n));
@@ -963,10 +976,6 @@ F32Plan plan_f32(char* base, int M, int V, int K, bool backward) {
     f.Z = c.take<float>((size_t)f.Mp * f.piece);
   }
   if (backward) {
-    // as many parts of dX's sum as make a round of its 128 x 128 tiles
-    const size_t tiles = up(f.Mp, 128) / 128 * (up(f.Kp, 128) / 128);
-    f.splits = 1;
-    while (f.splits < 32 && 2 * f.splits * tiles <= 256) f.splits *= 2;
     f.x_part = c.take<float>((size_t)f.splits * f.Mp * f.Kp);
     // Where dW has no whole tiles: in whole tiles here first, or, with a sum over few rows, straight on the slower ragged
     // tiles (64 x 44992 x 1944 700 and 595 us, 300 x 20000 x 1001 538 and 549).
@@ -989,8 +998,7 @@ F32Plan plan_f32(char* base, int M, int V, int K, bool backward) {
 bool direct(const u16* q, int ld, int K) { return al16(q) && ld % 8 == 0 && ld <= TILE16_MAX_LD && K % 64 == 0; }
 
 hipError_t pack_rows(u16* dst, const u16* src, int rows, int cols, int ld, int ldd, hipStream_t s) {
-  launch_kernel(pack_rows_kernel, row_grid(rows, ldd), dim3(256), 0, s, dst, src, rows, cols, ld, ldd,
-                (int)(reinterpret_cast<uintptr_t>(src) % 4 == 0 && ld % 2 == 0));
+  launch_kernel(pack_rows_kernel, row_grid(rows, ldd), dim3(256), 0, s, dst, src, rows, cols, ld, ldd);
   return hipGetLastError();
 }
 Transposition transposition(u16* dst, const u16* src, int rows, int cols, int ld, int ldd) {
@@ -1238,7 +1246,7 @@ hipError_t xent_backward_f32(int M, int V, int K, const float* X, int ldx, const
                   (int)(al16(target) && al16(lse) && al16(dloss)));
     TRY(hipGetLastError());
     int splits = f.splits;
-    while (cols_p % (splits * 32) != 0 || (splits > 1 && cols_p / splits < 256)) splits /= 2;
+    while (splits > 1 && (cols_p % (splits * 32) != 0 || cols_p / splits < 256)) --splits;
     float* dx = dx_direct ? dX : f.x_part;
     TRY(sgemm_tn(splits, f.Mp, f.Kp, cols_p / splits, f.Z, f.Mp, w, ld_w, dx, dx_direct ? lddx : f.Kp, (long long)f.Mp * f.Kp,
                  nullptr, 0, s, 0));
