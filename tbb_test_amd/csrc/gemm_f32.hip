@@ -1403,6 +1403,16 @@ hipError_t sgemm_nn(int M, int N, int K, const float* A, int lda, const float* B
   return dispatch<true, false, EPI_NONE>(p, 1, s, variant);
 }
 
+hipError_t sgemm_nn_parts(int parts, int M, int N, int K, const float* A, int lda, const float* B, int ldb, float* C,
+                          int ldc, long long strideC, hipStream_t s) {
+  GemmArgs p{};
+  p.M = M; p.N = N; p.K = K; p.A = A; p.B = B; p.C = C; p.lda = lda; p.ldb = ldb; p.ldc = ldc;
+  p.batchA = K;
+  p.batchB = (long long)K * ldb;
+  p.batchC = strideC;
+  return dispatch<true, false, EPI_NONE>(p, parts, s, 0);
+}
+
 hipError_t sgemm_tn(int R, int M, int N, int K, const float* A, int lda, const float* B, int ldb,
                     float* C, int ldc, long long strideC, float* colsum, long long stride_colsum,
                     hipStream_t s, int variant) {

@@ -72,6 +72,9 @@ hipError_t sgemm_nt(int M, int N, int K, const float* A, int lda, const float* B
                     int ldc, const float* bias, int relu, hipStream_t s, int variant);
 hipError_t sgemm_nn(int M, int N, int K, const float* A, int lda, const float* B, int ldb, float* C,
                     int ldc, const float* mask, int ldmask, hipStream_t s, int variant);
+// `parts` products without a mask, strideC apart, part r over columns [r K, (r + 1) K) of A and rows of B.
+hipError_t sgemm_nn_parts(int parts, int M, int N, int K, const float* A, int lda, const float* B, int ldb, float* C,
+                          int ldc, long long strideC, hipStream_t s);
 // colsum (may be null): colsum[r*stride_colsum + m] = sum over replica r's K rows of A[.][m]
 hipError_t sgemm_tn(int R, int M, int N, int K, const float* A, int lda, const float* B, int ldb,
                     float* C, int ldc, long long strideC, float* colsum, long long stride_colsum,

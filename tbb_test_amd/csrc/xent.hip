@@ -24,6 +24,12 @@ namespace {
 
 constexpr float LOG2E = 1.44269504088896340736f;
 
+// 16 bytes that start at any element: one load or store where the hardware's alignment rules ask for no more.
+template <class Element, class Vector>
+struct __attribute__((packed, aligned(sizeof(Element)))) Anywhere {
+  Vector v;
+};
+
 __device__ __forceinline__ float finite_or_zero(float m) { return __builtin_isinf(m) ? 0.0f : m; }
 
 // (m, s) stands for m' + log s with m' = 0 where m is infinite.  m = -inf: nothing but -inf (s = 0) or
@@ -223,7 +229,6 @@ struct EpiOut {
   struct Args {
     void* C;
     int ldc;
-    int vec;              // 16-byte stores allowed
     const float* base;    // [M][ld_base] or null; may be C
     int ld_base;          // a multiple of 64
     const float* factor;  // null: 1
@@ -272,12 +277,12 @@ struct EpiOut {
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] *= factor;
-        const bool whole = e.vec && col + 8 <= p.N;
+        const bool whole = col + 8 <= p.N;
         if constexpr (OUT_BF16) {
           u16* c = reinterpret_cast<u16*>(e.C) + at;
           if (whole) {
-            *reinterpret_cast<u32x4*>(c) = u32x4{pack16<false>(v[0], v[1]), pack16<false>(v[2], v[3]),
-                                                 pack16<false>(v[4], v[5]), pack16<false>(v[6], v[7])};
+            reinterpret_cast<Anywhere<u16, u32x4>*>(c)->v = u32x4{pack16<false>(v[0], v[1]), pack16<false>(v[2], v[3]),
+                                                                  pack16<false>(v[4], v[5]), pack16<false>(v[6], v[7])};
           } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
@@ -286,8 +291,8 @@ struct EpiOut {
         } else {
           float* c = reinterpret_cast<float*>(e.C) + at;
           if (whole) {
-            reinterpret_cast<f32x4*>(c)[0] = f32x4{v[0], v[1], v[2], v[3]};
-            reinterpret_cast<f32x4*>(c)[1] = f32x4{v[4], v[5], v[6], v[7]};
+            reinterpret_cast<Anywhere<float, f32x4>*>(c)[0].v = f32x4{v[0], v[1], v[2], v[3]};
+            reinterpret_cast<Anywhere<float, f32x4>*>(c)[1].v = f32x4{v[4], v[5], v[6], v[7]};
           } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
@@ -340,9 +345,7 @@ struct FewRows {
 template <class T, int QB, int NB, int AHEAD>
 __global__ __launch_bounds__(256) void xent_few_rows_kernel(FewRows<T> p) {
   constexpr int EACH = 16 / sizeof(T), CHUNK = 4 * EACH;  // elements of a piece, and of the four lanes of a class
-  struct __attribute__((packed, aligned(sizeof(T)))) Piece {
-    u32x4 v;
-  };
+  using Piece = Anywhere<T, u32x4>;
   __shared__ float2 red[4][16 * QB];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l16 = lane & 15, q = lane >> 4;
   const int c0 = ((int)blockIdx.x * 4 + wave) * 16 * NB;
@@ -500,16 +503,13 @@ __global__ __launch_bounds__(256) void xent_fold_kernel(const float2* __restrict
 // per lane, in one load that may start at any element.
 __global__ __launch_bounds__(256) void pack_rows_kernel(u16* __restrict__ dst, const u16* __restrict__ src, int rows, int cols,
                                                         int ld, int ldd) {
-  struct __attribute__((packed, aligned(2))) Piece {
-    u32x4 v;
-  };
   const int c = blockIdx.x * 512 + (threadIdx.x & 63) * 8;
   if (c >= ldd) return;
   for (int r = blockIdx.y * 4 + (threadIdx.x >> 6); r < rows; r += gridDim.y * 4) {
     const u16* from = src + (size_t)r * ld + c;
     u32x4 v = {0u, 0u, 0u, 0u};
     if (c + 8 <= cols) {
-      v = reinterpret_cast<const Piece*>(from)->v;
+      v = reinterpret_cast<const Anywhere<u16, u32x4>*>(from)->v;
     } else {
 #pragma unroll
       for (int k = 0; k < 8; ++k)
@@ -613,9 +613,7 @@ __global__ __launch_bounds__(256) void xent_transpose_kernel(Transposition w) {
 // wavefront takes 512 elements of a row, in 16-byte pieces (part's rows are whole ones, C's may start at any element).
 __global__ __launch_bounds__(256) void fold_slabs_kernel(float* __restrict__ C, int ldc, const float* __restrict__ part, int ldp,
                                                          long long slab, int slabs, int rows, int cols, int add) {
-  struct __attribute__((packed, aligned(4))) Piece {
-    f32x4 v;
-  };
+  using Piece = Anywhere<float, f32x4>;
   for (int r = blockIdx.y * 4 + (threadIdx.x >> 6); r < rows; r += gridDim.y * 4)
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
@@ -921,6 +919,7 @@ struct F32Plan {
   int most, piece;  // classes at a time: at most, and the largest piece in whole tiles
   bool backward;
   int splits;       // of the classes, for dX: at most
+  int w_splits;     // of the rows, for dW
   float *Xp, *Wp, *Z, *zt, *x_part, *w_part;
   float2* part;
   size_t bytes;
@@ -977,9 +976,14 @@ F32Plan plan_f32(char* base, int M, int V, int K, bool backward) {
   }
   if (backward) {
     f.x_part = c.take<float>((size_t)f.splits * f.Mp * f.Kp);
+    // Classes so few that dW has not a tile of 128 x 128 for every CU: its sum over the rows is dealt out too (2864 classes x
+    // 223 from 13056 rows: 305 -> 200 us).
+    const size_t w_tiles = up(f.piece, 128) / 128 * (up(f.Kp, 128) / 128);
+    f.w_splits = (int)std::min<size_t>(std::max<size_t>(256 / w_tiles, 1), std::max(f.Mp / 1024, 1));
+    while (f.w_splits > 1 && f.Mp % (f.w_splits * 32) != 0) --f.w_splits;
     // Where dW has no whole tiles: in whole tiles here first, or, with a sum over few rows, straight on the slower ragged
     // tiles (64 x 44992 x 1944 700 and 595 us, 300 x 20000 x 1001 538 and 549).
-    f.w_part = f.Mp > 128 ? c.take<float>((size_t)f.piece * f.Kp) : nullptr;
+    f.w_part = f.Mp > 128 ? c.take<float>((size_t)f.w_splits * f.piece * f.Kp) : nullptr;
   } else {
     f.zt = c.take<float>(M);
     f.part = c.take<float2>((size_t)M * (few ? up(V, 64) / 64 : 1));
@@ -1156,10 +1160,10 @@ hipError_t xent_backward_bf16(int M, int V, int K, const u16* X, int ldx, const 
       ld_t = padded;
     }
     const float* before = v0 > 0 ? b.x_sum : nullptr;
-    const EpiOut<true>::Args dx{dX, lddx, al16(dX) && lddx % 8 == 0, before, b.Kp, top};
+    const EpiOut<true>::Args dx{dX, lddx, before, b.Kp, top};
     void* dw = static_cast<char*>(dW) + (size_t)v0 * lddw * (dw_bf16 ? 2 : 4);
-    const EpiOut<true>::Args dw16{dw, lddw, al16(dw) && lddw % 8 == 0, nullptr, 0, top};
-    const EpiOut<false>::Args dw32{dw, lddw, al16(dw) && lddw % 4 == 0, nullptr, 0, top};
+    const EpiOut<true>::Args dw16{dw, lddw, nullptr, 0, top};
+    const EpiOut<false>::Args dw32{dw, lddw, nullptr, 0, top};
     if (together) {
       Tile16 px = product(b.G, b.ldg, wt, ld_t, M, K, steps * 64), pw = product(b.GT, b.Mp, b.Xt, b.Mp, cols, K, b.Mp);
       const int nx = (int)tile16_complete(px, b.x, nullptr), nw = (int)tile16_complete(pw, b.w, nullptr);
@@ -1169,7 +1173,7 @@ hipError_t xent_backward_bf16(int M, int V, int K, const u16* X, int ldx, const 
       continue;
     }
     if (v0 + cols < V) {
-      const EpiOut<false>::Args sum{b.x_sum, b.Kp, 1, before, b.Kp, nullptr};
+      const EpiOut<false>::Args sum{b.x_sum, b.Kp, before, b.Kp, nullptr};
       TRY(tiles<EpiOut<false>>(b.x, b.part, b.G, b.ldg, wt, ld_t, M, K, steps * 64, sum, s));
     } else {
       TRY(tiles<EpiOut<true>>(b.x, b.part, b.G, b.ldg, wt, ld_t, M, K, steps * 64, dx, s));
@@ -1254,13 +1258,14 @@ hipError_t xent_backward_f32(int M, int V, int K, const float* X, int ldx, const
       TRY(fold_slabs(dX, lddx, f.x_part, f.Kp, (long long)f.Mp * f.Kp, splits, M, K, v0 > 0, s));
     }
     float* dw = dW + (size_t)v0 * lddw;
-    if (whole(dw, lddw, cols, cols_p, K, f.Kp)) {
+    if (f.w_splits == 1 && whole(dw, lddw, cols, cols_p, K, f.Kp)) {
       TRY(sgemm_nn(cols_p, f.Kp, f.Mp, f.Z, f.Mp, X, ldx, dw, lddw, nullptr, 0, s, 0));
     } else if (f.w_part == nullptr) {
       TRY(sgemm_nn(cols, K, f.Mp, f.Z, f.Mp, X, ldx, dw, lddw, nullptr, 0, s, 0));
     } else {
-      TRY(sgemm_nn(cols_p, f.Kp, f.Mp, f.Z, f.Mp, X, ldx, f.w_part, f.Kp, nullptr, 0, s, 0));
-      TRY(fold_slabs(dw, lddw, f.w_part, f.Kp, 0, 1, cols, K, false, s));
+      const long long slab = (long long)cols_p * f.Kp;
+      TRY(sgemm_nn_parts(f.w_splits, cols_p, f.Kp, f.Mp / f.w_splits, f.Z, f.Mp, X, ldx, f.w_part, f.Kp, slab, s));
+      TRY(fold_slabs(dw, lddw, f.w_part, f.Kp, slab, f.w_splits, cols, K, false, s));
     }
   }
   return hipSuccess;

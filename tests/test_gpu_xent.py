@@ -207,7 +207,8 @@ def test_few_rows_against_many_classes(dtype, M, V, K, pad, offset):
 
 
 # pieces of whole rounds, of whole tiles and what is left over; parts of dX's sum in each
-@pytest.mark.parametrize("M,V,K", [(50, 20500, 1664), (200, 20100, 512), (130, 33000, 64), (256, 17000, 1999), (5, 9000, 3776)])
+@pytest.mark.parametrize("M,V,K", [(50, 20500, 1664), (200, 20100, 512), (130, 33000, 64), (256, 17000, 1999), (5, 9000, 3776),
+                                   (3000, 500, 64), (8000, 260, 130)])
 def test_fp32_gradients_in_pieces(M, V, K):
     p = Problem(capi.MI_F32, M, V, K)
     check_forward(p)
