@@ -1140,7 +1140,7 @@ hipError_t xent_backward_bf16(int M, int V, int K, const u16* X, int ldx, const 
       if (db) {
         const int lines = b.Mp / (shape.tile == 64 ? 16 : shape.tile / 2);  // a wavefront's rows each
         fold = ColumnFold{db + at, b.db_part + c0, b.piece, lines, n, top, (n + 63) / 64};
-        if (!together) {
+        if (!together || c0 + n < cols) {  // a part of db each; the shared launch takes the last one along
           launch_kernel(fold_columns_kernel, dim3(fold.workgroups), dim3(256), 0, s, fold);
           TRY(hipGetLastError());
         }

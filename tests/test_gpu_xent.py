@@ -555,3 +555,14 @@ def test_captured_and_replayed(dtype):
     rt.hipGraphExecDestroy(run)
     rt.hipGraphDestroy(graph)
     rt.hipStreamDestroy(stream)
+
+
+# A cut in two (a whole round of 256 x 256 tiles and some classes more) of a call so small that dX, dW and db share a
+# launch: both parts' column sums have to reach db.  In the first three the left-over classes are on 64 x 64 tiles,
+# in the last two on 128 x 128.
+@pytest.mark.parametrize("M,V,K", [(4096, 4300, 192), (4096, 4097, 128), (4300, 4300, 128), (6592, 5107, 96), (5376, 4096, 192)])
+def test_bias_gradient_of_classes_cut_in_two(M, V, K):
+    p = Problem(capi.MI_BF16, M, V, K)
+    check_forward(p)
+    check_backward(p, capi.MI_BF16)
+    check_backward(p, capi.MI_F32, dloss=False)
