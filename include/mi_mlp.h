@@ -212,8 +212,9 @@ int mi_convert_bf16_to_f32(float* dst, const void* src_bf16, size_t n, void* str
  *   z = X[M x K] * W[V x K]^T (+ bias[V])
  *   lse[i]  = log sum_j exp z_ij
  *   loss[i] = lse[i] - z_i,target[i]
- * A target outside [0, V) marks a row that does not count (padding): its loss is 0 and its gradient
- * zero, and it adds nothing to dW and dbias, whatever X and dloss hold there; its lse is still written.
+ * A target outside [0, V) marks a row that does not count (padding): its loss is 0 and its row of dX
+ * zero, whatever W holds, and it adds nothing to dW and dbias, whatever X and dloss hold there; its lse is
+ * still written.
  * Infinite logits mean what they mean in the formula: -inf (a bias of -inf, say) is a class of
  * probability zero, +inf or NaN makes the row's lse +inf or NaN.
  * Stands beside mi_l2_loss_static; no counterpart in the reference, whose harness has the L2 loss only.

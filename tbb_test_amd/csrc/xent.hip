@@ -220,10 +220,12 @@ struct EpiGrad : NoPre {
   }
 };
 
-// C = factor * (base + A B^T), fp32 or bf16; rows and columns behind the result are dropped.
+// C = factor * (base + A B^T), fp32 or bf16; rows and columns behind the result are dropped.  DX: rows that do not count
+// become zeros (their g is zero, but zero times an infinity or NaN of W is not); the other results' epilogues are left
+// without that (a run-time test takes 4 us of the 27 of dW of 32000 classes x 1024 from one row).
 // dW of 32768 classes x 4096 from 8192 rows: 1.59 ms, 1385 TFLOP/s; dX from 32768 classes 1.68 ms (rows of a caller's Wt
 // a power of two apart share memory channels).
-template <bool OUT_BF16>
+template <bool OUT_BF16, bool DX = false>
 struct EpiOut {
   static constexpr bool MAY_SPLIT = true;
   struct Args {
@@ -232,14 +234,21 @@ struct EpiOut {
     const float* base;    // [M][ld_base] or null; may be C
     int ld_base;          // a multiple of 64
     const float* factor;  // null: 1
+    const int* target;    // DX only
+    int vocab;
   };
   template <int QB>
   struct Pre {
+    int target[DX ? QB : 1];
     f32x4 base[QB][2][2];
   };
   template <int QB>
   static __device__ __forceinline__ Pre<QB> before(const Args& e, const Tile16& p, int row0, int colw, int lane, int) {
     Pre<QB> v;
+    if constexpr (DX) {
+#pragma unroll
+      for (int jq = 0; jq < QB; ++jq) v.target[jq] = e.target[min(row0 + 16 * jq + (lane & 15), p.M - 1)];
+    }
     if (!e.base) return v;
 #pragma unroll
     for (int jq = 0; jq < QB; ++jq)
@@ -263,6 +272,8 @@ struct EpiOut {
     for (int jq = 0; jq < QB; ++jq) {
       const int row = row0 + 16 * jq + l16;
       if (row >= p.M) continue;
+      bool counts = true;
+      if constexpr (DX) counts = pre.target[jq] >= 0 && pre.target[jq] < e.vocab;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int col = col0 + 32 * h;
@@ -276,7 +287,7 @@ struct EpiOut {
           for (int i = 0; i < 8; ++i) v[i] += pre.base[jq][h][i >> 2][i & 3];
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] *= factor;
+        for (int i = 0; i < 8; ++i) v[i] = counts ? v[i] * factor : 0.0f;
         const bool whole = col + 8 <= p.N;
         if constexpr (OUT_BF16) {
           u16* c = reinterpret_cast<u16*>(e.C) + at;
@@ -609,12 +620,15 @@ __global__ __launch_bounds__(256) void xent_transpose_kernel(Transposition w) {
   transpose_tile(w, blockIdx.x, tile);
 }
 
-// C[row][col] = sum over slabs, in slab order, of part[slab][row][col], on top of what C holds where `add`.  A
-// wavefront takes 512 elements of a row, in 16-byte pieces (part's rows are whole ones, C's may start at any element).
+// C[row][col] = sum over slabs, in slab order, of part[slab][row][col], on top of what C holds where `add`; zeros in rows
+// that do not count.  A wavefront takes 512 elements of a row, in 16-byte pieces (part's rows are whole ones, C's may
+// start at any element).
 __global__ __launch_bounds__(256) void fold_slabs_kernel(float* __restrict__ C, int ldc, const float* __restrict__ part, int ldp,
-                                                         long long slab, int slabs, int rows, int cols, int add) {
+                                                         long long slab, int slabs, int rows, int cols, int add,
+                                                         const int* __restrict__ target, int vocab) {
   using Piece = Anywhere<float, f32x4>;
-  for (int r = blockIdx.y * 4 + (threadIdx.x >> 6); r < rows; r += gridDim.y * 4)
+  for (int r = blockIdx.y * 4 + (threadIdx.x >> 6); r < rows; r += gridDim.y * 4) {
+    const bool counts = row_counts(target, vocab, r);
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       const int c = blockIdx.x * 512 + 256 * k + 4 * (threadIdx.x & 63);
@@ -629,11 +643,20 @@ __global__ __launch_bounds__(256) void fold_slabs_kernel(float* __restrict__ C, 
           if (c + i < cols) v[i] = dst[i];
 #pragma unroll 4
       for (int n = 0; n < slabs; ++n) v += *reinterpret_cast<const f32x4*>(src + (size_t)n * slab);
+      if (!counts) v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
       if (whole) reinterpret_cast<Piece*>(dst)->v = v;
       else
         for (int i = 0; i < 4; ++i)
           if (c + i < cols) dst[i] = v[i];
     }
+  }
+}
+// Zeros in the rows of C that do not count: where a GEMM writes dX itself.  C has whole tiles: 16-byte rows, cols a multiple of 32.
+__global__ __launch_bounds__(256) void clear_rows_kernel(float* __restrict__ C, int ldc, int rows, int cols, const int* __restrict__ target,
+                                                         int vocab) {
+  const int r = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (r >= rows || row_counts(target, vocab, r)) return;
+  for (int c = 4 * (threadIdx.x & 63); c < cols; c += 256) *reinterpret_cast<f32x4*>(C + (size_t)r * ldc + c) = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 }
 // out[c] = factor * sum over lines of part[line][c].  64 columns per workgroup, four groups of lines added up in order.
 struct ColumnFold {
@@ -817,8 +840,9 @@ inline bool al16(const void* q) { return (reinterpret_cast<uintptr_t>(q) & 15) =
 // Workgroups of four wavefronts, 512 columns of a row each.
 inline dim3 row_grid(int rows, int cols) { return dim3((cols + 511) / 512, std::min((rows + 3) / 4, 16384)); }
 hipError_t fold_slabs(float* C, int ldc, const float* part, int ldp, long long slab, int slabs, int rows, int cols, bool add,
-                      hipStream_t s) {
-  launch_kernel(fold_slabs_kernel, row_grid(rows, cols), dim3(256), 0, s, C, ldc, part, ldp, slab, slabs, rows, cols, (int)add);
+                      const int* target, int vocab, hipStream_t s) {
+  launch_kernel(fold_slabs_kernel, row_grid(rows, cols), dim3(256), 0, s, C, ldc, part, ldp, slab, slabs, rows, cols, (int)add, target,
+                vocab);
   return hipGetLastError();
 }
 
@@ -1011,10 +1035,10 @@ Transposition transposition(u16* dst, const u16* src, int rows, int cols, int ld
 }
 
 template <class EpiW>
-hipError_t launch_products(const Tile16& px, const EpiOut<true>::Args& ex, int nx, const Tile16& pw, const typename EpiW::Args& ew, int nw,
+hipError_t launch_products(const Tile16& px, const EpiOut<true, true>::Args& ex, int nx, const Tile16& pw, const typename EpiW::Args& ew, int nw,
                            const ColumnFold& db, hipStream_t s) {
   using Ring = TileKernel<64, 64, 4, 1, 4>;
-  auto kern = xent_products_kernel<EpiOut<true>, EpiW>;
+  auto kern = xent_products_kernel<EpiOut<true, true>, EpiW>;
   static LdsOptIn opt_in;
   TRY(opt_in.ensure(reinterpret_cast<const void*>(kern), Ring::LDS));
   launch_kernel(kern, dim3(nx + nw + db.workgroups), dim3(256), Ring::LDS, s, px, ex, nx, pw, ew, nw, db);
@@ -1160,7 +1184,7 @@ hipError_t xent_backward_bf16(int M, int V, int K, const u16* X, int ldx, const 
       ld_t = padded;
     }
     const float* before = v0 > 0 ? b.x_sum : nullptr;
-    const EpiOut<true>::Args dx{dX, lddx, before, b.Kp, top};
+    const EpiOut<true, true>::Args dx{dX, lddx, before, b.Kp, top, target, V};
     void* dw = static_cast<char*>(dW) + (size_t)v0 * lddw * (dw_bf16 ? 2 : 4);
     const EpiOut<true>::Args dw16{dw, lddw, nullptr, 0, top};
     const EpiOut<false>::Args dw32{dw, lddw, nullptr, 0, top};
@@ -1176,7 +1200,7 @@ hipError_t xent_backward_bf16(int M, int V, int K, const u16* X, int ldx, const 
       const EpiOut<false>::Args sum{b.x_sum, b.Kp, before, b.Kp, nullptr};
       TRY(tiles<EpiOut<false>>(b.x, b.part, b.G, b.ldg, wt, ld_t, M, K, steps * 64, sum, s));
     } else {
-      TRY(tiles<EpiOut<true>>(b.x, b.part, b.G, b.ldg, wt, ld_t, M, K, steps * 64, dx, s));
+      TRY((tiles<EpiOut<true, true>>(b.x, b.part, b.G, b.ldg, wt, ld_t, M, K, steps * 64, dx, s)));
     }
     // dW = g^T X
     if (dw_bf16) TRY(tiles<EpiOut<true>>(b.w, b.part, b.GT, b.Mp, b.Xt, b.Mp, cols, K, b.Mp, dw16, s));
@@ -1254,8 +1278,11 @@ hipError_t xent_backward_f32(int M, int V, int K, const float* X, int ldx, const
     float* dx = dx_direct ? dX : f.x_part;
     TRY(sgemm_tn(splits, f.Mp, f.Kp, cols_p / splits, f.Z, f.Mp, w, ld_w, dx, dx_direct ? lddx : f.Kp, (long long)f.Mp * f.Kp,
                  nullptr, 0, s, 0));
-    if (!dx_direct) {
-      TRY(fold_slabs(dX, lddx, f.x_part, f.Kp, (long long)f.Mp * f.Kp, splits, M, K, v0 > 0, s));
+    if (dx_direct) {
+      launch_kernel(clear_rows_kernel, dim3((M + 3) / 4), dim3(256), 0, s, dX, lddx, M, K, target, V);
+      TRY(hipGetLastError());
+    } else {
+      TRY(fold_slabs(dX, lddx, f.x_part, f.Kp, (long long)f.Mp * f.Kp, splits, M, K, v0 > 0, target, V, s));
     }
     float* dw = dW + (size_t)v0 * lddw;
     if (f.w_splits == 1 && whole(dw, lddw, cols, cols_p, K, f.Kp)) {
@@ -1265,7 +1292,7 @@ hipError_t xent_backward_f32(int M, int V, int K, const float* X, int ldx, const
     } else {
       const long long slab = (long long)cols_p * f.Kp;
       TRY(sgemm_nn_parts(f.w_splits, cols_p, f.Kp, f.Mp / f.w_splits, f.Z, f.Mp, X, ldx, f.w_part, f.Kp, slab, s));
-      TRY(fold_slabs(dw, lddw, f.w_part, f.Kp, slab, f.w_splits, cols, K, false, s));
+      TRY(fold_slabs(dw, lddw, f.w_part, f.Kp, slab, f.w_splits, cols, K, false, nullptr, 0, s));
     }
   }
   return hipSuccess;

@@ -566,3 +566,27 @@ def test_bias_gradient_of_classes_cut_in_two(M, V, K):
     check_forward(p)
     check_backward(p, capi.MI_BF16)
     check_backward(p, capi.MI_F32, dloss=False)
+
+
+# (M, V, K) by how dX is written: one launch for all results, tiles of one piece, sums over several pieces (2^27 / 16384 = 8192
+# classes each), fp32 sums folded, fp32 products straight into dX
+@pytest.mark.parametrize("dtype,M,V,K", [(capi.MI_BF16, 20, 300, 64), (capi.MI_BF16, 300, 700, 2048), (capi.MI_BF16, 16, 8300, 16384),
+                                         (capi.MI_F32, 20, 300, 64), (capi.MI_F32, 1024, 256, 4096), (capi.MI_F32, 1000, 256, 4096)])
+def test_rows_that_do_not_count_have_a_zero_gradient_whatever_the_weights_hold(dtype, M, V, K):
+    dead = [0, 5, M // 2, M - 1]
+
+    def tweak(X, W, b, t, d):
+        t[dead] = [-100, V, -1, 2 ** 31 - 1]
+        W[7, 3] = np.inf
+        W[V - 1, 0] = np.nan
+    with np.errstate(all="ignore"):
+        p = Problem(dtype, M, V, K, tweak=tweak, ignored=0.0)
+    p.forward()
+    p.make_outputs(dtype)
+    for use_wt in (True, False):
+        p.backward(use_wt)
+        capi.check(capi.lib().mi_stream_sync(None))
+        gX = widen(p.gX.get()) if p.bf16 else p.gX.get()
+        assert np.all(gX[dead] == 0.0)
+        alive = np.setdiff1d(np.arange(M), dead + ([3] if M > 4 else []))  # (row 3 of a Problem has the target V)
+        assert np.all(np.isnan(gX[alive]).any(1))  # a NaN logit makes lse NaN, and that every element of the row's g
