@@ -216,7 +216,7 @@ int mi_convert_bf16_to_f32(float* dst, const void* src_bf16, size_t n, void* str
  * zero, whatever W holds, and it adds nothing to dW and dbias, whatever X and dloss hold there; its lse is
  * still written.
  * Infinite logits mean what they mean in the formula: -inf (a bias of -inf, say) is a class of
- * probability zero, +inf or NaN makes the row's lse +inf or NaN.
+ * probability zero, +inf or NaN makes the row's lse +inf or NaN, and a target of +inf its loss NaN.
  * Stands beside mi_l2_loss_static; no counterpart in the reference, whose harness has the L2 loss only.
  *   dtype MI_BF16: X and W bf16, MFMA products with fp32 accumulation; MI_F32: X and W fp32.
  *   bias, loss, lse, dloss, dbias: fp32.  target: 32-bit integers.  bias may be NULL.

@@ -52,7 +52,8 @@ __device__ __forceinline__ void finish_row(float m, float s, bool counts, float 
   }
   const float d = others - zt;
   const float tail = log1pf(expf(-fabsf(d)));
-  *loss = fmaxf(d, 0.0f) + tail;  // d = NaN: the tail is NaN
+  // d = NaN: the tail is NaN; z_t = inf: lse - z_t is inf - inf, where the other form would make it 0
+  *loss = zt == __builtin_inff() ? __builtin_nanf("") : fmaxf(d, 0.0f) + tail;
   *lse = others == zt && __builtin_isinf(zt) ? zt : fmaxf(others, zt) + tail;
 }
 

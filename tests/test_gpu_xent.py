@@ -590,3 +590,39 @@ def test_rows_that_do_not_count_have_a_zero_gradient_whatever_the_weights_hold(d
         assert np.all(gX[dead] == 0.0)
         alive = np.setdiff1d(np.arange(M), dead + ([3] if M > 4 else []))  # (row 3 of a Problem has the target V)
         assert np.all(np.isnan(gX[alive]).any(1))  # a NaN logit makes lse NaN, and that every element of the row's g
+
+
+@pytest.mark.parametrize("dtype", [capi.MI_BF16, capi.MI_F32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("M,V,K", [(12, 300, 64), (12, 4400, 70), (300, 513, 64)])  # tiles, few rows, tiles of fp32 models
+def test_an_infinite_logit_of_the_target_is_no_small_loss(dtype, M, V, K):
+    """loss = lse - z_t: inf - inf is NaN, as the gradient is; the other rows lose infinitely much."""
+    def tweak(X, W, b, t, d):
+        b[9] = np.inf
+        t[:] = 8
+        t[::3] = 9
+        t[5] = -1
+    with np.errstate(all="ignore"):
+        p = Problem(dtype, M, V, K, tweak=tweak, ignored=0.0)
+    p.forward()
+    capi.check(capi.lib().mi_stream_sync(None))
+    loss, lse = p.loss.get()[0], p.lse.get()[0]
+    want = np.full(M, np.inf)
+    want[p.t == 9] = np.nan
+    want[p.t == -1] = 0.0
+    assert np.array_equal(loss, want, equal_nan=True)
+    assert np.all(lse == np.inf)
+
+
+@pytest.mark.parametrize("dtype", [capi.MI_BF16, capi.MI_F32], ids=["bf16", "f32"])
+def test_the_only_class_left_costs_nothing(dtype):
+    def tweak(X, W, b, t, d):
+        b[:] = -np.inf
+        b[4] = 0.5
+        t[:] = 4
+    with np.errstate(all="ignore"):
+        p = Problem(dtype, 9, 300, 64, tweak=tweak, ignored=0.0)
+    p.forward()
+    p.make_outputs(dtype)
+    p.backward()
+    capi.check(capi.lib().mi_stream_sync(None))
+    assert not p.loss.get().any() and not p.gX.get().any() and not p.gW.get().any() and not p.gb.get().any()
