@@ -626,3 +626,39 @@ def test_the_only_class_left_costs_nothing(dtype):
     p.backward()
     capi.check(capi.lib().mi_stream_sync(None))
     assert not p.loss.get().any() and not p.gX.get().any() and not p.gW.get().any() and not p.gb.get().any()
+
+
+class FarRows:
+    """A matrix whose rows lie `ld` elements apart, nothing between them touched from the host."""
+
+    def __init__(self, values, ld):
+        self.values, self.ld = np.ascontiguousarray(values), ld
+        size = self.values.dtype.itemsize
+        self.buf = capi.DeviceBuffer(((len(values) - 1) * ld + values.shape[1]) * size)
+        self.ptr, self.step = self.buf.ptr, ld * size
+        for i, row in enumerate(self.values):
+            capi.check(capi.lib().mi_memcpy_h2d(self.ptr + i * self.step, row.ctypes.data_as(ctypes.c_void_p), row.nbytes))
+
+    def get(self):
+        out = np.empty_like(self.values)
+        for i in range(len(out)):
+            capi.check(capi.lib().mi_memcpy_d2h(out[i].ctypes.data_as(ctypes.c_void_p), self.ptr + i * self.step, out[i].nbytes))
+        return out
+
+
+@pytest.mark.parametrize("dtype", [capi.MI_BF16, capi.MI_F32], ids=["bf16", "f32"])
+def test_far_rows_of_more_than_128_rows_of_x(dtype):
+    """As test_rows_so_far_apart_that_a_tile_passes_32_bits, with so many rows of X that an fp32 dW comes out of dense tiles
+    (up to 128 the product writes dW itself)."""
+    p = Problem(dtype, 256, 192, 64)
+    check_forward(p)
+    check_backward(p, dtype)
+    dense = [x.get() for x in (p.loss, p.lse, p.gX, p.gW, p.gb)]
+    p.dW_, p.gW = FarRows(p.dW_.get(), 9 << 20), FarRows(np.full((p.V, p.K), 7, p.dW_.dtype), 9 << 20)
+    p.loss, p.lse = Strided(1, p.M, p.M, 0, np.float32), Strided(1, p.M, p.M, 0, np.float32)
+    p.gX, p.gb = Strided(p.M, p.K, p.K, 0, p.dX_.dtype), Strided(1, p.V, p.V, 0, np.float32)
+    p.forward()
+    p.backward()
+    capi.check(capi.lib().mi_stream_sync(None))
+    for a, b in zip(dense, [x.get() for x in (p.loss, p.lse, p.gX, p.gW, p.gb)]):
+        assert np.array_equal(a, b)
