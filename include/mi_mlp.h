@@ -220,8 +220,11 @@ int mi_convert_bf16_to_f32(float* dst, const void* src_bf16, size_t n, void* str
  * Stands beside mi_l2_loss_static; no counterpart in the reference, whose harness has the L2 loss only.
  *   dtype MI_BF16: X and W bf16, MFMA products with fp32 accumulation; MI_F32: X and W fp32.
  *   bias, loss, lse, dloss, dbias: fp32.  target: 32-bit integers.  bias may be NULL.
- *   M, V, K: 1 .. 2097152.  Any strides and alignment of the element type; 16-byte aligned rows and
- *   K a multiple of 64 are read in place, others are copied into the workspace first.
+ *   M, V, K: 1 .. 2097152.  Any strides and alignment of the element type.  Read in place are operands
+ *   with 16-byte aligned rows at most 4194304 elements apart and K a multiple of 64, of fp32 models as far as
+ *   M and V make whole tiles (of 128, below 128 rows or classes of 32), and W of a forward call of few rows
+ *   (up to 64 bf16, 32 fp32, against 4096 classes and more) wherever it starts.  The rest is copied into the
+ *   workspace first, X also where such a call reads W in place and in every backward call of an fp32 model.
  * workspace: device memory, 256-byte aligned, at least what mi_xent_workspace says for the same dtype,
  * M, V and K.  Its contents do not matter before a call and mean nothing after it; calls that may run
  * at the same time need one each.  Nothing is allocated and nothing synchronises, so a call can be
@@ -240,9 +243,9 @@ int mi_xent_forward(int dtype, int M, int V, int K, const void* X, int ldx, cons
  * All three results are written, not added to; dbias may be NULL.  The outputs may not overlap the inputs.
  * Wt (MI_BF16 only, may be NULL): W^T [K x V] with leading dimension ldwt, the copy that
  * mi_reduce_sgd_bf16t_raw and mi_ortho_update_raw write; without it, or where its rows are not 16-byte
- * aligned, the call makes the copy itself, piece by piece.
+ * aligned or a piece of the classes is no multiple of 64, the call makes the copy itself, piece by piece.
  * dX has the dtype of X.  dW is bf16 (dw_dtype = MI_BF16) or fp32 (MI_F32; always for MI_F32 models).
- * bf16: g is rounded to bf16 (half a step, 2^-9 of each term) before the two products that read it,
+ * bf16: g is rounded to bf16 (half a step, at most 2^-8 of each term) before the two products that read it,
  * like every dY of the framework's bf16 models; dbias is summed before that rounding.
  */
 int mi_xent_backward(int dtype, int M, int V, int K, const void* X, int ldx, const void* W, int ldw,
@@ -260,7 +263,11 @@ int mi_xent_backward(int dtype, int M, int V, int K, const void* X, int ldx, con
  * (on the transposed matrix where rows > cols), which leaves singular values of G that are not tiny
  * against |G|_F between about 0.7 and 1.2.  `batch` matrices of one shape, strideG / strideO elements
  * apart; G is fp32 (in_dtype = MI_F32) or bf16, O is bf16.  The products run in fp16 with fp32
- * accumulation and the iterate is kept to 22 bits: O is off by 2e-4 .. 8e-4 of |O|_F before its rounding.
+ * accumulation and the iterate is kept to 22 bits, for fp32 gradients too.  After 5 steps O is off by
+ * 3e-4 .. 1.2e-3 of |O|_F before its rounding, from 64 rows and columns on.  The polynomial's slope is -1.6 near
+ * 0.87, so that each step makes the errors of singular values there larger, whatever the precision: a
+ * matrix with few of them can be off by several 1e-2 (2 x 2, one in a hundred by more than 5e-3), and after 16 steps
+ * 2e-3 .. 5e-3 are ordinary and 1e-1 happens.
  * G = 0 gives O = 0; a G with an infinity or NaN gives NaN throughout.  O may be G itself (bf16, same
  * strides).  rows, cols: 1 .. 65536, batch: 1 .. 4096.
  * workspace as for mi_xent_forward, sized by mi_ortho_workspace for the same batch, rows and cols.
@@ -276,8 +283,10 @@ int mi_orthogonalize(int in_dtype, int batch, int rows, int cols, const void* G,
  *   W <- (1 - lr decay) W - lr scale O
  * and, unless NULL, W_bf16 = W and Wt_bf16 = W^T rounded to bf16: what mi_reduce_sgd_bf16t_raw is for
  * plain SGD.  Every matrix is dense [rows x cols] (Wt_bf16 [cols x rows]); consecutive ones are
- * layer_stride elements apart in W, W_bf16, Wt_bf16, momentum and each replica of G alike, the layout
- * of the parameter arena of a model with equal layers.  momentum: zeros before the first call.
+ * layer_stride elements apart in W, W_bf16, Wt_bf16, momentum and each replica of G alike: equal layers
+ * of a caller's arena W_0 | b_0 | W_1 | b_1 ... (a handle's own arenas are reached by its own calls only).
+ * momentum: zeros before the first call.  The error of O reaches W times lr scale (an update of root mean
+ * square 2e-4 on weights of 0.03: 2e-6 of |W|_F); there is no form with fp32 products.
  * scale is the caller's convention for the step length, e.g. 0.2 sqrt(max(rows, cols)) for an update
  * of root mean square 0.2 lr, or sqrt(max(1, rows / cols)).
  */

@@ -12,8 +12,14 @@
 // X is kept to 22 bits, because the a X term carries every direction from one iteration to the next and
 // grows small ones 3.4 times each: with the fp16 operand in that term its white rounding noise grows along
 // (4e-2 for a floor of 1e-2).  The diagonals of A, near 1, and of b A + c A^2, near b + c, stay in fp32 and out of
-// the products: their rounding would be most of what is left.  Together: 2e-4 .. 4e-4 of |O| on flat and
-// mixed spectra, 8e-4 on steep ones.
+// the products: their rounding would be most of what is left.  Together, after five steps: 3e-4 of |O| (200 x 2000,
+// flat) .. 8e-4 (256 x 256 and 200 x 2000, steep) .. 1.2e-3 (64 x 64, steep).  p(s) = a s + b s^3 + c s^5 has the
+// slope -1.6 at its fixed point 0.87, so an error of a singular value near there grows by that with each step until it
+// has settled on the cycle around it: fp32 products start from 1e-6 and grow by the same factors.  Many singular values
+// average that out, few do not (2 x 2: 1e-3 at the median, 5e-3 .. 2.5e-2 at the 99th of 100, 6e-2 seen), nor do
+// many steps (16 steps: 2e-3 .. 5e-3 at the median, 2e-2 .. 3e-1 at the 99th of 100 up to 64 x 64).
+// fp16 for fp32 gradients and weights too: fp32 products run at a tenth of the rate, and the direction that a
+// stochastic gradient's momentum gives is not known to 1e-3.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -199,7 +205,7 @@ __global__ __launch_bounds__(256) void ortho_scale_kernel(const float* __restric
 // ---- the products -----------------------------------------------------------------------------------
 
 // A = X X^T without its diagonal (times GRAM_SCALE, fp16): a tile of the lower triangle and its mirror image; the
-// diagonal in fp32.  Bound by the MFMAs: 8192 x 8192 433 us for half of the product, 1270 TFLOP/s; 8 x 1024 x 1024 20 us,
+// diagonal in fp32.  Bound by the MFMAs: 8192 x 8192 429 us for half of the product, 1280 TFLOP/s; 8 x 1024 x 1024 17.5 us,
 // 36 tiles of 128 x 128 on the 32 CUs of an XCD.
 struct EpiGram : NoPre {
   static constexpr bool MAY_SPLIT = true;
@@ -242,8 +248,8 @@ struct EpiGram : NoPre {
 };
 
 // P = b A + c A A without its diagonal (times GRAM_SCALE, fp16), the diagonal in fp32.  With A = A' + D, D its
-// diagonal: P = c A' A' + b A' + c (D A' + A' D) off the diagonal, and b D + c (A' A' + D D) on it.  As fast as the
-// one above (449 and 23 us).
+// diagonal: P = c A' A' + b A' + c (D A' + A' D) off the diagonal, and b D + c (A' A' + D D) on it.  About as fast
+// as the one above (446 and 20 us).
 struct EpiPoly {
   static constexpr bool MAY_SPLIT = true;
   struct Args {
@@ -315,8 +321,8 @@ struct EpiPoly {
 };
 
 // X <- (a + diag) X + P X, in place, and the first half's transpose for the next iteration (null: last one).  8192 x 8192:
-// 902 us, 1220 TFLOP/s, of which the ten bytes an element take 0.1 ms; 8 x 1024 x 1024: 30 us, half of them those bytes
-// (17 MB in 3 us, and no K loop left to hide them behind).
+// 902 us, 1220 TFLOP/s, of which the ten bytes an element take 0.1 ms; 8 x 1024 x 1024: 28 us, half of them those bytes:
+// one round of 512 workgroups, two per CU, that all load, multiply and store at the same times.
 struct EpiStep {
   static constexpr bool MAY_SPLIT = true;
   struct Args {

@@ -8,7 +8,7 @@
 // a fold joins them.  The target is kept apart because lse - z_t cancels where a row is sure of its
 // answer; with o = log sum over the others, loss = softplus(o - z_t) does not.
 // Backward, bf16: the vocabulary is walked in pieces.  Per piece the tiles of z are computed again and
-// leave as g (rounded to bf16, the operand type of the products that follow: half a step of 2^-8 per
+// leave as g (rounded to bf16, the operand type of the products that follow: at most 2^-8 of each
 // term) in both orders that the next two products read, g for dX += g W and g^T for dW = g^T X.
 // fp32 models: the same pieces through the framework's fp32 GEMMs, with the softmax between them.
 #include <hip/hip_runtime.h>
@@ -911,7 +911,8 @@ BackwardPlan plan_backward(char* base, int M, int V, int K) {
   BackwardPlan b{};
   Carver c{base};
   b.Kp = (int)up(K, 64);
-  // g and g^T of a piece take at most 2 x 512 MB, the copies of W's piece 256 MB each
+  // g and g^T of a piece take 2 x 512 MB, the copies of W's piece 256 MB each, or what 256 classes take where that is
+  // more (from 2^20 rows or K = 2^19 on: 2.4 GB of g at 2^21 rows)
   const size_t most = std::min(((size_t)1 << 28) / up(M, 256), ((size_t)1 << 27) / b.Kp) / 256 * 256;
   const size_t widest = std::max<size_t>(most, 256);
   const Cut cut = cut_classes(M, (int)std::min<size_t>(V, widest), b.Kp);
