@@ -264,7 +264,7 @@ int mi_xent_backward(int dtype, int M, int V, int K, const void* X, int ldx, con
  * against |G|_F between about 0.7 and 1.2.  `batch` matrices of one shape, strideG / strideO elements
  * apart; G is fp32 (in_dtype = MI_F32) or bf16, O is bf16.  The products run in fp16 with fp32
  * accumulation and the iterate is kept to 22 bits, for fp32 gradients too.  After 5 steps O is off by
- * 3e-4 .. 1.2e-3 of |O|_F before its rounding, from 64 rows and columns on.  The polynomial's slope is -1.6 near
+ * 2e-4 .. 1.2e-3 of |O|_F before its rounding, from 64 rows and columns on.  The polynomial's slope is -1.6 near
  * 0.87, so that each step makes the errors of singular values there larger, whatever the precision: a
  * matrix with few of them can be off by several 1e-2 (2 x 2, one in a hundred by more than 5e-3), and after 16 steps
  * 2e-3 .. 5e-3 are ordinary and 1e-1 happens.
@@ -285,8 +285,8 @@ int mi_orthogonalize(int in_dtype, int batch, int rows, int cols, const void* G,
  * plain SGD.  Every matrix is dense [rows x cols] (Wt_bf16 [cols x rows]); consecutive ones are
  * layer_stride elements apart in W, W_bf16, Wt_bf16, momentum and each replica of G alike: equal layers
  * of a caller's arena W_0 | b_0 | W_1 | b_1 ... (a handle's own arenas are reached by its own calls only).
- * momentum: zeros before the first call.  The error of O reaches W times lr scale (an update of root mean
- * square 2e-4 on weights of 0.03: 2e-6 of |W|_F); there is no form with fp32 products.
+ * momentum: zeros before the first call.  The error of O reaches W times lr scale (updates of root mean
+ * square 2e-4 on weights of 1 / sqrt(cols): 3e-7 .. 5e-6 of |W|_F); there is no form with fp32 products.
  * scale is the caller's convention for the step length, e.g. 0.2 sqrt(max(rows, cols)) for an update
  * of root mean square 0.2 lr, or sqrt(max(1, rows / cols)).
  */
